@@ -679,6 +679,81 @@ int tcvom_flow_crop_resize(const float* src, float* dst, int32_t F, int32_t Hs, 
 int tcvom_pad_bottom_right(const float* src, float* dst, int32_t S, int32_t C, int32_t H, int32_t W, int32_t Ho, int32_t Wo,
                            const float* value, void* stream);
 
+/* ------------------------------------------------------------------ token operators
+ * Attention with a learned relative position bias and the norms around a block, for token sequences (frames of a clip, the pixels of a
+ * stride-8 / -16 map): beside the Temporal Attention Module and GuidedCxtAtten, which know no positions, and BatchNorm / GroupNorm, which
+ * normalise over pixels.  The reference has no counterpart.  Element types are arguments here, in both builds: */
+#define TCVOM_TYPE_F32 0
+#define TCVOM_TYPE_BF16 1
+#define TCVOM_TYPE_F16 2
+
+/* Buckets of the relative position rel = key position - query position.  Distance d = |rel| (bidirectional: the second half of the
+ * buckets is for rel > 0) or max(-rel, 0) (one-sided); d < exact has bucket d, bucket exact + k starts at distance starts[k]
+ * (starts[0] = exact, never decreasing), the last bucket of a side holds every longer distance.  A HOST struct. */
+#define TCVOM_MAX_BUCKETS 256
+#define TCVOM_MAX_BUCKET_STARTS 128
+#define TCVOM_MAX_BUCKET_REACH 1024
+typedef struct {
+    int32_t num_buckets, bidirectional, exact, n_starts;
+    int32_t starts[TCVOM_MAX_BUCKET_STARTS];
+} tcvom_rel_buckets;
+
+/* out[h][i][j] = table[bucket(j - i - q_start)][h]: table fp32 [num_buckets][heads], out [heads][q_len][k_len] of `type`.
+ * _bwd: dtable[b][h] = sum of dout over the elements with that bucket; work = tcvom_relbias_bwd_work(...) floats.  Fixed order of
+ * additions: equal calls give equal bits. */
+int tcvom_relbias_fwd(const float* table, void* out, const tcvom_rel_buckets* buckets, int32_t heads, int64_t q_len, int64_t k_len,
+                      int64_t q_start, int32_t type, void* stream);
+int64_t tcvom_relbias_bwd_work(const tcvom_rel_buckets* buckets, int32_t heads, int64_t q_len);
+int tcvom_relbias_bwd(const void* dout, float* dtable, float* work, int64_t work_floats, const tcvom_rel_buckets* buckets, int32_t heads,
+                      int64_t q_len, int64_t k_len, int64_t q_start, int32_t type, void* stream);
+
+/* Attention that adds the bias inside: q [B][Nq][H][D], k / v [B][Nk][Hkv][D] (bf16 or fp16; the innermost stride is 1, the others in
+ * elements and multiples of 8; H % Hkv == 0: consecutive heads share keys), out [B][Nq][H][D] contiguous:
+ *     out[b,i,h] = sum_j softmax_j( scale <q[b,i,h], k[b,j,h Hkv / H]> + table[bucket(j - i - q_start_b)][h] ) v[b,j,h Hkv / H]
+ * over the keys j < k_lens[b] (NULL: Nk) with key_mask[b][j] != 0 (NULL: all) and, causal, j <= i + q_start_b (q_starts[b], NULL: q_start).
+ * A row without such a key is zero; what lies behind the lengths and under the mask is not looked at.  A HOST struct. */
+typedef struct {
+    int32_t B, Nq, Nk, H, Hkv, D, type, causal, q_start;
+    float scale;                 /* > 0 */
+    int64_t q_stride[3], k_stride[3], v_stride[3];      /* batch, token, head */
+    const int32_t *k_lens, *q_starts;
+    const uint8_t* key_mask;
+    tcvom_rel_buckets buckets;
+} tcvom_attn_desc;
+/* lse (or NULL): fp32 [B][H][Nq], log2 of the row's sum of exponentials, -inf for an empty row.  out_lo (or NULL): what rounding out to
+ * 16 bits dropped, in 16 bits; asking for it also carries the probabilities in twice the bits (the backward's <dout, out> then is
+ * good to 2^-16, which the table's gradient, a sum of differences, needs).  work: tcvom_attn_fwd_work floats. */
+int64_t tcvom_attn_fwd_work(const tcvom_attn_desc* d);
+int tcvom_attn_fwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, void* out, void* out_lo,
+                   float* lse, float* work, int64_t work_floats, void* stream);
+/* Gradients from what the forward read and wrote (lse required); dout with strides like q's; dq / dk / dv contiguous, dtable (or NULL:
+ * not asked for) fp32 like table.  Keys and rows without a pair get zeros.  Fixed order of additions. */
+int64_t tcvom_attn_bwd_work(const tcvom_attn_desc* d);
+int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, const void* out,
+                   const void* out_lo, const float* lse, const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv,
+                   float* dtable, float* work, int64_t work_floats, void* stream);
+
+/* Norms around a block, T tokens of C <= 8192 channels, contiguous:
+ *     x_out = residual_scale x + branch_scale g N(y; post),   h = N(x_out; pre)        (h from the unrounded x_out)
+ * N = RMSNorm (layer = 0, no bias) or LayerNorm (layer = 1), weights fp32; a null post_weight leaves y as it is, a null pre_weight
+ * leaves h out, a null y gives h = N(x; pre) alone.  x / x_out of x_type, y / h of y_type: equal types, or fp32 with a 16-bit one.
+ * gate (or null): [T / gate_rows][C] fp32 (gate_f32) or y_type, token t uses row t / gate_rows.  stats: fp32 [T][4] for the backward
+ * (or null).
+ * _bwd: dx_out / dh are the two incoming gradients (either may be null); the gradients of the weights, the biases and the gate are
+ * written where their pointers are given; work = tcvom_block_norm_bwd_work(T, C, gate rows shared by several tokens, else 1) floats.
+ * Fixed order of additions. */
+#define TCVOM_MAX_NORM_CHANNELS 8192
+int tcvom_block_norm_fwd(const void* x, const void* y, const float* post_weight, const float* post_bias, const void* gate,
+                         int32_t gate_f32, int64_t gate_rows, const float* pre_weight, const float* pre_bias, float branch_scale,
+                         float residual_scale, float eps, int32_t layer, void* x_out, void* h, float* stats, int64_t T, int32_t C,
+                         int32_t x_type, int32_t y_type, void* stream);
+int64_t tcvom_block_norm_bwd_work(int64_t T, int32_t C, int64_t gate_groups);
+int tcvom_block_norm_bwd(const void* x, const void* y, const float* post_weight, const float* post_bias, const void* gate,
+                         int32_t gate_f32, int64_t gate_rows, const float* pre_weight, float branch_scale, float residual_scale,
+                         int32_t layer, const float* stats, const void* dx_out, const void* dh, void* dx, void* dy,
+                         float* dpost_weight, float* dpost_bias, void* dgate, float* dpre_weight, float* dpre_bias, float* work,
+                         int64_t work_floats, int64_t T, int32_t C, int32_t x_type, int32_t y_type, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

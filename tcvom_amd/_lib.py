@@ -62,6 +62,23 @@ class SnDot(C.Structure):
     _fields_ = [('out', C.c_void_p), ('frame_stride', C.c_int64), ('eps', C.c_float), ('training', C.c_int32), ('scale', C.c_float)]
 
 
+MAX_BUCKETS, MAX_BUCKET_STARTS, MAX_BUCKET_REACH, MAX_NORM_CHANNELS = 256, 128, 1024, 8192
+
+
+class RelBuckets(C.Structure):
+    """struct tcvom_rel_buckets: the buckets of a relative position (tcvom_amd/token_ops.py fills it)."""
+    _fields_ = [('num_buckets', C.c_int32), ('bidirectional', C.c_int32), ('exact', C.c_int32), ('n_starts', C.c_int32),
+                ('starts', C.c_int32 * MAX_BUCKET_STARTS)]
+
+
+class AttnDesc(C.Structure):
+    """struct tcvom_attn_desc."""
+    _fields_ = [('B', C.c_int32), ('Nq', C.c_int32), ('Nk', C.c_int32), ('H', C.c_int32), ('Hkv', C.c_int32), ('D', C.c_int32),
+                ('type', C.c_int32), ('causal', C.c_int32), ('q_start', C.c_int32), ('scale', C.c_float),
+                ('q_stride', C.c_int64 * 3), ('k_stride', C.c_int64 * 3), ('v_stride', C.c_int64 * 3),
+                ('k_lens', C.c_void_p), ('q_starts', C.c_void_p), ('key_mask', C.c_void_p), ('buckets', RelBuckets)]
+
+
 class TcvomError(RuntimeError):
     pass
 
@@ -85,6 +102,8 @@ DP = C.POINTER(ConvDesc)
 SP = C.POINTER(SnScratch)
 YP = C.POINTER(BnSync)
 TP = C.POINTER(SnDot)
+KP = C.POINTER(RelBuckets)
+AP = C.POINTER(AttnDesc)
 
 # name -> argtypes (all return int except the explicitly listed ones)
 _PROTOS = {
@@ -234,11 +253,24 @@ _PROTOS = {
     'tcvom_wgrad_igemm_hetero': [vp, vp, vp, i32, vp, vp, i32, i32, i32, vp],
     'tcvom_wgrad_igemm_hetero_max_problems': [],
     'tcvom_wgrad_ws_max_geometries': [],
+    'tcvom_relbias_fwd': [vp, vp, KP, i32, i64, i64, i64, i32, vp],
+    'tcvom_relbias_bwd_work': [KP, i32, i64],
+    'tcvom_relbias_bwd': [vp, vp, vp, i64, KP, i32, i64, i64, i64, i32, vp],
+    'tcvom_attn_fwd_work': [AP],
+    'tcvom_attn_fwd': [AP, vp, vp, vp, vp, vp, vp, vp, vp, i64, vp],
+    'tcvom_attn_bwd_work': [AP],
+    'tcvom_attn_bwd': [AP, vp, vp, vp, vp, vp, vp, vp, vp, C.POINTER(i64), vp, vp, vp, vp, vp, i64, vp],
+    'tcvom_block_norm_fwd': [vp, vp, vp, vp, vp, i32, i64, vp, vp, f32, f32, f32, i32, vp, vp, vp, i64, i32, i32, i32, vp],
+    'tcvom_block_norm_bwd_work': [i64, i32, i64],
+    'tcvom_block_norm_bwd': [vp, vp, vp, vp, vp, i32, i64, vp, f32, f32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i32,
+                             i32, i32, vp],
 }
 # entry points that return a count, not a status
 _PLAIN = {'tcvom_conv_stats_groups', 'tcvom_bn_bwd_groups', 'tcvom_bn_bwd_groups_n', 'tcvom_abi_version', 'tcvom_act_dtype', 'tcvom_bn_finalize_scratch_doubles',
           'tcvom_wgrad_ws_max_problems', 'tcvom_wgrad_ws_max_geometries', 'tcvom_dw3x3_stats_groups', 'tcvom_gca_scores_softmax_ok', 'tcvom_sn_apply_blocks',
-          'tcvom_adaptive_avgpool_scratch_floats', 'tcvom_wgrad_igemm_hetero_plan', 'tcvom_wgrad_igemm_hetero_max_problems'}
+          'tcvom_adaptive_avgpool_scratch_floats', 'tcvom_wgrad_igemm_hetero_plan', 'tcvom_wgrad_igemm_hetero_max_problems',
+          'tcvom_relbias_bwd_work', 'tcvom_attn_fwd_work', 'tcvom_attn_bwd_work', 'tcvom_block_norm_bwd_work'}
+_I64 = {'tcvom_relbias_bwd_work', 'tcvom_attn_fwd_work', 'tcvom_attn_bwd_work', 'tcvom_block_norm_bwd_work'}          # counts of 64 bits
 
 # entry points that return a string
 _STRING = {'tcvom_conv_igemm_variant': [DP, i32], 'tcvom_wgrad_igemm_variant': [DP]}
@@ -254,7 +286,7 @@ def _bind():
         except AttributeError as e:
             raise ImportError('tcvom_amd: %s does not export %s (stale build?)' % (LIB_PATH, name)) from e
         fn.argtypes = argtypes
-        fn.restype = C.c_int
+        fn.restype = C.c_int64 if name in _I64 else C.c_int
         fns[name] = fn
     for name, argtypes in _STRING.items():
         try:

@@ -1,0 +1,154 @@
+// Attention with a bucketed relative position bias, shared by attn.hip (forward) and attn_bwd.hip.
+//     x[i][j] = scale <q_i, k_j> + bias[h][j - i - q_start],   p = softmax over the keys row i sees,   out_i = sum_j p[i][j] v_j
+//
+// Products on v_mfma_f32_32x32x16.  Scores are formed TRANSPOSED, S^T = K Q^T (rows = keys, columns = queries): a lane then holds one
+// query (column lane & 31) and 16 keys of each 32-key block, key 8 (r / 4) + 4 (lane >> 5) + r % 4 in register r, so that a row's maximum
+// and sum are sums inside the lane plus one exchange with lane ^ 32, and the exponentials, rounded to 16 bits, ARE the second
+// operand of O^T = V^T P^T: the contraction index is permuted the same way on both sides (the transposing LDS read of V takes its 4-key
+// rows in that order).  Everything is in base 2: scale and bias are multiplied by log2(e) once.
+//
+// A head's bias is a "line" of values over the clamped relative position (token_common.h) in LDS.  A tile of keys whose relative
+// positions all lie past one end of the line adds a constant; the others read the line, 4 consecutive entries for 4 keys.
+#pragma once
+#include "token_common.h"
+
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2_t;
+
+template <class T> struct Mma;
+template <> struct Mma<__bf16> {
+    typedef __attribute__((ext_vector_type(8))) __bf16 v8;
+    typedef __attribute__((ext_vector_type(4))) __bf16 v4;
+    typedef __attribute__((ext_vector_type(2))) __bf16 v2;
+    static __device__ __forceinline__ f32x16_t mma(v8 a, v8 b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ v4 tr(const __bf16* p) {
+        return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((__attribute__((address_space(3))) v4*)p);
+    }
+    static constexpr float shift = 0.f;
+};
+template <> struct Mma<_Float16> {
+    typedef __attribute__((ext_vector_type(8))) _Float16 v8;
+    typedef __attribute__((ext_vector_type(4))) _Float16 v4;
+    typedef __attribute__((ext_vector_type(2))) _Float16 v2;
+    static __device__ __forceinline__ f32x16_t mma(v8 a, v8 b, f32x16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ v4 tr(const _Float16* p) {
+        typedef __attribute__((ext_vector_type(4))) __fp16 h4;
+        return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) h4*)p));
+    }
+    // probabilities are held as 2^shift p: most of a long row lies below fp16's smallest normal number, 2^-14
+    static constexpr float shift = 15.f;
+};
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int KT = 64;                       // keys a tile
+
+struct AttnArgs {
+    const void *q, *k, *v;
+    const float* table;                      // [buckets][H]
+    void *out, *out_lo;                      // [B][Nq][H][D]; out_lo: out's rounding error in 16 bits (training), or null
+    float* lse;                              // [B][H][Nq], base 2, -inf for a row without a key
+    const void* dout;
+    void *dq, *dk, *dv;
+    float *delta, *part;                     // backward: <dout, out> of every row; bucket sums of every workgroup
+    float* partial;                          // forward: the splits' outputs
+    const int *k_lens, *q_starts;            // [B] or null
+    const unsigned char* key_mask;           // [B][Nk] or null
+    long long qs[3], ks[3], vs[3], dos[3];   // strides of batch, token, head in elements
+    int B, Nq, Nk, H, Hkv, D, causal, q_start, splits, tiles;
+    float scale;                             // softmax scale, natural
+    tcvom_rel_buckets bk;
+};
+
+// keys of sequence b that exist, and the position of its first query
+__device__ __forceinline__ int seq_keys(const AttnArgs& a, int b) {
+    if (!a.k_lens) return a.Nk;
+    const int n = a.k_lens[b];
+    return n < 0 ? 0 : n > a.Nk ? a.Nk : n;
+}
+__device__ __forceinline__ int seq_start(const AttnArgs& a, int b) {
+    if (!a.q_starts) return a.q_start;
+    const int s = a.q_starts[b];
+    return s < -(1 << 29) ? -(1 << 29) : s > (1 << 29) ? (1 << 29) : s;
+}
+
+// workgroup -> work item: the hardware deals workgroups round-robin over the 8 XCDs, each with its own L2; consecutive items (tiles that
+// share keys and values) go to one XCD
+__device__ __forceinline__ int xcd_item(int id, int total) {
+    const int per = total / 8, whole = per * 8;
+    return id < whole ? (id & 7) * per + (id >> 3) : id;
+}
+
+// LDS position of 16-byte chunk c of row r, rows of DP elements.  The XOR spreads over the 64 banks (256 bytes) both (a) fragment reads, 16
+// consecutive rows at one chunk, and (b) transposing reads, 4 consecutive rows at 4 consecutive chunks.
+template <int DP> __device__ __forceinline__ int chunk_at(int r, int c) {
+    if constexpr (DP == 128) return r * 16 + (c ^ (((r & 3) << 2) | ((r >> 2) & 3)));
+    else if constexpr (DP == 64) return r * 8 + (c ^ (((r & 2) << 1) | ((r >> 2) & 3)));
+    else return r * 4 + (c ^ ((r >> 2) & 3));
+}
+
+__device__ __forceinline__ float half_max(float v) {       // maximum over lanes l and l ^ 32
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <class T>
+__device__ __forceinline__ typename Mma<T>::v8 join(typename Mma<T>::v4 lo, typename Mma<T>::v4 hi) {
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+// registers 8 s .. 8 s + 7 of a 32 x 32 block as the 16-bit operand of k-step s
+template <class T>
+__device__ __forceinline__ typename Mma<T>::v8 pack_step(const f32x16_t& p, int s) {
+    typename Mma<T>::v8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (T)p[8 * s + i];
+    return r;
+}
+// ... and what that rounding dropped, rounded again
+template <class T>
+__device__ __forceinline__ typename Mma<T>::v8 pack_rest(const f32x16_t& p, typename Mma<T>::v8 hi, int s) {
+    typename Mma<T>::v8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (T)(p[8 * s + i] - (float)hi[i]);
+    return r;
+}
+
+// operand A of a product that contracts the rows of an LDS tile, 16 of them from r0 (in the score registers' order): the tile's columns
+// 32 d + (lane & 31)
+template <class T, int DP>
+__device__ __forceinline__ typename Mma<T>::v8 read_columns(const T* tile, int r0, int d, int lane) {
+    const int r = r0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int ch = d * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), in = (lane & 1) * 4;
+    return join<T>(Mma<T>::tr(&tile[chunk_at<DP>(r, ch) * 8 + in]), Mma<T>::tr(&tile[chunk_at<DP>(r + 8, ch) * 8 + in]));
+}
+// operand A of a product over the tile's columns: row (lane & 31) from r0, columns 16 s + 8 (lane >> 5) ..
+template <class T, int DP>
+__device__ __forceinline__ typename Mma<T>::v8 read_rows(const T* tile, int r0, int s, int lane) {
+    return *reinterpret_cast<const typename Mma<T>::v8*>(&tile[chunk_at<DP>(r0 + (lane & 31), s * 2 + (lane >> 5)) * 8]);
+}
+// 16 bytes of a row, zeros where `ok` is false
+template <class V8, class T>
+__device__ __forceinline__ V8 load_or_zero(bool ok, const T* p) {
+    V8 z = {};
+    if (ok) z = *reinterpret_cast<const V8*>(p);
+    return z;
+}
+__device__ __forceinline__ f32x16_t zero16() {
+    f32x16_t z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.f;
+    return z;
+}
+// the line of head h, times log2(e)
+__device__ __forceinline__ void fill_line(float* line, const AttnArgs& a, int h, int threads) {
+    const int reach = line_reach(a.bk), last = reach + line_right(a.bk);
+    for (int t = threadIdx.x; t <= last; t += threads) line[t] = a.table[rel_bucket(a.bk, t - reach) * a.H + h] * LOG2E;
+}
+
+// host side
+int attn_check(const char* who, const tcvom_attn_desc* d, AttnArgs* a);
+static inline int attn_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }

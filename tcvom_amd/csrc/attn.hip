@@ -1,0 +1,526 @@
+// Forward of the attention with a relative position bias (attn.h), reached through tcvom_attn_fwd.
+#include "attn.h"
+
+// ---- many queries: a workgroup of 4 waves takes 128 QB queries of one head, a wave 32 QB of them, all through the same tiles of 64 keys.
+// K and V tiles go to LDS through registers (the next tile's loads are in flight during this tile's products), two buffers, one
+// barrier a tile.
+template <class T, int DP, int QB, bool LO>
+__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
+    typedef typename Mma<T>::v8 v8;
+    constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8, PER = KT * CH / 256;
+    constexpr int BM = 128 * QB;
+    __shared__ __align__(16) T lk[2][KT * DP];
+    __shared__ __align__(16) T lv[2][KT * DP];
+    extern __shared__ float line[];
+
+    const int item = xcd_item(blockIdx.x, gridDim.x);
+    const int bh = item / a.tiles, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
+    const int tile = a.causal ? a.tiles - 1 - item % a.tiles : item % a.tiles;          // long causal rows first
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+    const int i0 = tile * BM, start = seq_start(a, b), len = seq_keys(a, b);
+    // keys any query of the workgroup sees
+    const int i_last = min(i0 + BM, a.Nq) - 1;
+    const int kend = a.causal ? max(0, min(len, i_last + start + 1)) : len;
+    const int ntiles = (kend + KT - 1) / KT;
+    const int reach = line_reach(a.bk), right = line_right(a.bk), last = reach + right;
+    fill_line(line, a, h, 256);
+
+    const T* Q = (const T*)a.q + b * a.qs[0] + h * a.qs[2];
+    const T* K = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
+    const T* V = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
+    const unsigned char* mask = a.key_mask ? a.key_mask + (long long)b * a.Nk : nullptr;
+
+    int qi[QB];
+    v8 qf[QB][KS];
+#pragma unroll
+    for (int u = 0; u < QB; ++u) {
+        qi[u] = i0 + (wave * QB + u) * 32 + col;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = s * 16 + half * 8;
+            v8 z = {};
+            qf[u][s] = z;
+            if (qi[u] < a.Nq && d < a.D) qf[u][s] = *reinterpret_cast<const v8*>(Q + (long long)qi[u] * a.qs[1] + d);
+        }
+    }
+
+    u32x4_t rk[PER], rv[PER];
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            const int idx = n * 256 + threadIdx.x, r = idx / CH, c = idx % CH, key = t * KT + r;
+            u32x4_t z = {0, 0, 0, 0};
+            rk[n] = z;
+            rv[n] = z;
+            if (key < kend && c * 8 < a.D) {
+                rk[n] = *reinterpret_cast<const u32x4_t*>(K + (long long)key * a.ks[1] + c * 8);
+                // values of masked keys count as zero: 0 x inf would not
+                if (!mask || mask[key]) rv[n] = *reinterpret_cast<const u32x4_t*>(V + (long long)key * a.vs[1] + c * 8);
+            }
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            const int idx = n * 256 + threadIdx.x, r = idx / CH, c = idx % CH;
+            *reinterpret_cast<u32x4_t*>(&lk[buf][chunk_at<DP>(r, c) * 8]) = rk[n];
+            *reinterpret_cast<u32x4_t*>(&lv[buf][chunk_at<DP>(r, c) * 8]) = rv[n];
+        }
+    };
+
+    f32x16_t o[QB][DB];
+    float m[QB], l[QB];
+#pragma unroll
+    for (int u = 0; u < QB; ++u) {
+        m[u] = -INFINITY;
+        l[u] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[u][d][r] = 0.f;
+    }
+    const float c = a.scale * LOG2E;
+    if (ntiles > 0) {
+        fetch(0);
+        store(0);
+    }
+    __syncthreads();
+    for (int t = 0; t < ntiles; ++t) {
+        const int buf = t & 1, k0 = t * KT;
+        if (t + 1 < ntiles) fetch(t + 1);
+        unsigned long long bits = ~0ull;
+        if (mask) bits = __ballot(k0 + lane < a.Nk && mask[min(k0 + lane, a.Nk - 1)]);
+#pragma unroll
+        for (int u = 0; u < QB; ++u) {
+            // S^T of 64 keys x 32 queries
+            f32x16_t x[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[kb][r] = 0.f;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    x[kb] = Mma<T>::mma(read_rows<T, DP>(lk[buf], kb * 32, s, lane), qf[u][s], x[kb]);
+                }
+            }
+            const int w0 = i0 + (wave * QB + u) * 32;               // the wave's first query of this block
+            const int rel_hi = k0 + KT - 1 - w0 - start, rel_lo = k0 - (w0 + 31) - start;
+            const bool far = rel_hi <= -reach || rel_lo >= right;
+            float add = rel_hi <= -reach ? line[0] : line[last];
+            if (!far) {
+                add = 0.f;
+                int at = k0 + 4 * half - qi[u] - start + reach;       // line index of the lane's first key
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int e = at + kb * 32 + 8 * (r / 4) + r % 4;
+                        x[kb][r] = fmaf(x[kb][r], c, line[min(max(e, 0), last)]);
+                    }
+            }
+            const float mul = far ? c : 1.f;
+            // keys the lane's query sees: bit n of `see` = key k0 + n
+            const int lim = min(len, a.causal ? qi[u] + start + 1 : len) - k0;
+            if (bits != ~0ull || k0 + KT > min(len, a.causal ? w0 + start + 1 : len)) {
+                const unsigned long long see = lim >= 64 ? bits : lim <= 0 ? 0 : bits & ((1ull << lim) - 1);
+                const unsigned s0 = (unsigned)see >> (4 * half), s1 = (unsigned)(see >> 32) >> (4 * half);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    if (!(s0 >> (8 * (r / 4) + r % 4) & 1)) x[0][r] = -INFINITY;
+                    if (!(s1 >> (8 * (r / 4) + r % 4) & 1)) x[1][r] = -INFINITY;
+                }
+            }
+            float top = fmaxf(x[0][0], x[1][0]);
+#pragma unroll
+            for (int r = 1; r < 16; ++r) top = fmaxf(top, fmaxf(x[0][r], x[1][r]));
+            top = half_max(top);
+            top = far ? fmaf(top, c, add) : top;
+            const float mn = fmaxf(m[u], top);
+            if (__any(mn > m[u])) {
+                const float base = mn == -INFINITY ? 0.f : mn;
+                const float alpha = exp2_hw(m[u] - base);
+                l[u] *= alpha;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[u][d][r] *= alpha;
+                m[u] = mn;
+            }
+            const float sub = add + Mma<T>::shift - (m[u] == -INFINITY ? 0.f : m[u]);
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    x[kb][r] = exp2_hw(fmaf(x[kb][r], mul, sub));
+                    sum[r & 3] += x[kb][r];
+                }
+            l[u] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const v8 p = pack_step<T>(x[kb], s);
+                    v8 rest;
+                    if constexpr (LO) rest = pack_rest<T>(x[kb], p, s);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        const v8 vf = read_columns<T, DP>(lv[buf], kb * 32 + s * 16, d, lane);
+                        o[u][d] = Mma<T>::mma(vf, p, o[u][d]);
+                        if constexpr (LO) o[u][d] = Mma<T>::mma(vf, rest, o[u][d]);
+                    }
+                }
+        }
+        if (t + 1 < ntiles) store(buf ^ 1);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int u = 0; u < QB; ++u) {
+        const float sum = half_sum(l[u]);
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        if (qi[u] >= a.Nq) continue;
+        const long long row = ((long long)b * a.Nq + qi[u]) * a.H + h;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int at = d * 32 + g * 8 + half * 4;
+                if (at >= a.D) continue;
+                typename Mma<T>::v4 w, lo;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float f = sum > 0.f ? o[u][d][4 * g + j] * inv : 0.f;
+                    w[j] = (T)f;
+                    lo[j] = (T)(f - (float)w[j]);
+                }
+                *reinterpret_cast<typename Mma<T>::v4*>((T*)a.out + row * a.D + at) = w;
+                if (LO) *reinterpret_cast<typename Mma<T>::v4*>((T*)a.out_lo + row * a.D + at) = lo;
+            }
+        if (a.lse && half == 0)
+            a.lse[((long long)b * a.H + h) * a.Nq + qi[u]] = sum > 0.f ? m[u] + log2f(sum) - Mma<T>::shift : -INFINITY;
+    }
+}
+
+// ---- few queries (single tokens): bound by reading K and V once.  The G = H / Hkv heads that share keys times the queries are the 32
+// columns of one score tile, so that shared keys are read once; the keys are cut into `splits` ranges for workgroups to fill the
+// chip, and a range is dealt 32 keys at a time to 4 waves that keep their own maximum, sum and output and join at the end.
+// K fragments go from memory to registers (a lane reads the 16 bytes it needs), V through a wave's own LDS rows to be transposed:
+// no barrier inside the loop, the next 32 keys in flight.
+template <class T, int DP>
+__global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
+    typedef typename Mma<T>::v8 v8;
+    constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8, PER = 32 * CH / 64;
+    __shared__ __align__(16) T lv[4][32 * DP];                         // after the loop: 32 x DP floats of two waves at a time
+    __shared__ float lm[4][32], ll[4][32];
+    extern __shared__ float tab[];                                     // [buckets][G]: times log2(e), then the bucket of each line entry
+    const int G = a.H / a.Hkv, rows = G * a.Nq;
+    const int reach = line_reach(a.bk), right = line_right(a.bk), last = reach + right;
+    unsigned char* bucket = (unsigned char*)(tab + a.bk.num_buckets * G);
+    const int split = blockIdx.x % a.splits, rt = blockIdx.x / a.splits % a.tiles, bh = blockIdx.x / (a.splits * a.tiles);
+    const int b = bh / a.Hkv, hk = bh % a.Hkv;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+    const int start = seq_start(a, b), len = seq_keys(a, b);
+    const int kend = a.causal ? max(0, min(len, a.Nq + start)) : len;
+    // this split's keys: an equal share of the existing ones, in whole rounds of 128
+    const int share = (kend + a.splits * 128 - 1) / (a.splits * 128) * 128;
+    const int ka = min(kend, split * share), kz = min(kend, ka + share);
+    for (int t = threadIdx.x; t < a.bk.num_buckets * G; t += 256)
+        tab[t] = a.table[(long long)(t / G) * a.H + hk * G + t % G] * LOG2E;
+    for (int t = threadIdx.x; t <= last; t += 256) bucket[t] = (unsigned char)rel_bucket(a.bk, t - reach);
+
+    const int row = rt * 32 + col, g = min(row, rows - 1) / a.Nq, i = min(row, rows - 1) % a.Nq, h = hk * G + g;
+    const bool live = row < rows;
+    const T* Q = (const T*)a.q + b * a.qs[0] + h * a.qs[2] + (long long)i * a.qs[1];
+    const T* K = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
+    const T* V = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
+    const unsigned char* mask = a.key_mask ? a.key_mask + (long long)b * a.Nk : nullptr;
+    v8 qf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        const int d = s * 16 + half * 8;
+        v8 z = {};
+        qf[s] = z;
+        if (live && d < a.D) qf[s] = *reinterpret_cast<const v8*>(Q + d);
+    }
+    v8 kf[KS];
+    u32x4_t rv[PER];
+    auto fetch = [&](int k0) {
+        const int key = k0 + col;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const int d = s * 16 + half * 8;
+            v8 z = {};
+            kf[s] = z;
+            if (key < kz && d < a.D) kf[s] = *reinterpret_cast<const v8*>(K + (long long)key * a.ks[1] + d);
+        }
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            const int idx = n * 64 + lane, r = idx / CH, ch = idx % CH;
+            u32x4_t z = {0, 0, 0, 0};
+            rv[n] = z;
+            if (k0 + r < kz && ch * 8 < a.D && (!mask || mask[k0 + r]))
+                rv[n] = *reinterpret_cast<const u32x4_t*>(V + (long long)(k0 + r) * a.vs[1] + ch * 8);
+        }
+    };
+    f32x16_t o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const float c = a.scale * LOG2E;
+    int k0 = ka + wave * 32;
+    if (k0 < kz) fetch(k0);
+    __syncthreads();
+    const float bias_lo = tab[bucket[0] * G + g], bias_hi = tab[bucket[last] * G + g];
+    for (; k0 < kz; k0 += 128) {
+        f32x16_t x;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) x = Mma<T>::mma(kf[s], qf[s], x);
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            const int idx = n * 64 + lane, r = idx / CH, ch = idx % CH;
+            *reinterpret_cast<u32x4_t*>(&lv[wave][chunk_at<DP>(r, ch) * 8]) = rv[n];
+        }
+        unsigned bits = ~0u;
+        if (mask) bits = (unsigned)__ballot(mask[min(k0 + col, a.Nk - 1)]);
+        if (k0 + 128 < kz) fetch(k0 + 128);
+        // one bias for the tile, or one for each element
+        if (k0 + 31 - start <= -reach || k0 - (a.Nq - 1) - start >= right) {
+            const float add = k0 + 31 - start <= -reach ? bias_lo : bias_hi;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], c, add);
+        } else {
+            const int at = k0 + 4 * half - i - start + reach;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int e = at + 8 * (r / 4) + r % 4;
+                x[r] = fmaf(x[r], c, tab[bucket[min(max(e, 0), last)] * G + g]);
+            }
+        }
+        const int lim = min(kz, a.causal ? i + start + 1 : kz) - k0;
+        if (mask || k0 + 32 > kz || (a.causal && k0 + 32 > start + 1)) {
+            const unsigned see = (lim >= 32 ? bits : lim <= 0 ? 0 : bits & ((1u << lim) - 1)) >> (4 * half);
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (!(see >> (8 * (r / 4) + r % 4) & 1)) x[r] = -INFINITY;
+        }
+        float top = x[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
+        const float mn = fmaxf(m, half_max(top));
+        const float base = mn == -INFINITY ? 0.f : mn;
+        if (__any(mn > m)) {
+            const float alpha = exp2_hw(m - base);
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+            m = mn;
+        }
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            x[r] = exp2_hw(x[r] + (Mma<T>::shift - base));
+            sum[r & 1] += x[r];
+        }
+        l += sum[0] + sum[1];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const v8 p = pack_step<T>(x, s);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] = Mma<T>::mma(read_columns<T, DP>(lv[wave], s * 16, d, lane), p, o[d]);
+        }
+    }
+    // join the 4 waves: common maximum, then the outputs are added two waves at a time in LDS
+    l = half_sum(l);
+    if (half == 0) {
+        lm[wave][col] = m;
+        ll[wave][col] = l;
+    }
+    __syncthreads();
+    float M = fmaxf(fmaxf(lm[0][col], lm[1][col]), fmaxf(lm[2][col], lm[3][col]));
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) L += ll[w][col] * exp2_hw(lm[w][col] - base);
+    const float mine = exp2_hw(m - base);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[d][r] *= mine;
+    // element (d, r) of a wave at [(d 16 + r) 64 + lane]: DP / 2 x 64 floats = 32 DP a wave, the size of two waves' V rows
+    float* red = reinterpret_cast<float*>(&lv[0][0]);
+    constexpr int WORDS = 32 * DP;
+    for (int step = 2; step > 0; step >>= 1) {
+        __syncthreads();
+        if (wave >= step && wave < 2 * step)
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) red[(wave - step) * WORDS + (d * 16 + r) * 64 + lane] = o[d][r];
+        __syncthreads();
+        if (wave < step)
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][r] += red[wave * WORDS + (d * 16 + r) * 64 + lane];
+    }
+    if (wave != 0 || !live) return;
+    const long long out_row = ((long long)b * a.Nq + i) * a.H + h;
+    if (a.splits == 1) {
+        const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int at = d * 32 + q * 8 + half * 4;
+                if (at >= a.D) continue;
+                typename Mma<T>::v4 w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = (T)(L > 0.f ? o[d][4 * q + j] * inv : 0.f);
+                *reinterpret_cast<typename Mma<T>::v4*>((T*)a.out + out_row * a.D + at) = w;
+            }
+        if (a.lse && half == 0) a.lse[((long long)b * a.H + h) * a.Nq + i] = L > 0.f ? M + log2f(L) - Mma<T>::shift : -INFINITY;
+        return;
+    }
+    // partial [split][out_row][D + 2]: output, maximum, sum
+    float* part = a.partial + ((long long)split * a.B * a.Nq * a.H + out_row) * (a.D + 4);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int at = d * 32 + q * 8 + half * 4;
+            if (at < a.D) *reinterpret_cast<float4*>(part + at) = make_float4(o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]);
+        }
+    if (half == 0) {
+        part[a.D] = M;
+        part[a.D + 1] = L;
+    }
+}
+
+// joins the splits of a row: a wave a row, a lane 2 channels (D <= 128)
+template <class T>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+    const int lane = threadIdx.x & 63;
+    const long long rows = (long long)a.B * a.Nq * a.H, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int ld = a.D + 4;
+    const float* p = a.partial + row * ld;
+    const long long step = rows * ld;
+    float M = -INFINITY;
+    for (int s = lane; s < a.splits; s += 64) M = fmaxf(M, p[s * step + a.D]);
+    M = wave_max(M);
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, o0 = 0.f, o1 = 0.f;
+    const int d = lane * 2;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+        const float w = exp2_hw(p[s * step + a.D] - base);
+        L += w * p[s * step + a.D + 1];
+        if (d < a.D) {
+            const float2 f = *reinterpret_cast<const float2*>(p + s * step + d);
+            o0 += w * f.x;
+            o1 += w * f.y;
+        }
+    }
+    const float inv = L > 0.f ? 1.f / L : 0.f;
+    if (d < a.D) {
+        typename Mma<T>::v2 w = {(T)(L > 0.f ? o0 * inv : 0.f), (T)(L > 0.f ? o1 * inv : 0.f)};
+        *reinterpret_cast<typename Mma<T>::v2*>((T*)a.out + row * a.D + d) = w;
+    }
+    if (a.lse && lane == 0) {
+        const long long b = row / ((long long)a.Nq * a.H), i = row / a.H % a.Nq, h = row % a.H;
+        a.lse[(b * a.H + h) * a.Nq + i] = L > 0.f ? M + log2f(L) - Mma<T>::shift : -INFINITY;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+int attn_check(const char* who, const tcvom_attn_desc* d, AttnArgs* a) {
+    if (!d) return tcvom_fail(TCVOM_ERR_ARG, "%s: null description", who);
+    TCVOM_CHECK_ARG(d->type == TCVOM_TYPE_BF16 || d->type == TCVOM_TYPE_F16, "%s: type %d", who, d->type);
+    TCVOM_CHECK_ARG(d->B >= 0 && d->H > 0 && d->Hkv > 0 && d->H % d->Hkv == 0, "%s: B=%d H=%d Hkv=%d", who, d->B, d->H, d->Hkv);
+    TCVOM_CHECK_ARG(d->D >= 8 && d->D <= 128 && d->D % 8 == 0, "%s: head width %d (8..128, a multiple of 8)", who, d->D);
+    TCVOM_CHECK_ARG(d->Nq >= 0 && d->Nk >= 0 && d->Nq <= (1 << 28) && d->Nk <= (1 << 28), "%s: Nq=%d Nk=%d", who, d->Nq, d->Nk);
+    TCVOM_CHECK_ARG(d->q_start >= -(1 << 29) && d->q_start <= (1 << 29), "%s: q_start=%d", who, d->q_start);
+    TCVOM_CHECK_ARG(d->scale > 0.f && d->scale < INFINITY, "%s: scale %g", who, d->scale);
+    for (int n = 0; n < 3; ++n)
+        TCVOM_CHECK_ARG(d->q_stride[n] % 8 == 0 && d->k_stride[n] % 8 == 0 && d->v_stride[n] % 8 == 0 && d->q_stride[n] >= 0 &&
+                            d->k_stride[n] >= 0 && d->v_stride[n] >= 0, "%s: strides are multiples of 8 elements", who);
+    if (const int rc = check_buckets(who, &d->buckets)) return rc;
+    *a = AttnArgs();
+    a->B = d->B; a->Nq = d->Nq; a->Nk = d->Nk; a->H = d->H; a->Hkv = d->Hkv; a->D = d->D;
+    a->causal = d->causal; a->q_start = d->q_start; a->scale = d->scale;
+    a->k_lens = d->k_lens; a->q_starts = d->q_starts; a->key_mask = d->key_mask; a->bk = d->buckets;
+    for (int n = 0; n < 3; ++n) { a->qs[n] = d->q_stride[n]; a->ks[n] = d->k_stride[n]; a->vs[n] = d->v_stride[n]; }
+    return 0;
+}
+
+// few queries: see attn_few_kernel; a single tile of 32 columns then serves all heads of a group
+static bool attn_few(const tcvom_attn_desc* d) { return d->Nq <= 32; }
+static void few_shape(const tcvom_attn_desc* d, int* tiles, int* splits) {
+    *tiles = cdiv((long long)d->H / d->Hkv * d->Nq, 32);
+    const long long wgs = (long long)d->B * d->Hkv * *tiles;
+    // two workgroups a CU, and at least 256 keys a workgroup
+    long long s = wgs ? 512 / wgs : 1;
+    const long long most = d->Nk / 256;
+    if (s > most) s = most;
+    *splits = (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+}
+
+extern "C" int64_t tcvom_attn_fwd_work(const tcvom_attn_desc* d) {
+    if (!d || d->B <= 0 || d->Nq <= 0 || d->Hkv <= 0 || !attn_few(d)) return 0;
+    int tiles, splits;
+    few_shape(d, &tiles, &splits);
+    return splits > 1 ? (int64_t)splits * d->B * d->Nq * d->H * (d->D + 4) : 0;
+}
+
+template <class T, int DP>
+static void launch_fwd(AttnArgs a, const tcvom_attn_desc* d, hipStream_t st) {
+    const int last = line_reach(a.bk) + line_right(a.bk);
+    if (attn_few(d) && !a.out_lo) {
+        few_shape(d, &a.tiles, &a.splits);
+        const size_t lds = sizeof(float) * a.bk.num_buckets * (a.H / a.Hkv) + last + 1;
+        const dim3 grid((unsigned)((long long)a.B * a.Hkv * a.tiles * a.splits));
+        hipLaunchKernelGGL((attn_few_kernel<T, DP>), grid, dim3(256), lds, st, a);
+        if (a.splits > 1)
+            hipLaunchKernelGGL((attn_join_kernel<T>), dim3(cdiv((long long)a.B * a.Nq * a.H, 4)), dim3(256), 0, st, a);
+        return;
+    }
+    constexpr int QB = 1;
+    a.tiles = cdiv(a.Nq, 128 * QB);
+    const dim3 grid((unsigned)((long long)a.B * a.H * a.tiles));
+    const size_t lds = sizeof(float) * (last + 1);
+    if (a.out_lo) hipLaunchKernelGGL((attn_fwd_kernel<T, DP, QB, true>), grid, dim3(256), lds, st, a);
+    else hipLaunchKernelGGL((attn_fwd_kernel<T, DP, QB, false>), grid, dim3(256), lds, st, a);
+}
+
+extern "C" int tcvom_attn_fwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, void* out,
+                              void* out_lo, float* lse, float* work, int64_t work_floats, void* stream) {
+    AttnArgs a;
+    if (const int rc = attn_check("attn_fwd", d, &a)) return rc;
+    if (d->B == 0 || d->Nq == 0) return 0;
+    TCVOM_CHECK_ARG(q && table && out && (d->Nk == 0 || (k && v)), "attn_fwd: null tensor");
+    TCVOM_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_lo), "attn_fwd: tensors start at multiples of 16 bytes");
+    TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 32) < (1LL << 30), "attn_fwd: too many queries for one launch");
+    TCVOM_CHECK_ARG(d->H / d->Hkv <= 64 || d->Nq > 32, "attn_fwd: %d heads share keys (at most 64)", d->H / d->Hkv);
+    TCVOM_CHECK_ARG(work_floats >= tcvom_attn_fwd_work(d) && (work || tcvom_attn_fwd_work(d) == 0), "attn_fwd: %lld floats of workspace",
+                    (long long)work_floats);
+    a.q = q; a.k = k; a.v = v; a.table = table; a.out = out; a.out_lo = out_lo; a.lse = lse; a.partial = work;
+    const hipStream_t st = (hipStream_t)stream;
+    const int DP = attn_width(d->D);
+    if (d->type == TCVOM_TYPE_BF16) {
+        if (DP == 32) launch_fwd<__bf16, 32>(a, d, st);
+        else if (DP == 64) launch_fwd<__bf16, 64>(a, d, st);
+        else launch_fwd<__bf16, 128>(a, d, st);
+    } else {
+        if (DP == 32) launch_fwd<_Float16, 32>(a, d, st);
+        else if (DP == 64) launch_fwd<_Float16, 64>(a, d, st);
+        else launch_fwd<_Float16, 128>(a, d, st);
+    }
+    TCVOM_LAUNCH_CHECK("attn_fwd");
+    return 0;
+}

@@ -1,0 +1,430 @@
+// Backward of the attention with a relative position bias (attn.h), reached through tcvom_attn_bwd.
+//   p  = exp(x - lse)             dv_j = sum_i p_ij do_i            dp_ij = <do_i, v_j>
+//   ds = p (dp - delta_i),        delta_i = <do_i, out_i>           dbias[h][j - i - q_start] = sum ds
+//   dq_i = scale sum_j ds_ij k_j                                    dk_j = scale sum_i ds_ij q_i
+// Two kernels, each adding in registers what it owns: the queries' one (dq, delta, bucket sums) walks the keys, the keys' one (dk, dv
+// over all heads that share them) walks the queries.  Scores are formed in both: 7 products instead of the 5 of a single pass, which
+// would have to add dq (or dk, dv) into memory in an order that changes from run to run.
+//
+// Rounding to 16 bits: p and ds as operands of the matrix products, as the forward rounds p.  The bucket sums take ds in 32 bits.
+#include "attn.h"
+
+// ---- dq, delta, bucket sums: a wave owns 32 queries of one head (S^T and dP^T as in the forward), the workgroup walks tiles of 64 keys.
+// Bucket sums: a tile past an end of the line adds to one register a lane; in a tile that crosses the line every element is added to
+// the entry of its relative position in LDS.  Each half wave has its own copy of the line, within which the 32 lanes of a step (one
+// key, 32 queries) have different entries, so that every entry is a sum in program order: equal calls give equal bits.
+template <class T, int DP, bool TABLE>
+__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
+    typedef typename Mma<T>::v8 v8;
+    constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8, PER = KT * CH / 256, BM = 128;
+    __shared__ __align__(16) T lk[2][KT * DP];
+    __shared__ __align__(16) T lv[2][KT * DP];
+    extern __shared__ float line[];
+
+    const int item = xcd_item(blockIdx.x, gridDim.x);
+    const int bh = item / a.tiles, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
+    const int tile = a.causal ? a.tiles - 1 - item % a.tiles : item % a.tiles;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+    const int i0 = tile * BM, start = seq_start(a, b), len = seq_keys(a, b);
+    const int i_last = min(i0 + BM, a.Nq) - 1;
+    const int kend = a.causal ? max(0, min(len, i_last + start + 1)) : len;
+    const int ntiles = (kend + KT - 1) / KT;
+    const int reach = line_reach(a.bk), right = line_right(a.bk), last = reach + right;
+    fill_line(line, a, h, 256);
+    float* sums = line + last + 1;                          // [8][last + 1]: half waves
+    if (TABLE)
+        for (int t = threadIdx.x; t < 8 * (last + 1); t += 256) sums[t] = 0.f;
+    float* mine = sums + (wave * 2 + half) * (last + 1);
+
+    const T* Q = (const T*)a.q + b * a.qs[0] + h * a.qs[2];
+    const T* K = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
+    const T* V = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
+    const T* dO = (const T*)a.dout + b * a.dos[0] + h * a.dos[2];
+    const unsigned char* mask = a.key_mask ? a.key_mask + (long long)b * a.Nk : nullptr;
+
+    const int w0 = i0 + wave * 32, qi = w0 + col;
+    const long long stat = ((long long)b * a.H + h) * a.Nq + qi, orow = (((long long)b * a.Nq + qi) * a.H + h) * a.D;
+    const float raw = qi < a.Nq ? a.lse[stat] : -INFINITY;
+    const bool live = raw != -INFINITY;                     // a row without a key has no gradient, whatever its dout holds
+    const float lse = live ? raw : 0.f;
+    v8 qf[KS], gf[KS];
+    float delta = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        const int d = s * 16 + half * 8;
+        const bool ok = live && d < a.D;
+        qf[s] = load_or_zero<v8>(ok, Q + (long long)qi * a.qs[1] + d);
+        gf[s] = load_or_zero<v8>(ok, dO + (long long)qi * a.dos[1] + d);
+        const v8 hi = load_or_zero<v8>(ok, (const T*)a.out + orow + d);
+        const v8 lo = load_or_zero<v8>(ok && a.out_lo, (const T*)a.out_lo + orow + d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[s][j], (float)hi[j] + (float)lo[j], delta);
+    }
+    delta = half_sum(delta);
+    if (half == 0 && qi < a.Nq) a.delta[stat] = delta;
+
+    u32x4_t rk[PER], rv[PER];
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            const int idx = n * 256 + threadIdx.x, r = idx / CH, c = idx % CH, key = t * KT + r;
+            const bool ok = key < kend && c * 8 < a.D && (!mask || mask[key]);
+            rk[n] = load_or_zero<u32x4_t>(ok, K + (long long)key * a.ks[1] + c * 8);
+            rv[n] = load_or_zero<u32x4_t>(ok, V + (long long)key * a.vs[1] + c * 8);
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            const int idx = n * 256 + threadIdx.x, r = idx / CH, c = idx % CH;
+            *reinterpret_cast<u32x4_t*>(&lk[buf][chunk_at<DP>(r, c) * 8]) = rk[n];
+            *reinterpret_cast<u32x4_t*>(&lv[buf][chunk_at<DP>(r, c) * 8]) = rv[n];
+        }
+    };
+    f32x16_t acc[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) acc[d] = zero16();
+    float far_lo = 0.f, far_hi = 0.f;
+    const float c = a.scale * LOG2E;
+    if (ntiles > 0) {
+        fetch(0);
+        store(0);
+    }
+    __syncthreads();
+    for (int t = 0; t < ntiles; ++t) {
+        const int buf = t & 1, k0 = t * KT;
+        if (t + 1 < ntiles) fetch(t + 1);
+        unsigned long long bits = ~0ull;
+        if (mask) bits = __ballot(k0 + lane < a.Nk && mask[min(k0 + lane, a.Nk - 1)]);
+        const int lim = min(len, a.causal ? qi + start + 1 : len) - k0;
+        const bool holes = bits != ~0ull || k0 + KT > min(len, a.causal ? w0 + start + 1 : len);
+        const unsigned long long see = lim >= 64 ? bits : lim <= 0 ? 0 : bits & ((1ull << lim) - 1);
+        const int rel_hi = k0 + KT - 1 - w0 - start, rel_lo = k0 - (w0 + 31) - start;
+        const bool far = rel_hi <= -reach || rel_lo >= right;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            f32x16_t x = zero16(), g = zero16();
+#pragma unroll
+            for (int s = 0; s < KS; ++s) x = Mma<T>::mma(read_rows<T, DP>(lk[buf], kb * 32, s, lane), qf[s], x);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) g = Mma<T>::mma(read_rows<T, DP>(lv[buf], kb * 32, s, lane), gf[s], g);
+            const int at = k0 + kb * 32 + 4 * half - qi - start + reach;
+            if (far) {
+                const float add = (rel_hi <= -reach ? line[0] : line[last]) - lse;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = exp2_hw(fmaf(x[r], c, add));
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int e = at + 8 * (r / 4) + r % 4;
+                    x[r] = exp2_hw(fmaf(x[r], c, line[min(max(e, 0), last)] - lse));
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] *= g[r] - delta;
+            if (holes || !live) {
+                const unsigned w = live ? (unsigned)(see >> (32 * kb)) >> (4 * half) : 0u;
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (!(w >> (8 * (r / 4) + r % 4) & 1)) x[r] = 0.f;
+            }
+            if (TABLE) {
+                if (far) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s += x[r];
+                    if (rel_hi <= -reach) far_lo += s; else far_hi += s;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int e = at + 8 * (r / 4) + r % 4;
+                        if (e <= 0) far_lo += x[r];
+                        else if (e >= last) far_hi += x[r];
+                        else atomicAdd(mine + e, x[r]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const v8 p = pack_step<T>(x, s);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::mma(read_columns<T, DP>(lk[buf], kb * 32 + s * 16, d, lane), p, acc[d]);
+            }
+        }
+        if (t + 1 < ntiles) store(buf ^ 1);
+        __syncthreads();
+    }
+    if (qi < a.Nq) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int at = d * 32 + g * 8 + half * 4;
+                if (at >= a.D) continue;
+                typename Mma<T>::v4 w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = (T)(acc[d][4 * g + j] * a.scale);
+                *reinterpret_cast<typename Mma<T>::v4*>((T*)a.dq + orow + at) = w;
+            }
+    }
+    if (!TABLE) return;
+    // the half waves' lines become one (in place of the bias), with the far sums at its two ends, then the buckets' sums
+    __shared__ float ends[2][4];
+    const float lo = wave_sum(far_lo), hi = wave_sum(far_hi);
+    if (lane == 0) {
+        ends[0][wave] = lo;
+        ends[1][wave] = hi;
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t <= last; t += 256) {
+        float s = 0.f;
+        if (t == 0 || t == last) {
+            const float* e = ends[t ? 1 : 0];
+            s = (e[0] + e[1]) + (e[2] + e[3]);
+        } else {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) s += sums[n * (last + 1) + t];
+        }
+        line[t] = s;
+    }
+    __syncthreads();
+    for (int n = threadIdx.x; n < a.bk.num_buckets; n += 256) {
+        int t0, t1;
+        bucket_entries(a.bk, n, t0, t1);
+        float s = 0.f;
+        for (int t = t0; t < t1; ++t) s += line[t];
+        a.part[(((long long)h * a.B + b) * a.tiles + tile) * a.bk.num_buckets + n] = s;
+    }
+}
+
+// dtable[n][h] = sum over the workgroups of head h, in 64 bits: a workgroup a head, 1024 threads = buckets x slices of the workgroups
+__global__ __launch_bounds__(1024) void attn_table_kernel(const float* part, float* dtable, int buckets, int H, long long parts) {
+    __shared__ double red[1024];
+    const int h = blockIdx.x, slices = 1024 / buckets, n = threadIdx.x % buckets, s = threadIdx.x / buckets;
+    double t = 0.;
+    if (s < slices)
+        for (long long i = s; i < parts; i += slices) t += (double)part[(h * parts + i) * buckets + n];
+    red[threadIdx.x] = t;
+    __syncthreads();
+    if (threadIdx.x >= buckets) return;
+    t = 0.;
+    for (int i = 0; i < slices; ++i) t += red[i * buckets + threadIdx.x];
+    dtable[threadIdx.x * H + h] = (float)t;
+}
+
+// ---- dk, dv: a wave owns 32 keys of one key head, the workgroup (128 keys) walks the queries of every head that shares them, 32 at a
+// time.  Scores here are S = Q K^T (rows = queries, columns = keys): p and ds are again the register operand of dV^T = dO^T P and
+// dK^T = Q^T dS.
+template <class T, int DP>
+__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
+    typedef typename Mma<T>::v8 v8;
+    constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8, QT = 32, PER = (QT * CH + 255) / 256, BN = 128;
+    __shared__ __align__(16) T lq[2][QT * DP];
+    __shared__ __align__(16) T lg[2][QT * DP];
+    __shared__ __align__(16) float ls[2][QT], ld[2][QT];
+    extern __shared__ float line[];
+
+    const int item = xcd_item(blockIdx.x, gridDim.x);
+    const int bh = item / a.tiles, b = bh / a.Hkv, hk = bh % a.Hkv, tile = item % a.tiles, G = a.H / a.Hkv;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+    const int start = seq_start(a, b), len = seq_keys(a, b);
+    const int j0 = tile * BN, w0 = j0 + wave * 32, key = w0 + col;
+    const int reach = line_reach(a.bk), right = line_right(a.bk), last = reach + right;
+    const unsigned char* mask = a.key_mask ? a.key_mask + (long long)b * a.Nk : nullptr;
+    const bool seen = key < len && (!mask || mask[key]);
+    const T* K = (const T*)a.k + b * a.ks[0] + hk * a.ks[2] + (long long)key * a.ks[1];
+    const T* V = (const T*)a.v + b * a.vs[0] + hk * a.vs[2] + (long long)key * a.vs[1];
+    v8 kf[KS], vf[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        const int d = s * 16 + half * 8;
+        kf[s] = load_or_zero<v8>(seen && d < a.D, K + d);
+        vf[s] = load_or_zero<v8>(seen && d < a.D, V + d);
+    }
+    f32x16_t dk[DB], dv[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+        dk[d] = zero16();
+        dv[d] = zero16();
+    }
+    const float c = a.scale * LOG2E;
+    constexpr float small = Mma<T>::shift > 0.f ? 1.f / 32768.f : 1.f;       // 2^-shift
+    // queries that see a key of this workgroup: from i >= j0 - start on if causal, none if the keys do not exist
+    const int i_first = a.causal ? max(0, j0 - start) / QT * QT : 0;
+    const int nt = j0 < len && i_first < a.Nq ? (a.Nq - i_first + QT - 1) / QT : 0;
+    u32x4_t rq[PER], rg[PER];
+    float rs = 0.f, rd = 0.f;
+    auto fetch = [&](int t) {                               // t counts the query tiles of all heads of the group
+        const int h = hk * G + t / nt, i0 = i_first + t % nt * QT;
+        const T* Q = (const T*)a.q + b * a.qs[0] + h * a.qs[2];
+        const T* dO = (const T*)a.dout + b * a.dos[0] + h * a.dos[2];
+        const long long stat = ((long long)b * a.H + h) * a.Nq;
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            const int idx = n * 256 + threadIdx.x, r = idx / CH, ch = idx % CH, i = i0 + r;
+            const bool ok = r < QT && i < a.Nq && ch * 8 < a.D && a.lse[stat + i] != -INFINITY;
+            rq[n] = load_or_zero<u32x4_t>(ok, Q + (long long)i * a.qs[1] + ch * 8);
+            rg[n] = load_or_zero<u32x4_t>(ok, dO + (long long)i * a.dos[1] + ch * 8);
+        }
+        if (threadIdx.x < QT) {
+            const int i = i0 + threadIdx.x;
+            const float l = i < a.Nq ? a.lse[stat + i] : -INFINITY;
+            rs = l == -INFINITY ? INFINITY : l - Mma<T>::shift;             // p = 0 for rows that are empty or past the end
+            rd = i < a.Nq ? a.delta[stat + i] * small : 0.f;
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            const int idx = n * 256 + threadIdx.x, r = idx / CH, ch = idx % CH;
+            if (r >= QT) continue;
+            *reinterpret_cast<u32x4_t*>(&lq[buf][chunk_at<DP>(r, ch) * 8]) = rq[n];
+            *reinterpret_cast<u32x4_t*>(&lg[buf][chunk_at<DP>(r, ch) * 8]) = rg[n];
+        }
+        if (threadIdx.x < QT) {
+            ls[buf][threadIdx.x] = rs;
+            ld[buf][threadIdx.x] = rd;
+        }
+    };
+    const int total = nt * G;
+    if (total > 0) {
+        fetch(0);
+        store(0);
+    }
+    for (int t = 0; t < total; ++t) {
+        const int buf = t & 1, i0 = i_first + t % nt * QT;
+        if (t % nt == 0) {                                   // another head's bias
+            __syncthreads();
+            fill_line(line, a, hk * G + t / nt, 256);
+            __syncthreads();
+        }
+        if (t + 1 < total) fetch(t + 1);
+        f32x16_t x = zero16(), g = zero16();
+#pragma unroll
+        for (int s = 0; s < KS; ++s) x = Mma<T>::mma(read_rows<T, DP>(lq[buf], 0, s, lane), kf[s], x);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) g = Mma<T>::mma(read_rows<T, DP>(lg[buf], 0, s, lane), vf[s], g);
+        const int rel_hi = w0 + 31 - i0 - start, rel_lo = w0 - (i0 + QT - 1) - start;
+        const bool far = rel_hi <= -reach || rel_lo >= right;
+        float sub[16], del[16];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float4 s4 = *reinterpret_cast<const float4*>(&ls[buf][8 * q + 4 * half]);
+            const float4 d4 = *reinterpret_cast<const float4*>(&ld[buf][8 * q + 4 * half]);
+            sub[4 * q] = s4.x; sub[4 * q + 1] = s4.y; sub[4 * q + 2] = s4.z; sub[4 * q + 3] = s4.w;
+            del[4 * q] = d4.x; del[4 * q + 1] = d4.y; del[4 * q + 2] = d4.z; del[4 * q + 3] = d4.w;
+        }
+        if (far) {
+            const float add = rel_hi <= -reach ? line[0] : line[last];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = exp2_hw(fmaf(x[r], c, add - sub[r]));
+        } else {
+            const int at = key - i0 - 4 * half - start + reach;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int e = at - 8 * (r / 4) - r % 4;
+                x[r] = exp2_hw(fmaf(x[r], c, line[min(max(e, 0), last)] - sub[r]));
+            }
+        }
+        const int first = a.causal ? key - start - i0 - 4 * half : -1 << 30;     // the first row of the tile that sees the key, less 4 half
+        if (!seen || first > -4) {
+            const int from = seen ? first : 1 << 30;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (8 * (r / 4) + r % 4 < from) x[r] = 0.f;
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const v8 p = pack_step<T>(x, s);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) dv[d] = Mma<T>::mma(read_columns<T, DP>(lg[buf], s * 16, d, lane), p, dv[d]);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] *= fmaf(g[r], small, -del[r]);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const v8 p = pack_step<T>(x, s);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) dk[d] = Mma<T>::mma(read_columns<T, DP>(lq[buf], s * 16, d, lane), p, dk[d]);
+        }
+        if (t + 1 < total) store(buf ^ 1);
+        __syncthreads();
+    }
+    if (key >= a.Nk) return;
+    const long long row = (((long long)b * a.Nk + key) * a.Hkv + hk) * a.D;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int at = d * 32 + q * 8 + half * 4;
+            if (at >= a.D) continue;
+            typename Mma<T>::v4 w, u;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                w[j] = (T)(dk[d][4 * q + j] * a.scale);
+                u[j] = (T)(dv[d][4 * q + j] * small);
+            }
+            *reinterpret_cast<typename Mma<T>::v4*>((T*)a.dk + row + at) = w;
+            *reinterpret_cast<typename Mma<T>::v4*>((T*)a.dv + row + at) = u;
+        }
+}
+
+template <class T, int DP>
+static int launch_bwd(AttnArgs a, float* dtable, hipStream_t st) {
+    const int last = line_reach(a.bk) + line_right(a.bk);
+    if (a.Nq > 0) {
+        a.tiles = cdiv(a.Nq, 128);
+        const dim3 grid((unsigned)((long long)a.B * a.H * a.tiles));
+        if (dtable) {
+            hipLaunchKernelGGL((attn_dq_kernel<T, DP, true>), grid, dim3(256), sizeof(float) * 9 * (last + 1), st, a);
+            hipLaunchKernelGGL(attn_table_kernel, dim3(a.H), dim3(1024), 0, st, a.part, dtable, a.bk.num_buckets, a.H, (long long)a.B * a.tiles);
+        } else {
+            hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), sizeof(float) * (last + 1), st, a);
+        }
+    }
+    if (a.Nk > 0) {
+        a.tiles = cdiv(a.Nk, 128);
+        hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3((unsigned)((long long)a.B * a.Hkv * a.tiles)), dim3(256), sizeof(float) * (last + 1), st, a);
+    }
+    return 0;
+}
+
+extern "C" int64_t tcvom_attn_bwd_work(const tcvom_attn_desc* d) {
+    if (!d || d->B <= 0 || d->H <= 0 || d->Nq < 0) return 0;
+    return (int64_t)d->B * d->H * d->Nq + (int64_t)d->B * d->H * cdiv(d->Nq, 128) * d->buckets.num_buckets;
+}
+
+extern "C" int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, const void* out,
+                              const void* out_lo, const float* lse, const void* dout, const int64_t* dout_stride, void* dq, void* dk,
+                              void* dv, float* dtable, float* work, int64_t work_floats, void* stream) {
+    AttnArgs a;
+    if (const int rc = attn_check("attn_bwd", d, &a)) return rc;
+    TCVOM_CHECK_ARG(d->B > 0 && d->Nq > 0 && d->Nk > 0, "attn_bwd: B=%d Nq=%d Nk=%d", d->B, d->Nq, d->Nk);
+    TCVOM_CHECK_ARG(q && k && v && table && out && lse && dout && dout_stride && dq && dk && dv && work, "attn_bwd: null tensor");
+    TCVOM_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_lo) && aligned16(dout) &&
+                        aligned16(dq) && aligned16(dk) && aligned16(dv), "attn_bwd: tensors start at multiples of 16 bytes");
+    TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 32) < (1LL << 30) && (long long)d->B * d->Hkv * cdiv(d->Nk, 32) < (1LL << 30),
+                    "attn_bwd: too many rows for one launch");
+    TCVOM_CHECK_ARG(work_floats >= tcvom_attn_bwd_work(d), "attn_bwd: %lld floats of workspace", (long long)work_floats);
+    for (int n = 0; n < 3; ++n) {
+        TCVOM_CHECK_ARG(dout_stride[n] % 8 == 0 && dout_stride[n] >= 0, "attn_bwd: strides are multiples of 8 elements");
+        a.dos[n] = dout_stride[n];
+    }
+    a.q = q; a.k = k; a.v = v; a.table = table; a.out = (void*)out; a.out_lo = (void*)out_lo; a.lse = (float*)lse; a.dout = dout;
+    a.dq = dq; a.dk = dk; a.dv = dv;
+    a.delta = work;
+    a.part = work + (int64_t)d->B * d->H * d->Nq;
+    const hipStream_t st = (hipStream_t)stream;
+    const int DP = attn_width(d->D);
+    if (d->type == TCVOM_TYPE_BF16) {
+        if (DP == 32) launch_bwd<__bf16, 32>(a, dtable, st);
+        else if (DP == 64) launch_bwd<__bf16, 64>(a, dtable, st);
+        else launch_bwd<__bf16, 128>(a, dtable, st);
+    } else {
+        if (DP == 32) launch_bwd<_Float16, 32>(a, dtable, st);
+        else if (DP == 64) launch_bwd<_Float16, 64>(a, dtable, st);
+        else launch_bwd<_Float16, 128>(a, dtable, st);
+    }
+    TCVOM_LAUNCH_CHECK("attn_bwd");
+    return 0;
+}

@@ -1,0 +1,293 @@
+// Backward of the norms around a block (blocknorm.h), reached through tcvom_block_norm_bwd.
+//   a   = dh w2                       dX = dx' + r2 (a - [mean a] - xhat mean(a xhat))          ([..]: LayerNorm only)
+//   dx  = rs dX                       dn = bs g dX,   dg = bs n dX,   n = N1(y)
+//   e   = dn w1                       dy = r1 (e - [mean e] - yhat mean(e yhat))
+//   dw1 = sum dn yhat, db1 = sum dn, dw2 = sum dh xhat, db2 = sum dh over the tokens
+// x' is formed again in 32 bits from x and y (the same bytes as reading the rounded x', none of its rounding); the row statistics come
+// from the forward.  Column sums: a workgroup keeps its channels' sums in registers over its rows, adds its row groups through LDS
+// and writes one partial row; a second kernel adds the partial rows in a fixed order (no atomics: equal calls give equal bits).
+#include "blocknorm.h"
+
+enum { SUM_W1 = 0, SUM_B1, SUM_W2, SUM_B2, SUM_G, SUMS };
+
+template <class TX, class TY, int V, int TPR, int R, int NV, bool LAYER>
+__global__ __launch_bounds__(TPR * R) void block_norm_bwd_kernel(NormArgs a) {
+    constexpr int RED = TPR > 64 ? 4 * R * (TPR / 64) : 1;
+    constexpr int COLS = R > 1 ? TPR * R * V : 1;
+    __shared__ float lds[RED];
+    __shared__ float cols[COLS];
+    int slot = 0;
+    const int lane = threadIdx.x % TPR, g = threadIdx.x / TPR;
+    const int C = a.C;
+    const float inv = 1.f / (float)C;
+    const bool has_y = a.y != nullptr, post = a.w1 != nullptr, pre = a.w2 != nullptr && a.dh != nullptr;
+    const bool token_gate = a.gate && a.gate_rows == 1;
+    float w1[NV][V], b1[NV][V], w2[NV][V], gt[NV][V];
+    float s_w1[NV][V], s_b1[NV][V], s_w2[NV][V], s_b2[NV][V], s_g[NV][V];
+    bool in[NV];
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+        const int c = (n * TPR + lane) * V;
+        in[n] = c < C;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            w1[n][j] = 1.f; b1[n][j] = 0.f; w2[n][j] = 1.f; gt[n][j] = 1.f;
+            s_w1[n][j] = s_b1[n][j] = s_w2[n][j] = s_b2[n][j] = s_g[n][j] = 0.f;
+        }
+        if (!in[n]) continue;
+        if (post) load_vec<float, V>(a.w1 + c, w1[n]);
+        if (LAYER && post && a.b1) load_vec<float, V>(a.b1 + c, b1[n]);
+        if (pre) load_vec<float, V>(a.w2 + c, w2[n]);
+    }
+    auto load_gate = [&](long long grow) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const int c = (n * TPR + lane) * V;
+            if (!in[n]) continue;
+            if (a.gate_f32) load_vec<float, V>((const float*)a.gate + grow * C + c, gt[n]);
+            else load_vec<TY, V>((const TY*)a.gate + grow * C + c, gt[n]);
+        }
+    };
+    // blockIdx.y = gate row (its tokens' sums stay apart), blockIdx.x = workgroup among its tokens
+    const long long group_rows = a.gate && !token_gate ? a.gate_rows : a.T;
+    const long long first = (long long)blockIdx.y * group_rows + (long long)blockIdx.x * a.rows_per_wg;
+    const long long end = (long long)(blockIdx.y + 1) * group_rows;
+    if (a.gate && !token_gate) load_gate(blockIdx.y);
+    for (int k = 0; k < a.rows_per_wg; k += R) {
+        const long long row = first + k + g;
+        const bool live = k + g < a.rows_per_wg && row < end;
+        const long long base = row * C;
+        float x[NV][V], y[NV][V], dX[NV][V], dh[NV][V];
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const int c = (n * TPR + lane) * V;
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[n][j] = y[n][j] = dX[n][j] = dh[n][j] = 0.f;
+            if (live && in[n]) {
+                if (pre) load_vec<TX, V>((const TX*)a.x + base + c, x[n]);
+                if (has_y) load_vec<TY, V>((const TY*)a.y + base + c, y[n]);
+                if (a.dxo) load_vec<TX, V>((const TX*)a.dxo + base + c, dX[n]);
+                if (pre) load_vec<TY, V>((const TY*)a.dh + base + c, dh[n]);
+            }
+        }
+        if (token_gate && live) load_gate(row);
+        float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
+        if (live) st = *reinterpret_cast<const float4*>(a.stats + row * 4);
+        const float m1 = st.x, r1 = st.y, m2 = st.z, r2 = st.w;
+        // y <- yhat, x <- xhat of x'
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+            if (in[n])
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    if (post) y[n][j] = (y[n][j] - m1) * r1;
+                    const float t = post ? y[n][j] * w1[n][j] + b1[n][j] : y[n][j];
+                    const float x1 = has_y ? a.rs * x[n][j] + a.bs * gt[n][j] * t : x[n][j];
+                    x[n][j] = (x1 - m2) * r2;
+                }
+        if (pre) {
+            float s[2] = {0.f, 0.f};
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+                if (in[n])
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        if (live) { s_w2[n][j] += dh[n][j] * x[n][j]; s_b2[n][j] += dh[n][j]; }
+                        dh[n][j] *= w2[n][j];
+                        s[0] += dh[n][j] * x[n][j];
+                        s[1] += dh[n][j];
+                    }
+            group_sum<TPR, R, 2>(s, lds, slot);
+            const float p = s[0] * inv, q = LAYER ? s[1] * inv : 0.f;
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+#pragma unroll
+                for (int j = 0; j < V; ++j) dX[n][j] += r2 * (dh[n][j] - q - x[n][j] * p);
+        }
+        if (live)
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const int c = (n * TPR + lane) * V;
+                if (!in[n]) continue;
+                float o[V];
+#pragma unroll
+                for (int j = 0; j < V; ++j) o[j] = has_y ? a.rs * dX[n][j] : dX[n][j];
+                store_vec<TX, V>((TX*)a.dx + base + c, o);
+            }
+        if (!has_y) continue;
+        float s[2] = {0.f, 0.f};
+        float dg[NV][V];
+#pragma unroll
+        for (int n = 0; n < NV; ++n)
+            if (in[n])
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float t = post ? y[n][j] * w1[n][j] + b1[n][j] : y[n][j];
+                    dg[n][j] = a.bs * t * dX[n][j];
+                    const float dn = a.bs * gt[n][j] * dX[n][j];
+                    if (live) { s_g[n][j] += dg[n][j]; s_w1[n][j] += dn * y[n][j]; s_b1[n][j] += dn; }
+                    dX[n][j] = dn * w1[n][j];
+                    s[0] += dX[n][j] * y[n][j];
+                    s[1] += dX[n][j];
+                }
+        float p = 0.f, q = 0.f;
+        if (post) {
+            group_sum<TPR, R, 2>(s, lds, slot);
+            p = s[0] * inv;
+            q = LAYER ? s[1] * inv : 0.f;
+        }
+        if (!live) continue;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const int c = (n * TPR + lane) * V;
+            if (!in[n]) continue;
+            float o[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] = post ? r1 * (dX[n][j] - q - y[n][j] * p) : dX[n][j];
+            store_vec<TY, V>((TY*)a.dy + base + c, o);
+            if (token_gate && a.dgate) {
+                if (a.gate_f32) store_vec<float, V>((float*)a.dgate + base + c, dg[n]);
+                else store_vec<TY, V>((TY*)a.dgate + base + c, dg[n]);
+            }
+        }
+    }
+    float* part = a.part + ((long long)blockIdx.y * gridDim.x + blockIdx.x) * SUMS * C;
+    auto flush = [&](int q, float (&t)[NV][V]) {
+        if (!(a.want >> q & 1)) return;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const int c = (n * TPR + lane) * V;
+            if constexpr (R > 1) {
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < V; ++j) cols[threadIdx.x * V + j] = t[n][j];
+                __syncthreads();
+                if (g == 0)
+                    for (int i = 1; i < R; ++i)
+#pragma unroll
+                        for (int j = 0; j < V; ++j) t[n][j] += cols[(i * TPR + lane) * V + j];
+            }
+            if (g == 0 && in[n]) store_vec<float, V>(part + (long long)q * C + c, t[n]);
+        }
+    };
+    flush(SUM_W1, s_w1);
+    flush(SUM_W2, s_w2);
+    if constexpr (LAYER) {
+        flush(SUM_B1, s_b1);
+        flush(SUM_B2, s_b2);
+    }
+    flush(SUM_G, s_g);
+}
+
+// out[q] = sum of the partial rows: 64 channels x 16 slices of the rows a workgroup; blockIdx.y = which output
+struct NormSums { float* out[SUMS - 1]; void* dgate; int gate_f32, gate_type; int parts, groups, C, nq; int q[SUMS]; };
+__global__ __launch_bounds__(1024) void block_norm_sums_kernel(const float* part, NormSums s) {
+    __shared__ float red[16][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
+    const bool is_gate = (int)blockIdx.y >= s.nq;            // rows nq.. of the grid: one gate row each
+    const int q = is_gate ? (int)SUM_G : s.q[blockIdx.y];
+    const int lo = is_gate ? ((int)blockIdx.y - s.nq) * s.parts : 0, hi = is_gate ? lo + s.parts : s.parts * s.groups;
+    float t = 0.f;
+    if (c < s.C)
+        for (int i = lo + slice; i < hi; i += 16) t += part[((long long)i * SUMS + q) * s.C + c];
+    red[slice][threadIdx.x & 63] = t;
+    __syncthreads();
+    if (slice || c >= s.C) return;
+    t = 0.f;
+    for (int i = 0; i < 16; ++i) t += red[i][threadIdx.x];
+    if (!is_gate) { s.out[q][c] = t; return; }
+    const long long at = (long long)((int)blockIdx.y - s.nq) * s.C + c;
+    if (s.gate_f32) ((float*)s.dgate)[at] = t;
+    else if (s.gate_type == TCVOM_TYPE_BF16) ((__bf16*)s.dgate)[at] = (__bf16)t;
+    else if (s.gate_type == TCVOM_TYPE_F16) ((_Float16*)s.dgate)[at] = (_Float16)t;
+    else ((float*)s.dgate)[at] = t;
+}
+
+// workgroups of a launch: at most this many partial rows in all (two workgroups a CU), at least one a gate row
+static int bwd_wgs(int64_t T, int64_t groups, int R, int threads) {
+    const int64_t rows = T / groups;
+    const int64_t want = (int64_t)256 * (threads > 256 ? 1 : 2);
+    int64_t n = (want + groups - 1) / groups;
+    const int64_t most = (rows + R - 1) / R;
+    return (int)(n < 1 ? 1 : n > most ? most : n);
+}
+static void bwd_shape(int C, bool vec, int* R, int* threads) {
+    *R = vec ? (C <= 128 ? 16 : C <= 1024 ? 4 : 1) : (C <= 512 ? 4 : 1);
+    *threads = C <= 4096 ? 256 : 512;
+}
+
+extern "C" int64_t tcvom_block_norm_bwd_work(int64_t T, int32_t C, int64_t gate_groups) {
+    if (T <= 0 || C <= 0 || gate_groups <= 0) return 0;
+    // the larger of the aligned and the unaligned form: the caller need not know which one runs
+    int64_t most = 0;
+    for (int v = 0; v < 2; ++v) {
+        int R, threads;
+        bwd_shape(C, v, &R, &threads);
+        const int64_t n = (int64_t)bwd_wgs(T, gate_groups, R, threads) * gate_groups;
+        most = n > most ? n : most;
+    }
+    return most * SUMS * C;
+}
+
+extern "C" int tcvom_block_norm_bwd(const void* x, const void* y, const float* post_weight, const float* post_bias, const void* gate,
+                                    int32_t gate_f32, int64_t gate_rows, const float* pre_weight, float branch_scale, float residual_scale,
+                                    int32_t layer, const float* stats, const void* dx_out, const void* dh, void* dx, void* dy,
+                                    float* dpost_weight, float* dpost_bias, void* dgate, float* dpre_weight, float* dpre_bias, float* work,
+                                    int64_t work_floats, int64_t T, int32_t C, int32_t x_type, int32_t y_type, void* stream) {
+    TCVOM_CHECK_ARG(x && dx && stats && T >= 0 && C > 0 && C <= TCVOM_MAX_NORM_CHANNELS, "block_norm_bwd: T=%lld C=%d (1..%d)", (long long)T,
+                    C, TCVOM_MAX_NORM_CHANNELS);
+    TCVOM_CHECK_ARG(norm_types_ok(x_type, y_type), "block_norm_bwd: types %d, %d", x_type, y_type);
+    TCVOM_CHECK_ARG(y ? dy != nullptr : !post_weight && !gate, "block_norm_bwd: outputs / weights do not match y");
+    TCVOM_CHECK_ARG(!gate || (gate_rows > 0 && T % gate_rows == 0), "block_norm_bwd: %lld tokens a gate row", (long long)gate_rows);
+    TCVOM_CHECK_ARG((!dpost_weight && !dpost_bias) || post_weight, "block_norm_bwd: gradient of an absent post norm");
+    TCVOM_CHECK_ARG((!dpre_weight && !dpre_bias) || (pre_weight && dh), "block_norm_bwd: gradient of an absent pre norm");
+    TCVOM_CHECK_ARG(layer || (!post_bias && !dpost_bias && !dpre_bias), "block_norm_bwd: a bias belongs to LayerNorm");
+    TCVOM_CHECK_ARG(!dgate || gate, "block_norm_bwd: gradient of an absent gate");
+    TCVOM_CHECK_ARG(T < (1LL << 31), "block_norm_bwd: %lld tokens", (long long)T);
+    if (T == 0) return 0;
+    const bool token_gate = gate && gate_rows == 1 && T > 1;
+    const int64_t groups = gate && !token_gate ? T / gate_rows : 1;
+    TCVOM_CHECK_ARG(groups <= 32768, "block_norm_bwd: %lld gate rows of several tokens (at most 32768)", (long long)groups);
+    TCVOM_CHECK_ARG(work && work_floats >= tcvom_block_norm_bwd_work(T, C, groups), "block_norm_bwd: %lld floats of workspace",
+                    (long long)work_floats);
+    NormArgs a = {};
+    a.x = x; a.y = y; a.w1 = post_weight; a.b1 = post_bias; a.w2 = pre_weight;
+    a.gate = gate; a.gate_f32 = gate_f32; a.gate_rows = gate ? (token_gate ? 1 : gate_rows) : 1;
+    a.bs = branch_scale; a.rs = residual_scale; a.T = T; a.C = C;
+    a.stats = (float*)stats; a.dxo = dx_out; a.dh = dh; a.dx = dx; a.dy = dy; a.part = work;
+    a.dgate = token_gate ? dgate : nullptr;
+    a.want = (dpost_weight ? 1 << SUM_W1 : 0) | (dpost_bias ? 1 << SUM_B1 : 0) | (dpre_weight ? 1 << SUM_W2 : 0) |
+             (dpre_bias ? 1 << SUM_B2 : 0) | (dgate && !token_gate ? 1 << SUM_G : 0);
+    const bool vec = C % 8 == 0 && aligned16(x) && aligned16(y) && aligned16(post_weight) && aligned16(post_bias) && aligned16(gate) &&
+                     aligned16(pre_weight) && aligned16(dx_out) && aligned16(dh) && aligned16(dx) && aligned16(dy) && aligned16(a.dgate) &&
+                     aligned16(work);
+    int R0, threads0;
+    bwd_shape(C, vec, &R0, &threads0);
+    const int wgs = bwd_wgs(T, groups, R0, threads0);
+    const int64_t rows = T / groups;
+    const hipStream_t st = (hipStream_t)stream;
+    const int per = cdiv(cdiv(rows, wgs), R0) * R0;
+    const int used = cdiv(rows, per);                        // <= wgs: rounding up to whole row groups can leave some without rows
+    a.rows_per_wg = per;
+#define BWD(TX, TY, V, TPR, R, NV)                                                                                      \
+    do {                                                                                                                \
+        const dim3 grid(used, (unsigned)groups);                                                                        \
+        if (layer) hipLaunchKernelGGL((block_norm_bwd_kernel<TX, TY, V, TPR, R, NV, true>), grid, dim3(TPR * R), 0, st, a);  \
+        else hipLaunchKernelGGL((block_norm_bwd_kernel<TX, TY, V, TPR, R, NV, false>), grid, dim3(TPR * R), 0, st, a);       \
+    } while (0)
+    NORM_TYPES(BWD);
+#undef BWD
+    TCVOM_LAUNCH_CHECK("block_norm_bwd");
+    if (!a.want) return 0;
+    NormSums s = {};
+    float* outs[SUMS - 1] = {dpost_weight, dpost_bias, dpre_weight, dpre_bias};
+    for (int q = 0; q < SUMS - 1; ++q) {
+        s.out[q] = outs[q];
+        if (outs[q]) s.q[s.nq++] = q;
+    }
+    s.dgate = dgate; s.gate_f32 = gate_f32; s.gate_type = y_type; s.parts = used; s.groups = (int)groups; s.C = C;
+    const int gate_blocks = a.want >> SUM_G & 1 ? (int)groups : 0;
+    hipLaunchKernelGGL(block_norm_sums_kernel, dim3(cdiv(C, 64), s.nq + gate_blocks), dim3(1024), 0, st, work, s);
+    TCVOM_LAUNCH_CHECK("block_norm_sums");
+    return 0;
+}

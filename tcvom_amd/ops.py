@@ -1681,3 +1681,9 @@ class _GcaAttention(torch.autograd.Function):
 
 
 gca_attention = _GcaAttention.apply
+
+
+# =============================================================================================
+# Token sequences (token_ops.py)
+# =============================================================================================
+from .token_ops import biased_attention, block_norm, relative_position_bias  # noqa: E402,F401

@@ -1,0 +1,355 @@
+"""Operators on token sequences: a learned relative position bias, the attention that adds it inside, the norms around a block.
+
+They stand beside the attention and the norms of `ops` (re-exported there): TAM and GuidedCxtAtten know no positions and work on maps,
+BatchNorm / GroupNorm normalise over pixels; a block over tokens -- the frames of a clip, the pixels of a stride-8 or -16 map --
+needs these.  The reference has no counterpart.
+
+    h = ops.block_norm(x, None, pre_weight=w0)[1]
+    y = attention_projection(ops.biased_attention(q(h), k(h), v(h), table))
+    x, h = ops.block_norm(x, y, post_weight=w1, gate=g, pre_weight=w2)        # h enters the next block
+
+Element types are arguments: bf16, fp16 and, for the bias matrix and the norms, fp32, in either build of the library.  16-bit results are
+rounded to nearest even without saturation.  Gradients are added in a fixed order: equal calls give equal bits.  First derivatives
+only.
+"""
+import ctypes as C
+import functools
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _check_cuda(name, *tensors):
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not torch.is_tensor(t):
+            raise TypeError('%s: expected a tensor, got %s' % (name, type(t).__name__))
+        if not t.is_cuda:
+            raise RuntimeError('tcvom_amd ops run on the GPU through libtcvom_hip.so only (no CPU fallback); %s got a %s tensor'
+                               % (name, t.device))
+        if dev is not None and t.device != dev:
+            raise RuntimeError('%s: tensors on %s and %s' % (name, dev, t.device))
+        dev = t.device
+
+
+def _c(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+# =============================================================================================
+# buckets
+# =============================================================================================
+@functools.lru_cache(maxsize=64)
+def rel_buckets(num_buckets, max_distance, bidirectional):
+    """struct tcvom_rel_buckets: `num_buckets` buckets (half of them for each direction if bidirectional).  Half the buckets of a side
+    hold one distance each; bucket exact + k of the others starts at the smallest distance d with
+    (d / exact)^m >= (max_distance / exact)^k, m = their number -- in whole numbers, so that no border depends on a logarithm's
+    rounding."""
+    side = num_buckets // 2 if bidirectional else num_buckets
+    if num_buckets < 2 or num_buckets > L.MAX_BUCKETS or (bidirectional and num_buckets % 2) or side < 2:
+        raise ValueError('%d buckets: 2..%d, even and at least 4 if bidirectional' % (num_buckets, L.MAX_BUCKETS))
+    exact = side // 2
+    m = side - exact
+    if not exact < max_distance <= L.MAX_BUCKET_REACH:
+        raise ValueError('max_distance %d: more than the %d distances with a bucket of their own, at most %d'
+                         % (max_distance, exact, L.MAX_BUCKET_REACH))
+    starts, d = [], exact
+    for k in range(m):
+        while d ** m * exact ** k < max_distance ** k * exact ** m:
+            d += 1
+        starts.append(d)
+    b = L.RelBuckets(num_buckets, int(bidirectional), exact, m)
+    b.starts[:m] = starts
+    return b
+
+
+def _check_table(name, table):
+    _check_cuda(name, table)
+    if table.dim() != 2 or table.dtype != torch.float32:
+        raise ValueError('%s: the table is fp32 [buckets, heads], got %s %s' % (name, table.dtype, tuple(table.shape)))
+
+
+# =============================================================================================
+# the bias as a matrix
+# =============================================================================================
+class _RelBias(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, buckets, q_len, k_len, q_start, dtype):
+        heads = table.shape[1]
+        with torch.cuda.device(table.device):
+            out = torch.empty((heads, q_len, k_len), dtype=dtype, device=table.device)
+            L.call('tcvom_relbias_fwd', L.ptr(_c(table)), L.ptr(out), C.byref(buckets), heads, q_len, k_len, q_start, _TYPES[dtype],
+                   L.stream_ptr())
+        ctx.args = (buckets, heads, q_len, k_len, q_start, dtype)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        buckets, heads, q_len, k_len, q_start, dtype = ctx.args
+        with torch.cuda.device(dout.device):
+            dtable = torch.empty((buckets.num_buckets, heads), dtype=torch.float32, device=dout.device)
+            if q_len == 0 or k_len == 0:
+                return dtable.zero_(), None, None, None, None, None
+            n = L.call('tcvom_relbias_bwd_work', C.byref(buckets), heads, q_len)
+            work = torch.empty(n, dtype=torch.float32, device=dout.device)
+            L.call('tcvom_relbias_bwd', L.ptr(_c(dout)), L.ptr(dtable), L.ptr(work), n, C.byref(buckets), heads, q_len, k_len, q_start,
+                   _TYPES[dtype], L.stream_ptr())
+        return dtable, None, None, None, None, None
+
+
+def relative_position_bias(table, q_len, k_len, max_distance=128, bidirectional=True, q_start=0, dtype=torch.float32):
+    """bias[h, i, j] = table[bucket(j - i - q_start), h]: [heads, q_len, k_len] of `dtype`, to be added to attention logits.
+
+    table: fp32 [buckets, heads].  Bidirectional: half the buckets for keys behind the query, half for keys after it (distance
+    |j - i - q_start|); one-sided: every key after the query counts as distance 0.  The first half of a side's buckets hold one
+    distance each, the others grow geometrically up to max_distance (at most 1024), the last holds everything beyond.  q_start:
+    position of the first query."""
+    _check_table('relative_position_bias', table)
+    if dtype not in _TYPES:
+        raise TypeError('relative_position_bias: dtype %s' % dtype)
+    if q_len < 0 or k_len < 0:
+        raise ValueError('relative_position_bias: lengths %d, %d' % (q_len, k_len))
+    buckets = rel_buckets(table.shape[0], int(max_distance), bool(bidirectional))
+    return _RelBias.apply(table, buckets, int(q_len), int(k_len), int(q_start), dtype)
+
+
+# =============================================================================================
+# attention with the bias inside
+# =============================================================================================
+def _rows16(t):
+    """[B, N, heads, width] as the kernels read it: innermost stride 1, the others multiples of 8, 16-byte aligned; a copy if not."""
+    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t):
+    return [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])]
+
+
+def _attn_desc(q, k, v, buckets, causal, scale, k_lens, key_mask, q_start, q_starts):
+    d = L.AttnDesc()
+    d.B, d.Nq, d.H, d.D = q.shape
+    d.Nk, d.Hkv = k.shape[1], k.shape[2]
+    d.type, d.causal, d.scale, d.q_start = _TYPES[q.dtype], int(causal), scale, q_start
+    d.q_stride[:], d.k_stride[:], d.v_stride[:] = _strides(q), _strides(k), _strides(v)
+    d.k_lens = None if k_lens is None else k_lens.data_ptr()
+    d.q_starts = None if q_starts is None else q_starts.data_ptr()
+    d.key_mask = None if key_mask is None else key_mask.data_ptr()
+    d.buckets = buckets
+    return d
+
+
+class _BiasedAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, buckets, causal, scale, k_lens, key_mask, q_start, q_starts):
+        q, k, v, table = _rows16(q), _rows16(k), _rows16(v), _c(table)
+        train = any(ctx.needs_input_grad[:4])
+        with torch.cuda.device(q.device):
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            lse = out_lo = work = None
+            if train:
+                lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
+                if ctx.needs_input_grad[3]:
+                    out_lo = torch.empty_like(out)
+            d = _attn_desc(q, k, v, buckets, causal, scale, k_lens, key_mask, q_start, q_starts)
+            n = L.call('tcvom_attn_fwd_work', C.byref(d))
+            if n:
+                work = torch.empty(n, dtype=torch.float32, device=q.device)
+            L.call('tcvom_attn_fwd', C.byref(d), L.ptr(q), L.ptr(k), L.ptr(v), L.ptr(table), L.ptr(out), L.ptr(out_lo), L.ptr(lse),
+                   L.ptr(work), n, L.stream_ptr())
+        if train:
+            ctx.save_for_backward(q, k, v, table, out, out_lo, lse, k_lens, key_mask, q_starts)
+            ctx.args = (buckets, causal, scale, q_start)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, out, out_lo, lse, k_lens, key_mask, q_starts = ctx.saved_tensors
+        buckets, causal, scale, q_start = ctx.args
+        none = (None,) * 7
+        with torch.cuda.device(q.device):
+            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+            dtable = torch.empty_like(table) if ctx.needs_input_grad[3] else None
+            if q.numel() == 0 or k.numel() == 0:
+                return (dq.zero_(), dk.zero_(), dv.zero_(), None if dtable is None else dtable.zero_()) + none
+            dout = _rows16(dout)
+            d = _attn_desc(q, k, v, buckets, causal, scale, k_lens, key_mask, q_start, q_starts)
+            n = L.call('tcvom_attn_bwd_work', C.byref(d))
+            work = torch.empty(n, dtype=torch.float32, device=q.device)
+            L.call('tcvom_attn_bwd', C.byref(d), L.ptr(q), L.ptr(k), L.ptr(v), L.ptr(table), L.ptr(out), L.ptr(out_lo), L.ptr(lse),
+                   L.ptr(dout), (C.c_int64 * 3)(*_strides(dout)), L.ptr(dq), L.ptr(dk), L.ptr(dv), L.ptr(dtable), L.ptr(work), n,
+                   L.stream_ptr())
+        return (dq, dk, dv, dtable) + none
+
+
+def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causal=False, scale=None, k_lens=None, key_mask=None,
+                     q_start=0):
+    """softmax(scale q k^T + bias) v with bias = relative_position_bias(table, ...), never formed as a matrix: [B, Nq, H, D].
+
+    q [B, Nq, H, D], k / v [B, Nk, Hkv, D], bf16 or fp16, D a multiple of 8 up to 128; H a multiple of Hkv (consecutive heads share
+    keys; at most 64 of them for 32 queries and fewer).  Any strides with contiguous rows of D; others are copied.
+    table fp32 [buckets, H] and max_distance as in relative_position_bias; bidirectional: default not causal.
+    scale: default D ** -0.5, positive.  Key j sits at position j, query i of sequence b at i + q_start[b] (an int, or int32 [B]).
+    Query i sees key j if j < k_lens[b] (int32 [B]; clamped to 0..Nk), key_mask[b, j] (bool or uint8 [B, Nk]) and, causal,
+    j <= i + q_start[b].  A query that sees nothing gives zeros and no gradient.  What lies behind the lengths or under the mask
+    may hold anything, NaN included.  For one new token against caches of Nk slots: k_lens = lengths with the new token,
+    q_start = k_lens - 1, causal.
+
+    Gradients of q, k, v and table.  Probabilities and their gradients are rounded to the 16-bit type as operands of the matrix
+    products, everything else is held in 32 bits."""
+    name = 'biased_attention'
+    _check_cuda(name, q, k, v, table, k_lens, key_mask)
+    _check_table(name, table)
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError('%s: q, k, v are all bf16 or all fp16, got %s, %s, %s' % (name, q.dtype, k.dtype, v.dtype))
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError('%s: q [B, Nq, H, D], k and v [B, Nk, Hkv, D]; got %s, %s, %s' % (name, tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    B, Nq, H, D = q.shape
+    Nk, Hkv = k.shape[1:3]
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError('%s: head width %d (a multiple of 8 up to 128)' % (name, D))
+    if H == 0 or Hkv == 0 or H % Hkv:
+        raise ValueError('%s: %d heads on %d key heads' % (name, H, Hkv))
+    if table.shape[1] != H:
+        raise ValueError('%s: the table has %d heads, q %d' % (name, table.shape[1], H))
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError('%s: scale %g' % (name, scale))
+    q_starts = None
+    if torch.is_tensor(q_start):
+        q_starts, q_start = q_start, 0
+    for what, t in (('k_lens', k_lens), ('q_start', q_starts)):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (B,)):
+            raise ValueError('%s: %s is int32 [%d], got %s %s' % (name, what, B, t.dtype, tuple(t.shape)))
+    _check_cuda(name, q, q_starts)
+    if key_mask is not None:
+        if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (B, Nk):
+            raise ValueError('%s: key_mask is bool or uint8 [%d, %d], got %s %s' % (name, B, Nk, key_mask.dtype, tuple(key_mask.shape)))
+        key_mask = _c(key_mask).view(torch.uint8)
+    if not -(1 << 29) <= int(q_start) <= 1 << 29:
+        raise ValueError('%s: q_start %d' % (name, q_start))
+    buckets = rel_buckets(table.shape[0], int(max_distance), bool(not causal if bidirectional is None else bidirectional))
+    return _BiasedAttention.apply(q, k, v, table, buckets, bool(causal), scale, _c(k_lens), key_mask, int(q_start), _c(q_starts))
+
+
+# =============================================================================================
+# norms around a block
+# =============================================================================================
+class _BlockNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, post_weight, post_bias, gate, pre_weight, pre_bias, gate_rows, branch_scale, residual_scale, eps, layer):
+        ctx.set_materialize_grads(False)
+        x, y, post_weight, post_bias, gate, pre_weight, pre_bias = (_c(t) for t in (x, y, post_weight, post_bias, gate, pre_weight, pre_bias))
+        Cc = x.shape[-1]
+        T = x.numel() // Cc
+        y_type = x.dtype if y is None else y.dtype
+        train = any(ctx.needs_input_grad[:7])
+        with torch.cuda.device(x.device):
+            xo = None if y is None else torch.empty_like(x)
+            h = None if pre_weight is None else torch.empty(x.shape, dtype=y_type, device=x.device)
+            stats = torch.empty((T, 4), dtype=torch.float32, device=x.device) if train else None
+            L.call('tcvom_block_norm_fwd', L.ptr(x), L.ptr(y), L.ptr(post_weight), L.ptr(post_bias), L.ptr(gate),
+                   int(gate is not None and gate.dtype == torch.float32), gate_rows, L.ptr(pre_weight), L.ptr(pre_bias), branch_scale,
+                   residual_scale, eps, int(layer), L.ptr(xo), L.ptr(h), L.ptr(stats), T, Cc, _TYPES[x.dtype], _TYPES[y_type],
+                   L.stream_ptr())
+        if train:
+            ctx.save_for_backward(x, y, post_weight, post_bias, gate, pre_weight, stats)
+            ctx.args = (gate_rows, branch_scale, residual_scale, layer, T, Cc, y_type)
+        return xo, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dxo, dh):
+        x, y, post_weight, post_bias, gate, pre_weight, stats = ctx.saved_tensors
+        gate_rows, branch_scale, residual_scale, layer, T, Cc, y_type = ctx.args
+        need = ctx.needs_input_grad
+        if dxo is None and dh is None:
+            return (None,) * 12
+        with torch.cuda.device(x.device):
+            dxo, dh = _c(dxo), _c(dh)
+
+            def like(t, wanted=True):
+                return torch.empty_like(t) if t is not None and wanted else None
+
+            pre = dh is not None
+            dx, dy = like(x), like(y)
+            dw1, db1, dg = like(post_weight, need[2]), like(post_bias, need[3]), like(gate, need[4])
+            dw2 = like(pre_weight, need[5] and pre)
+            db2 = torch.empty(Cc, dtype=torch.float32, device=x.device) if need[6] and pre else None
+            if T == 0:
+                return tuple(None if t is None else t.zero_() for t in (dx, dy, dw1, db1, dg, dw2, db2)) + (None,) * 5
+            groups = T // gate_rows if gate is not None and gate_rows > 1 else 1
+            n = L.call('tcvom_block_norm_bwd_work', T, Cc, groups)
+            work = torch.empty(n, dtype=torch.float32, device=x.device)
+            L.call('tcvom_block_norm_bwd', L.ptr(x), L.ptr(y), L.ptr(post_weight), L.ptr(post_bias), L.ptr(gate),
+                   int(gate is not None and gate.dtype == torch.float32), gate_rows, L.ptr(pre_weight), branch_scale, residual_scale,
+                   int(layer), L.ptr(stats), L.ptr(dxo), L.ptr(dh), L.ptr(dx), L.ptr(dy), L.ptr(dw1), L.ptr(db1), L.ptr(dg), L.ptr(dw2),
+                   L.ptr(db2), L.ptr(work), n, T, Cc, _TYPES[x.dtype], _TYPES[y_type], L.stream_ptr())
+        return (dx, dy, dw1, db1, dg, dw2, db2) + (None,) * 5
+
+
+def _gate_rows(x, gate):
+    """Tokens that share a row of the gate."""
+    lead = x.shape[:-1]
+    g = tuple(gate.shape[:-1])
+    if gate.shape[-1:] != x.shape[-1:]:
+        raise ValueError('block_norm: a gate of %s for %s' % (tuple(gate.shape), tuple(x.shape)))
+    g = g + (1,) * (len(lead) - len(g))
+    n = len(g)
+    while n and g[n - 1] == 1:
+        n -= 1
+    if len(g) != len(lead) or g[:n] != tuple(lead[:n]):
+        raise ValueError('block_norm: a gate of %s for %s: one of each channel, of each leading index, or of each token'
+                         % (tuple(gate.shape), tuple(x.shape)))
+    return max(math.prod(lead[n:]), 1)
+
+
+def block_norm(x, y, post_weight=None, post_bias=None, gate=None, branch_scale=1.0, residual_scale=1.0, pre_weight=None, pre_bias=None,
+               kind='rms', eps=1e-6):
+    """(x', h): x' = residual_scale x + branch_scale gate N(y; post), h = N(x'; pre), in one pass.
+
+    x [..., C]: the residual stream, y (same shape): what a block made of the last h; N: RMSNorm (kind 'rms') or LayerNorm ('layer') over
+    the C <= 8192 channels, weights and biases fp32 [C] (biases with LayerNorm only).  Without post_weight y enters as it is; without
+    pre_weight h is None; y None: (x, N(x; pre)), the norm in front of the first block.  h is formed from x' before x' is rounded.
+    gate: [C], [lead..., C] where lead are the first dimensions of x (a gate of each sample), or the shape of x; fp32 or y's type.
+    x and y of one type (fp32, bf16, fp16), or x fp32 with a 16-bit y; h has y's type.
+
+    Gradients of every tensor argument."""
+    name = 'block_norm'
+    _check_cuda(name, x, y, post_weight, post_bias, gate, pre_weight, pre_bias)
+    if kind not in ('rms', 'layer'):
+        raise ValueError('%s: kind %r' % (name, kind))
+    if x.dtype not in _TYPES or (y is not None and (y.dtype not in _TYPES or (y.dtype != x.dtype and x.dtype != torch.float32))):
+        raise TypeError('%s: x %s, y %s' % (name, x.dtype, None if y is None else y.dtype))
+    if x.dim() < 1 or not 0 < x.shape[-1] <= L.MAX_NORM_CHANNELS:
+        raise ValueError('%s: %s (1..%d channels)' % (name, tuple(x.shape), L.MAX_NORM_CHANNELS))
+    if y is None:
+        if pre_weight is None or post_weight is not None or post_bias is not None or gate is not None or residual_scale != 1.0:
+            raise ValueError('%s: without y there is the pre norm only' % name)
+    elif y.shape != x.shape:
+        raise ValueError('%s: x %s, y %s' % (name, tuple(x.shape), tuple(y.shape)))
+    for w, b, what in ((post_weight, post_bias, 'post'), (pre_weight, pre_bias, 'pre')):
+        for t in (w, b):
+            if t is not None and (t.dtype != torch.float32 or t.shape != x.shape[-1:]):
+                raise ValueError('%s: the %s weight and bias are fp32 [%d], got %s %s' % (name, what, x.shape[-1], t.dtype, tuple(t.shape)))
+        if b is not None and (w is None or kind != 'layer'):
+            raise ValueError('%s: a %s bias goes with LayerNorm and a weight' % (name, what))
+    rows = 1
+    if gate is not None:
+        if gate.dtype not in (torch.float32, y.dtype):
+            raise TypeError('%s: gate %s with y %s' % (name, gate.dtype, y.dtype))
+        rows = _gate_rows(x, gate)
+        if rows > 1 and x.numel() // x.shape[-1] // rows > 32768:
+            raise ValueError('%s: %d gate rows of several tokens (at most 32768)' % (name, x.numel() // x.shape[-1] // rows))
+    xo, h = _BlockNorm.apply(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, rows, float(branch_scale), float(residual_scale),
+                             float(eps), kind == 'layer')
+    return (x if y is None else xo), h

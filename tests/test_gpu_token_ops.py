@@ -1,0 +1,344 @@
+"""GPU parity of the token operators (tcvom_amd/token_ops.py): relative position bias, attention with it, norms around a block, forward
+and gradients against plain implementations in 64 bits on the CPU.
+
+Tolerances, from the roundings alone.  u = eps / 2 of the 16-bit type: half a step.
+  * bias matrix: one rounding, u |value|.  Table gradient: fp32 sums, 2^-24 a partial sum, far below 1e-6 of the sum of magnitudes.
+  * norms: 32-bit arithmetic and one rounding at the end, u |value| plus a few 2^-24 of the terms' sizes, taken as 1e-6 of the largest.
+  * attention: out = sum p v with p rounded to 16 bits, relative error u each: at most u sum |p| |v|, then the rounding of the result, u |out|;
+    the same for gradients with the magnitudes of what is summed (`slack` below computes those sums).  The 32-bit part (scores of
+    magnitude |x| <= 64 in base 2, hardware exponentials) adds 2^-24 |x| relative, taken as 2e-5.
+"""
+import math
+
+import pytest
+import torch
+
+from tcvom_amd import _lib as L
+from tcvom_amd import ops
+from tcvom_amd.token_ops import rel_buckets
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+HALF = [torch.bfloat16, torch.float16]
+ids = lambda t: str(t).replace('torch.', '') if isinstance(t, torch.dtype) else None  # noqa: E731
+
+
+def step(dt):
+    return 2.0 ** -24 if dt == torch.float32 else torch.finfo(dt).eps / 2
+
+
+def rnd(*shape, seed=0, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(shape, generator=g, dtype=torch.float64) * std
+
+
+def bucket_matrix(n, max_distance, bidirectional, nq, nk, start):
+    """Bucket of every (query, key) by the definition, one element at a time."""
+    b = rel_buckets(n, max_distance, bidirectional)
+    side = n // 2 if bidirectional else n
+
+    def one(rel):
+        d = abs(rel) if bidirectional else max(-rel, 0)
+        k = d if d < b.exact else b.exact - 1 + sum(1 for s in b.starts[:b.n_starts] if s <= d)
+        return k + (side if bidirectional and rel > 0 else 0)
+
+    lo = -(nq - 1) - start
+    line = torch.tensor([one(r) for r in range(lo, nk - start)] or [0])
+    i, j = torch.arange(nq)[:, None], torch.arange(nk)[None, :]
+    return line[(j - i - start) - lo]
+
+
+def close(got, want, bound, what=''):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape, what
+    assert torch.isfinite(got).all(), what
+    over = ((got - want).abs() - bound).max().item() if want.numel() else 0.0
+    assert over <= 0, '%s: %.3g over a bound of %.3g' % (what, over, float(torch.as_tensor(bound).max()))
+
+
+# --------------------------------------------------------------------------------------------- bias matrix
+BIAS = [
+    # heads, q_len, k_len, buckets, max_distance, bidirectional, q_start
+    (1, 1, 1, 32, 128, True, 0),
+    (3, 7, 13, 8, 16, True, 0),
+    (2, 65, 64, 32, 128, False, 0),
+    (5, 130, 401, 32, 128, True, 37),
+    (2, 1, 1000, 32, 128, False, 999),
+    (4, 333, 517, 64, 200, True, -20),
+    (2, 257, 1500, 128, 1000, True, 300),
+    (1, 40, 33, 4, 3, True, 5),
+    (2, 20, 30, 256, 1024, False, 5000),
+    (1, 300, 3, 2, 2, False, -400),
+]
+
+
+@pytest.mark.parametrize('dt', HALF + [torch.float32], ids=ids)
+@pytest.mark.parametrize('case', BIAS, ids=lambda c: 'x'.join(str(int(v)) for v in c))
+def test_bias_matrix_and_its_gradient(case, dt):
+    H, nq, nk, n, far, bidir, start = case
+    table = rnd(n, H, seed=1).float()
+    leaf = table.to(DEV).requires_grad_(True)
+    out = ops.relative_position_bias(leaf, nq, nk, max_distance=far, bidirectional=bidir, q_start=start, dtype=dt)
+    at = bucket_matrix(n, far, bidir, nq, nk, start)
+    want = table.double().t()[:, at]
+    assert out.dtype == dt
+    close(out, want, step(dt) * want.abs(), 'bias')
+    dout = rnd(H, nq, nk, seed=2).to(dt)
+    g, = torch.autograd.grad(out, leaf, dout.to(DEV))
+    wg, size = torch.zeros(n, H, dtype=torch.float64), torch.zeros(n, H, dtype=torch.float64)
+    for h in range(H):
+        wg[:, h].index_add_(0, at.flatten(), dout[h].double().flatten())
+        size[:, h].index_add_(0, at.flatten(), dout[h].double().abs().flatten())
+    close(g, wg, 1e-6 * size, 'table gradient')
+    again, = torch.autograd.grad(ops.relative_position_bias(leaf, nq, nk, far, bidir, start, dt), leaf, dout.to(DEV))
+    assert torch.equal(g, again)
+
+
+def test_bias_matrix_of_no_rows_and_no_columns():
+    leaf = rnd(32, 2).float().to(DEV).requires_grad_(True)
+    for nq, nk in ((0, 5), (5, 0)):
+        out = ops.relative_position_bias(leaf, nq, nk)
+        assert out.shape == (2, nq, nk)
+        g, = torch.autograd.grad(out, leaf, torch.zeros_like(out))
+        assert not g.any()
+
+
+# --------------------------------------------------------------------------------------------- norms
+def norm64(x, y, w1, b1, gate, rows, bs, rs, w2, b2, layer, eps):
+    def n(t, w, b):
+        t = t - t.mean(-1, keepdim=True) if layer else t
+        t = t / torch.sqrt((t * t).mean(-1, keepdim=True) + eps) * w
+        return t if b is None else t + b
+
+    C = x.shape[-1]
+    if y is None:
+        return None, n(x, w2, b2)
+    t = y if w1 is None else n(y, w1, b1)
+    if gate is not None:
+        t = gate.reshape(-1, 1, C).expand(-1, rows, C).reshape(x.shape) * t
+    xo = rs * x + bs * t
+    return xo, None if w2 is None else n(xo, w2, b2)
+
+
+NORM_TYPES = [(torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.float32, torch.float16),
+              (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16)]
+NORMS = [
+    # shape, kind, post, gate, pre, branch_scale, residual_scale, offset (elements the tensors start off a 16-byte boundary)
+    ((1, 1, 128), 'rms', True, 'channel', True, 1.0, 1.0, 0),
+    ((2, 9, 64), 'layer', True, 'sample', True, 0.5, 1.0, 0),
+    ((3, 33, 512), 'rms', True, 'token', True, 1.0, 0.7, 0),
+    ((2, 70, 1000), 'layer', True, 'channel', True, 2.0, 1.3, 0),
+    ((4, 5, 2048), 'rms', False, None, True, 1.0, 1.0, 0),
+    ((2, 3, 4096), 'layer', True, 'sample', False, 1.0, 1.0, 0),
+    ((1, 3, 8192), 'layer', True, 'token', True, 1.0, 1.0, 0),
+    ((5, 7, 37), 'layer', True, 'sample', True, 1.0, 1.0, 0),
+    ((3, 11, 1001), 'rms', True, 'channel', True, 1.0, 1.0, 0),
+    ((1, 2, 5001), 'layer', True, 'channel', True, 1.0, 1.0, 0),
+    ((130, 1, 96), 'rms', True, 'sample', True, 1.0, 1.0, 0),
+    ((700, 40), 'rms', None, None, True, 1.0, 1.0, 0),
+    ((2, 17, 256), 'rms', True, 'channel', True, 1.0, 1.0, 1),
+    ((1500, 128), 'layer', True, 'channel', True, 1.0, 1.0, 0),
+    ((3, 1), 'rms', True, 'channel', True, 1.0, 1.0, 0),
+]
+
+
+@pytest.mark.parametrize('types', NORM_TYPES, ids=lambda t: '%s-%s' % (ids(t[0]), ids(t[1])))
+@pytest.mark.parametrize('case', NORMS, ids=lambda c: '%s-%s-%s' % ('x'.join(map(str, c[0])), c[1], c[3]))
+def test_block_norm_and_its_gradients(case, types):
+    shape, kind, post, gate, pre, bs, rs, off = case
+    xt, yt = types
+    C, layer, eps = shape[-1], kind == 'layer', 1e-6
+    gshape = {None: None, 'channel': (C,), 'sample': (shape[0], C), 'token': shape}[gate]
+    rows = {None: 1, 'channel': math.prod(shape[:-1]), 'sample': math.prod(shape[1:-1]), 'token': 1}[gate]
+    host = dict(x=(rnd(*shape, seed=1, std=2.0) + 0.5).to(xt), y=None if post is None else (rnd(*shape, seed=2) - 0.3).to(yt),
+                w1=1 + rnd(C, seed=3, std=0.2) if post else None, b1=rnd(C, seed=4, std=0.2) if post and layer else None,
+                gate=None if gate is None else (0.5 + rnd(*gshape, seed=5, std=0.3)).to(yt if gate == 'token' else torch.float32),
+                w2=1 + rnd(C, seed=6, std=0.2) if pre else None, b2=rnd(C, seed=7, std=0.2) if pre and layer else None)
+    for n in ('w1', 'b1', 'w2', 'b2'):
+        host[n] = None if host[n] is None else host[n].float()
+
+    def on_gpu(t):
+        if t is None:
+            return None
+        flat = torch.empty(t.numel() + off, dtype=t.dtype, device=DEV)
+        flat[off:] = t.flatten().to(DEV)
+        return flat[off:].view(t.shape).requires_grad_(True)
+
+    dev = {n: on_gpu(t) for n, t in host.items()}
+    ref = {n: None if t is None else t.double().requires_grad_(True) for n, t in host.items()}
+    xo, h = ops.block_norm(dev['x'], dev['y'], dev['w1'], dev['b1'], dev['gate'], bs, rs, dev['w2'], dev['b2'], kind, eps)
+    wxo, wh = norm64(ref['x'], ref['y'], ref['w1'], ref['b1'], ref['gate'], rows, bs, rs, ref['w2'], ref['b2'], layer, eps)
+    outs, wants, douts = [], [], []
+    if post is None:
+        assert xo is dev['x']
+    else:
+        outs, wants, douts = [xo], [wxo], [rnd(*shape, seed=8).to(xt)]
+    if pre:
+        outs, wants, douts = outs + [h], wants + [wh], douts + [rnd(*shape, seed=9).to(yt)]
+    else:
+        assert h is None
+    for o, w in zip(outs, wants):
+        w = w.detach()
+        assert o.dtype == (yt if o is h and post is not None else o.dtype)
+        close(o, w, step(o.dtype) * w.abs() * (1 + 1e-3) + 2e-6 * (1 + w.abs().max()), 'output')
+    names = [n for n in host if host[n] is not None]
+    got = torch.autograd.grad(outs, [dev[n] for n in names], [d.to(DEV) for d in douts])
+    want = torch.autograd.grad(wants, [ref[n] for n in names], [d.double() for d in douts])
+    tokens = math.prod(shape[:-1])
+    for n, g, w in zip(names, got, want):
+        assert g.dtype == host[n].dtype and g.shape == host[n].shape
+        # sums over the tokens of terms about as large as the largest entry of a token's: fp32 errors grow with sqrt(tokens) at most
+        scale = w.abs().max() + (math.sqrt(tokens) if n in ('w1', 'b1', 'w2', 'b2', 'gate') else 1.0)
+        extra = 16 if C == 1 else 1                     # one channel: 1 / |t| amplifies
+        close(g, w, step(g.dtype) * w.abs() * (1 + 1e-3) + 4e-6 * extra * scale, n)
+    again = torch.autograd.grad(ops.block_norm(dev['x'], dev['y'], dev['w1'], dev['b1'], dev['gate'], bs, rs, dev['w2'], dev['b2'], kind, eps)
+                                [0 if post is not None else 1:2 if pre else 1], [dev[n] for n in names], [d.to(DEV) for d in douts])
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+def test_block_norm_passes_only_one_gradient():
+    x, y, w = rnd(4, 6, 256, seed=1).float(), rnd(4, 6, 256, seed=2).float(), 1 + rnd(256, seed=3, std=0.1).float()
+    for which in (0, 1):
+        dev = [t.to(DEV).requires_grad_(True) for t in (x, y, w, w)]
+        ref = [t.double().requires_grad_(True) for t in (x, y, w, w)]
+        o = ops.block_norm(dev[0], dev[1], post_weight=dev[2], pre_weight=dev[3])[which]
+        r = norm64(ref[0], ref[1], ref[2], None, None, 1, 1.0, 1.0, ref[3], None, False, 1e-6)[which]
+        (o * o).sum().backward()
+        (r * r).sum().backward()
+        for d, t in zip(dev, ref):
+            if t.grad is None:
+                assert d.grad is None
+            else:
+                close(d.grad, t.grad, 1e-5 * (1 + t.grad.abs().max()), str(which))
+
+
+def test_block_norm_keeps_nan_and_inf_in_their_rows():
+    x, y, w = rnd(8, 128, seed=1).bfloat16(), rnd(8, 128, seed=2).bfloat16(), torch.ones(128)
+    y[3, 5], y[6, 0] = float('nan'), float('inf')
+    xo, h = ops.block_norm(x.to(DEV), y.to(DEV), post_weight=w.to(DEV), pre_weight=w.to(DEV))
+    bad = ~torch.isfinite(h.float()).all(-1).cpu()
+    assert bad.tolist() == [False] * 3 + [True] + [False] * 2 + [True] + [False]
+
+
+# --------------------------------------------------------------------------------------------- attention
+def attention64(q, k, v, table, at, see, scale):
+    """Outputs, and for each what the 16-bit rounding of the probabilities can add: sum |p| |v|."""
+    H, Hkv = q.shape[2], k.shape[2]
+    k, v = (t.repeat_interleave(H // Hkv, 2) for t in (k, v))
+    x = scale * torch.einsum('bihd,bjhd->bhij', q, k) + table.t()[:, at].transpose(0, 1)
+    x = x.masked_fill(~see[:, None], -math.inf)
+    top = x.amax(-1, keepdim=True) if x.shape[-1] else x.new_zeros(x.shape[:-1] + (1,))
+    p = torch.exp(x - torch.where(top == -math.inf, torch.zeros_like(top), top).detach())
+    total = p.sum(-1, keepdim=True)
+    p = p / torch.where(total == 0, torch.ones_like(total), total)
+    return torch.einsum('bhij,bjhd->bihd', p, torch.where(see.any(1)[:, :, None, None], v, torch.zeros_like(v))), p
+
+
+ATTN = [
+    # B, Nq, Nk, H, Hkv, D, causal, k_lens, mask, q_start, buckets, max_distance
+    dict(B=1, Nq=1, Nk=1, H=1, Hkv=1, D=8),
+    dict(B=2, Nq=33, Nk=65, H=2, Hkv=1, D=32),
+    dict(B=2, Nq=64, Nk=64, H=4, Hkv=4, D=64, causal=True),
+    dict(B=1, Nq=129, Nk=200, H=2, Hkv=2, D=40),
+    dict(B=3, Nq=77, Nk=93, H=4, Hkv=2, D=40, mask=True),
+    dict(B=2, Nq=300, Nk=300, H=4, Hkv=1, D=128, causal=True, lens=[300, 177]),
+    dict(B=3, Nq=65, Nk=130, H=2, Hkv=2, D=64, lens=[0, 1, 130]),
+    dict(B=2, Nq=257, Nk=190, H=2, Hkv=2, D=96, causal=True, start=-100),
+    dict(B=2, Nq=40, Nk=517, H=6, Hkv=2, D=128, causal=True, start=[477, 100], lens=[517, 140]),
+    dict(B=1, Nq=513, Nk=700, H=2, Hkv=2, D=64, buckets=64, far=700),
+    dict(B=1, Nq=200, Nk=333, H=2, Hkv=2, D=16, buckets=4, far=3, mask=True, causal=True),
+    dict(B=2, Nq=150, Nk=150, H=3, Hkv=3, D=64, causal=True, bidirectional=True),
+    # few queries
+    dict(B=1, Nq=1, Nk=197, H=8, Hkv=8, D=64, causal=True, start=196),
+    dict(B=4, Nq=1, Nk=700, H=8, Hkv=2, D=128, causal=True, start=[699, 0, -1, 300], lens=[700, 1, 0, 301]),
+    dict(B=2, Nq=5, Nk=3000, H=16, Hkv=2, D=64, causal=True, start=[2995, 1200], lens=[3000, 1205]),
+    dict(B=2, Nq=3, Nk=900, H=4, Hkv=4, D=80, mask=True),
+    dict(B=1, Nq=32, Nk=1100, H=4, Hkv=2, D=32, buckets=128, far=1000),
+    dict(B=1, Nq=2, Nk=0, H=2, Hkv=2, D=64),
+    dict(B=1, Nq=70, Nk=0, H=2, Hkv=2, D=64),
+]
+
+
+def attn_case(c, dt):
+    B, Nq, Nk, H, Hkv, D = (c[n] for n in ('B', 'Nq', 'Nk', 'H', 'Hkv', 'D'))
+    causal, n, far = c.get('causal', False), c.get('buckets', 32), c.get('far', 128)
+    bidir = c.get('bidirectional', not causal)
+    start = c.get('start', 0)
+    starts = start if isinstance(start, list) else [start] * B
+    lens = c.get('lens')
+    mask = torch.rand(B, Nk, generator=torch.Generator().manual_seed(9)) < 0.6 if c.get('mask') else None
+    host = dict(q=rnd(B, Nq, H, D, seed=1).to(dt), k=rnd(B, Nk, Hkv, D, seed=2).to(dt), v=rnd(B, Nk, Hkv, D, seed=3).to(dt),
+                table=rnd(n, H, seed=4).float())
+    at = torch.stack([bucket_matrix(n, far, bidir, Nq, Nk, s) for s in starts])
+    i, j = torch.arange(Nq)[:, None], torch.arange(Nk)[None, :]
+    see = torch.stack([(j < (lens[b] if lens else Nk)) & ((j <= i + starts[b]) if causal else (j >= 0)) for b in range(B)])
+    if mask is not None:
+        see = see & mask[:, None]
+    kw = dict(max_distance=far, causal=causal, bidirectional=c.get('bidirectional'),
+              k_lens=None if lens is None else torch.tensor(lens, dtype=torch.int32, device=DEV),
+              key_mask=None if mask is None else mask.to(DEV),
+              q_start=torch.tensor(start, dtype=torch.int32, device=DEV) if isinstance(start, list) else start)
+    return host, at, see, kw
+
+
+def attn_id(c):
+    return '-'.join('%s%s' % (k, '_'.join(map(str, v)) if isinstance(v, list) else int(v)) for k, v in c.items())
+
+
+@pytest.mark.parametrize('dt', HALF, ids=ids)
+@pytest.mark.parametrize('case', ATTN, ids=attn_id)
+def test_attention_and_its_gradients(case, dt):
+    host, at, see, kw = attn_case(case, dt)
+    D, u = case['D'], step(dt)
+    G = case['H'] // case['Hkv']
+    ref = {n: t.double().requires_grad_(True) for n, t in host.items()}
+    want, p = attention64(ref['q'], ref['k'], ref['v'], ref['table'], at, see, D ** -0.5)
+    v_abs = host['v'].double().abs().repeat_interleave(G, 2)
+    spread = torch.einsum('bhij,bjhd->bihd', p.detach(), v_abs)
+    want_d = want.detach()
+    with torch.no_grad():                                   # inference: the few-query kernel where it applies
+        out = ops.biased_attention(*(host[n].to(DEV) for n in ('q', 'k', 'v', 'table')), **kw)
+    close(out, want_d, u * want_d.abs() * 1.01 + (u + 2e-5) * spread + 1e-7, 'out')
+    # what is hidden from everybody may hold anything
+    hidden = ~see.any(1)
+    bad_k, bad_v = host['k'].clone(), host['v'].clone()
+    bad_k[hidden], bad_v[hidden] = float('nan'), float('inf')
+    if not (case.get('causal') and kw['k_lens'] is None and kw['key_mask'] is None) or case['Nk'] <= case['Nq']:
+        with torch.no_grad():
+            assert torch.equal(out, ops.biased_attention(host['q'].to(DEV), bad_k.to(DEV), bad_v.to(DEV), host['table'].to(DEV), **kw))
+    # gradients
+    leaf = {n: t.to(DEV).requires_grad_(True) for n, t in host.items()}
+    out = ops.biased_attention(leaf['q'], leaf['k'], leaf['v'], leaf['table'], **kw)
+    close(out, want_d, u * want_d.abs() * 1.01 + (u + 2e-5) * spread + 1e-7, 'training out')
+    dout = rnd(*host['q'].shape, seed=5).to(dt)
+    names = ['q', 'k', 'v', 'table']
+    got = dict(zip(names, torch.autograd.grad(out, [leaf[n] for n in names], dout.to(DEV))))
+    want_g = dict(zip(names, torch.autograd.grad(want, [ref[n] for n in names], dout.double())))
+    # magnitudes of what the rounding of p and ds (u each) is summed over
+    with torch.no_grad():
+        do = dout.double()
+        vv, kk = (host[n].double().repeat_interleave(G, 2) for n in ('v', 'k'))
+        vv = torch.where(see.any(1)[:, :, None, None], vv, torch.zeros_like(vv))
+        dp = torch.einsum('bihd,bjhd->bhij', do, vv)
+        delta = (p * dp).sum(-1, keepdim=True)
+        ds = (p * (dp - delta)).abs()
+        size = p * (dp.abs() + (p * dp.abs()).sum(-1, keepdim=True))          # ds without its cancellation: 32-bit errors go by this
+        kt, qt = kk.abs(), host['q'].double().abs()
+        group = lambda t: t.reshape(t.shape[0], t.shape[1], case['Hkv'], G, D).sum(3)  # noqa: E731
+        slack = dict(q=D ** -0.5 * torch.einsum('bhij,bjhd->bihd', u * ds + 2e-5 * size, kt),
+                     k=group(D ** -0.5 * torch.einsum('bhij,bihd->bjhd', u * ds + 2e-5 * size, qt)),
+                     v=group(torch.einsum('bhij,bihd->bjhd', (u + 2e-5) * p, do.abs())))
+        st = torch.zeros_like(want_g['table'])
+        for b in range(case['B']):
+            for h in range(case['H']):
+                st[:, h].index_add_(0, at[b].flatten(), size[b, h].flatten())
+        slack['table'] = (2e-5 + u * u) * st
+    for n in names:
+        w = want_g[n]
+        assert got[n].dtype == host[n].dtype
+        # fp16: results and operands below 2^-14 step by 2^-24
+        tiny = 0.0 if n == 'table' else 1e-6 if dt == torch.bfloat16 else 2.0 ** -25 * (2 + case['Nk'] + case['Nq'] * G)
+        close(got[n], w, (u * 1.01 if n != 'table' else 1e-6) * w.abs() + slack[n] + tiny, 'd' + n)
+    again = torch.autograd.grad(ops.biased_attention(leaf['q'], leaf['k'], leaf['v'], leaf['table'], **kw), [leaf[n] for n in names], dout.to(DEV))
+    for n, a in zip(names, again):
+        assert torch.equal(got[n], a), n
