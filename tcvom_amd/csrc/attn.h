@@ -50,11 +50,11 @@ struct AttnArgs {
     const void* dout;
     void *dq, *dk, *dv;
     float *delta, *part;                     // backward: <dout, out> of every row; bucket sums of every workgroup
-    float* partial;                          // forward: the splits' outputs
+    float* partial;                          // forward: the splits' outputs; backward: each head's dk and dv where a group is taken apart
     const int *k_lens, *q_starts;            // [B] or null
     const unsigned char* key_mask;           // [B][Nk] or null
     long long qs[3], ks[3], vs[3], dos[3];   // strides of batch, token, head in elements
-    int B, Nq, Nk, H, Hkv, D, causal, q_start, splits, tiles;
+    int B, Nq, Nk, H, Hkv, D, causal, q_start, splits, tiles, apart;
     float scale;                             // softmax scale, natural
     tcvom_rel_buckets bk;
 };
@@ -117,18 +117,31 @@ __device__ __forceinline__ typename Mma<T>::v8 pack_rest(const f32x16_t& p, type
     return r;
 }
 
-// operand A of a product that contracts the rows of an LDS tile, 16 of them from r0 (in the score registers' order): the tile's columns
-// 32 d + (lane & 31)
-template <class T, int DP>
-__device__ __forceinline__ typename Mma<T>::v8 read_columns(const T* tile, int r0, int d, int lane) {
-    const int r = r0 + 4 * (lane >> 5) + ((lane & 15) >> 2);
-    const int ch = d * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1), in = (lane & 1) * 4;
-    return join<T>(Mma<T>::tr(&tile[chunk_at<DP>(r, ch) * 8 + in]), Mma<T>::tr(&tile[chunk_at<DP>(r + 8, ch) * 8 + in]));
-}
-// operand A of a product over the tile's columns: row (lane & 31) from r0, columns 16 s + 8 (lane >> 5) ..
-template <class T, int DP>
-__device__ __forceinline__ typename Mma<T>::v8 read_rows(const T* tile, int r0, int s, int lane) {
-    return *reinterpret_cast<const typename Mma<T>::v8*>(&tile[chunk_at<DP>(r0 + (lane & 31), s * 2 + (lane >> 5)) * 8]);
+// Operands from an LDS tile of rows of DP elements (layout: chunk_at).  A lane's byte offset differs between steps by an XOR of a few low
+// bits and a constant, so that one register and one instruction a step address them all; `keep` stops the compiler from holding
+// every step's address in a register of its own across the loop.
+template <class T, int DP> struct Tile {
+    typedef typename Mma<T>::v8 v8;
+    static constexpr int ROW = DP * 2;
+    // rows r0 + (lane & 31), columns 16 s + 8 (lane >> 5) ..: operand of a product over the columns
+    static __device__ __forceinline__ unsigned rows_at(int lane) { return chunk_at<DP>(lane & 31, lane >> 5) * 16; }
+    static __device__ __forceinline__ v8 rows(const T* tile, unsigned off, int r0, int s) {
+        return *reinterpret_cast<const v8*>(reinterpret_cast<const char*>(tile) + (off ^ (s << 5)) + r0 * ROW);
+    }
+    // column 32 d + (lane & 31), 16 rows from r0 (a multiple of 16) in the order of the score registers: operand of a product that
+    // contracts the rows
+    static __device__ __forceinline__ unsigned cols_at(int lane) {
+        return chunk_at<DP>(4 * (lane >> 5) + ((lane & 15) >> 2), ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
+    }
+    static __device__ __forceinline__ v8 cols(const T* tile, unsigned off, int r0, int d) {
+        const char* p = reinterpret_cast<const char*>(tile) + r0 * ROW;
+        return join<T>(Mma<T>::tr(reinterpret_cast<const T*>(p + (off ^ (d << 6)))),
+                       Mma<T>::tr(reinterpret_cast<const T*>(p + (off ^ (d << 6) ^ 32) + 8 * ROW)));
+    }
+};
+__device__ __forceinline__ unsigned keep(unsigned v) {
+    asm volatile("" : "+v"(v));
+    return v;
 }
 // 16 bytes of a row, zeros where `ok` is false
 template <class V8, class T>

@@ -80,6 +80,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
             for (int r = 0; r < 16; ++r) o[u][d][r] = 0.f;
     }
     const float c = a.scale * LOG2E;
+    const unsigned rows_at = Tile<T, DP>::rows_at(lane), cols_at = Tile<T, DP>::cols_at(lane);
     if (ntiles > 0) {
         fetch(0);
         store(0);
@@ -87,6 +88,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
     __syncthreads();
     for (int t = 0; t < ntiles; ++t) {
         const int buf = t & 1, k0 = t * KT;
+        const unsigned ra = keep(rows_at) + buf * (KT * DP * 2), ca = keep(cols_at) + buf * (KT * DP * 2);
         if (t + 1 < ntiles) fetch(t + 1);
         unsigned long long bits = ~0ull;
         if (mask) bits = __ballot(k0 + lane < a.Nk && mask[min(k0 + lane, a.Nk - 1)]);
@@ -100,7 +102,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
                 for (int r = 0; r < 16; ++r) x[kb][r] = 0.f;
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    x[kb] = Mma<T>::mma(read_rows<T, DP>(lk[buf], kb * 32, s, lane), qf[u][s], x[kb]);
+                    x[kb] = Mma<T>::mma(Tile<T, DP>::rows(lk[0], ra, kb * 32, s), qf[u][s], x[kb]);
                 }
             }
             const int w0 = i0 + (wave * QB + u) * 32;               // the wave's first query of this block
@@ -165,7 +167,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
                     if constexpr (LO) rest = pack_rest<T>(x[kb], p, s);
 #pragma unroll
                     for (int d = 0; d < DB; ++d) {
-                        const v8 vf = read_columns<T, DP>(lv[buf], kb * 32 + s * 16, d, lane);
+                        const v8 vf = Tile<T, DP>::cols(lv[0], ca, kb * 32 + s * 16, d);
                         o[u][d] = Mma<T>::mma(vf, p, o[u][d]);
                         if constexpr (LO) o[u][d] = Mma<T>::mma(vf, rest, o[u][d]);
                     }
@@ -269,6 +271,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
         for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
     float m = -INFINITY, l = 0.f;
     const float c = a.scale * LOG2E;
+    const unsigned cols_at = Tile<T, DP>::cols_at(lane);
     int k0 = ka + wave * 32;
     if (k0 < kz) fetch(k0);
     __syncthreads();
@@ -332,7 +335,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
         for (int s = 0; s < 2; ++s) {
             const v8 p = pack_step<T>(x, s);
 #pragma unroll
-            for (int d = 0; d < DB; ++d) o[d] = Mma<T>::mma(read_columns<T, DP>(lv[wave], s * 16, d, lane), p, o[d]);
+            for (int d = 0; d < DB; ++d) o[d] = Mma<T>::mma(Tile<T, DP>::cols(lv[wave], cols_at, s * 16, d), p, o[d]);
         }
     }
     // join the 4 waves: common maximum, then the outputs are added two waves at a time in LDS

@@ -14,8 +14,9 @@
 // the entry of its relative position in LDS.  Each half wave has its own copy of the line, within which the 32 lanes of a step (one
 // key, 32 queries) have different entries, so that every entry is a sum in program order: equal calls give equal bits.
 template <class T, int DP, bool TABLE>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;
+    constexpr int KT = DP == 128 ? 32 : 64;                 // keys a tile: two waves a SIMD fit the registers
     constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8, PER = KT * CH / 256, BM = 128;
     __shared__ __align__(16) T lk[2][KT * DP];
     __shared__ __align__(16) T lv[2][KT * DP];
@@ -86,6 +87,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dq_kernel(AttnArg
     for (int d = 0; d < DB; ++d) acc[d] = zero16();
     float far_lo = 0.f, far_hi = 0.f;
     const float c = a.scale * LOG2E;
+    const unsigned rows_at = Tile<T, DP>::rows_at(lane), cols_at = Tile<T, DP>::cols_at(lane);
     if (ntiles > 0) {
         fetch(0);
         store(0);
@@ -93,6 +95,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dq_kernel(AttnArg
     __syncthreads();
     for (int t = 0; t < ntiles; ++t) {
         const int buf = t & 1, k0 = t * KT;
+        const unsigned ra = keep(rows_at) + buf * (KT * DP * 2), ca = keep(cols_at) + buf * (KT * DP * 2);
         if (t + 1 < ntiles) fetch(t + 1);
         unsigned long long bits = ~0ull;
         if (mask) bits = __ballot(k0 + lane < a.Nk && mask[min(k0 + lane, a.Nk - 1)]);
@@ -102,12 +105,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dq_kernel(AttnArg
         const int rel_hi = k0 + KT - 1 - w0 - start, rel_lo = k0 - (w0 + 31) - start;
         const bool far = rel_hi <= -reach || rel_lo >= right;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int kb = 0; kb < KT / 32; ++kb) {
             f32x16_t x = zero16(), g = zero16();
 #pragma unroll
-            for (int s = 0; s < KS; ++s) x = Mma<T>::mma(read_rows<T, DP>(lk[buf], kb * 32, s, lane), qf[s], x);
+            for (int s = 0; s < KS; ++s) x = Mma<T>::mma(Tile<T, DP>::rows(lk[0], ra, kb * 32, s), qf[s], x);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) g = Mma<T>::mma(read_rows<T, DP>(lv[buf], kb * 32, s, lane), gf[s], g);
+            for (int s = 0; s < KS; ++s) g = Mma<T>::mma(Tile<T, DP>::rows(lv[0], ra, kb * 32, s), gf[s], g);
             const int at = k0 + kb * 32 + 4 * half - qi - start + reach;
             if (far) {
                 const float add = (rel_hi <= -reach ? line[0] : line[last]) - lse;
@@ -148,7 +151,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dq_kernel(AttnArg
             for (int s = 0; s < 2; ++s) {
                 const v8 p = pack_step<T>(x, s);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::mma(read_columns<T, DP>(lk[buf], kb * 32 + s * 16, d, lane), p, acc[d]);
+                for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::mma(Tile<T, DP>::cols(lk[0], ca, kb * 32 + s * 16, d), p, acc[d]);
             }
         }
         if (t + 1 < ntiles) store(buf ^ 1);
@@ -215,17 +218,23 @@ __global__ __launch_bounds__(1024) void attn_table_kernel(const float* part, flo
 // ---- dk, dv: a wave owns 32 keys of one key head, the workgroup (128 keys) walks the queries of every head that shares them, 32 at a
 // time.  Scores here are S = Q K^T (rows = queries, columns = keys): p and ds are again the register operand of dV^T = dO^T P and
 // dK^T = Q^T dS.
+//
+// Causal key tiles have very different numbers of queries, and a group of heads that share keys multiplies a workgroup's work: with
+// few workgroups (attn_apart) each head of a group gets workgroups of its own, which write fp32 partial sums [2][B][Nk][H][D] that
+// attn_heads_kernel adds in order.  The tiles with most queries come first.
 template <class T, int DP>
-__global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;
     constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8, QT = 32, PER = (QT * CH + 255) / 256, BN = 128;
     __shared__ __align__(16) T lq[2][QT * DP];
     __shared__ __align__(16) T lg[2][QT * DP];
+    __shared__ __align__(16) T lv[BN * DP];                 // this workgroup's values, operand B of dP = dO V^T: no registers left for them
     __shared__ __align__(16) float ls[2][QT], ld[2][QT];
     extern __shared__ float line[];
 
-    const int item = xcd_item(blockIdx.x, gridDim.x);
-    const int bh = item / a.tiles, b = bh / a.Hkv, hk = bh % a.Hkv, tile = item % a.tiles, G = a.H / a.Hkv;
+    const int item = xcd_item(blockIdx.x, gridDim.x);           // (tile 0 of a causal head, with most queries, comes first)
+    const int heads = a.apart ? a.H : a.Hkv, G = a.apart ? 1 : a.H / a.Hkv;      // of the grid, and of a workgroup
+    const int bh = item / a.tiles, b = bh / heads, h0 = bh % heads * G, hk = h0 / (a.H / a.Hkv), tile = item % a.tiles;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
     const int start = seq_start(a, b), len = seq_keys(a, b);
     const int j0 = tile * BN, w0 = j0 + wave * 32, key = w0 + col;
@@ -234,12 +243,12 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnAr
     const bool seen = key < len && (!mask || mask[key]);
     const T* K = (const T*)a.k + b * a.ks[0] + hk * a.ks[2] + (long long)key * a.ks[1];
     const T* V = (const T*)a.v + b * a.vs[0] + hk * a.vs[2] + (long long)key * a.vs[1];
-    v8 kf[KS], vf[KS];
+    v8 kf[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
         const int d = s * 16 + half * 8;
         kf[s] = load_or_zero<v8>(seen && d < a.D, K + d);
-        vf[s] = load_or_zero<v8>(seen && d < a.D, V + d);
+        *reinterpret_cast<v8*>(&lv[chunk_at<DP>(wave * 32 + col, s * 2 + half) * 8]) = load_or_zero<v8>(seen && d < a.D, V + d);
     }
     f32x16_t dk[DB], dv[DB];
 #pragma unroll
@@ -248,6 +257,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnAr
         dv[d] = zero16();
     }
     const float c = a.scale * LOG2E;
+    const unsigned rows_at = Tile<T, DP>::rows_at(lane), cols_at = Tile<T, DP>::cols_at(lane);
     constexpr float small = Mma<T>::shift > 0.f ? 1.f / 32768.f : 1.f;       // 2^-shift
     // queries that see a key of this workgroup: from i >= j0 - start on if causal, none if the keys do not exist
     const int i_first = a.causal ? max(0, j0 - start) / QT * QT : 0;
@@ -255,7 +265,7 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnAr
     u32x4_t rq[PER], rg[PER];
     float rs = 0.f, rd = 0.f;
     auto fetch = [&](int t) {                               // t counts the query tiles of all heads of the group
-        const int h = hk * G + t / nt, i0 = i_first + t % nt * QT;
+        const int h = h0 + t / nt, i0 = i_first + t % nt * QT;
         const T* Q = (const T*)a.q + b * a.qs[0] + h * a.qs[2];
         const T* dO = (const T*)a.dout + b * a.dos[0] + h * a.dos[2];
         const long long stat = ((long long)b * a.H + h) * a.Nq;
@@ -293,26 +303,23 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnAr
     }
     for (int t = 0; t < total; ++t) {
         const int buf = t & 1, i0 = i_first + t % nt * QT;
+        const unsigned va = keep(rows_at), ra = va + buf * (QT * DP * 2), ca = keep(cols_at) + buf * (QT * DP * 2);
         if (t % nt == 0) {                                   // another head's bias
             __syncthreads();
-            fill_line(line, a, hk * G + t / nt, 256);
+            fill_line(line, a, h0 + t / nt, 256);
             __syncthreads();
         }
         if (t + 1 < total) fetch(t + 1);
-        f32x16_t x = zero16(), g = zero16();
+        f32x16_t x = zero16();
 #pragma unroll
-        for (int s = 0; s < KS; ++s) x = Mma<T>::mma(read_rows<T, DP>(lq[buf], 0, s, lane), kf[s], x);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) g = Mma<T>::mma(read_rows<T, DP>(lg[buf], 0, s, lane), vf[s], g);
+        for (int s = 0; s < KS; ++s) x = Mma<T>::mma(Tile<T, DP>::rows(lq[0], ra, 0, s), kf[s], x);
         const int rel_hi = w0 + 31 - i0 - start, rel_lo = w0 - (i0 + QT - 1) - start;
         const bool far = rel_hi <= -reach || rel_lo >= right;
-        float sub[16], del[16];
+        float sub[16];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const float4 s4 = *reinterpret_cast<const float4*>(&ls[buf][8 * q + 4 * half]);
-            const float4 d4 = *reinterpret_cast<const float4*>(&ld[buf][8 * q + 4 * half]);
             sub[4 * q] = s4.x; sub[4 * q + 1] = s4.y; sub[4 * q + 2] = s4.z; sub[4 * q + 3] = s4.w;
-            del[4 * q] = d4.x; del[4 * q + 1] = d4.y; del[4 * q + 2] = d4.z; del[4 * q + 3] = d4.w;
         }
         if (far) {
             const float add = rel_hi <= -reach ? line[0] : line[last];
@@ -337,20 +344,44 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnAr
         for (int s = 0; s < 2; ++s) {
             const v8 p = pack_step<T>(x, s);
 #pragma unroll
-            for (int d = 0; d < DB; ++d) dv[d] = Mma<T>::mma(read_columns<T, DP>(lg[buf], s * 16, d, lane), p, dv[d]);
+            for (int d = 0; d < DB; ++d) dv[d] = Mma<T>::mma(Tile<T, DP>::cols(lg[0], ca, s * 16, d), p, dv[d]);
         }
+        if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);      // (the next product's operands would not fit beside this one's)
+        f32x16_t g = zero16();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] *= fmaf(g[r], small, -del[r]);
+        for (int s = 0; s < KS; ++s) g = Mma<T>::mma(Tile<T, DP>::rows(lg[0], ra, 0, s), Tile<T, DP>::rows(lv + wave * 32 * DP, va, 0, s), g);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float4 d4 = *reinterpret_cast<const float4*>(&ld[buf][8 * q + 4 * half]);
+            x[4 * q] *= fmaf(g[4 * q], small, -d4.x);
+            x[4 * q + 1] *= fmaf(g[4 * q + 1], small, -d4.y);
+            x[4 * q + 2] *= fmaf(g[4 * q + 2], small, -d4.z);
+            x[4 * q + 3] *= fmaf(g[4 * q + 3], small, -d4.w);
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const v8 p = pack_step<T>(x, s);
 #pragma unroll
-            for (int d = 0; d < DB; ++d) dk[d] = Mma<T>::mma(read_columns<T, DP>(lq[buf], s * 16, d, lane), p, dk[d]);
+            for (int d = 0; d < DB; ++d) dk[d] = Mma<T>::mma(Tile<T, DP>::cols(lq[0], ca, s * 16, d), p, dk[d]);
         }
         if (t + 1 < total) store(buf ^ 1);
         __syncthreads();
     }
     if (key >= a.Nk) return;
+    if (a.apart) {
+        float* dst = a.partial + (((long long)b * a.Nk + key) * a.H + h0) * a.D;
+        const long long next = (long long)a.B * a.Nk * a.H * a.D;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int at = d * 32 + q * 8 + half * 4;
+                if (at >= a.D) continue;
+                *reinterpret_cast<float4*>(dst + at) = make_float4(dk[d][4 * q], dk[d][4 * q + 1], dk[d][4 * q + 2], dk[d][4 * q + 3]);
+                *reinterpret_cast<float4*>(dst + next + at) = make_float4(dv[d][4 * q], dv[d][4 * q + 1], dv[d][4 * q + 2], dv[d][4 * q + 3]);
+            }
+        return;
+    }
     const long long row = (((long long)b * a.Nk + key) * a.Hkv + hk) * a.D;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -369,6 +400,29 @@ __global__ __launch_bounds__(256, DP == 128 ? 1 : 2) void attn_dkv_kernel(AttnAr
         }
 }
 
+// dk, dv of a key head = the sums of its query heads' (attn_dkv_kernel, `apart`): 4 channels a thread
+template <class T>
+__global__ __launch_bounds__(256) void attn_heads_kernel(AttnArgs a) {
+    const int G = a.H / a.Hkv, quads = a.D / 4;
+    const long long n = (long long)a.B * a.Nk * a.Hkv * quads, at = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (at >= n) return;
+    const long long row = at / quads;                       // (b, key, key head)
+    const int c = (int)(at % quads) * 4;
+    const float* src = a.partial + (row / a.Hkv * a.H + row % a.Hkv * G) * a.D + c + blockIdx.y * ((long long)a.B * a.Nk * a.H * a.D);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int g = 0; g < G; ++g) {
+        const float4 f = *reinterpret_cast<const float4*>(src + (long long)g * a.D);
+        s.x += f.x; s.y += f.y; s.z += f.z; s.w += f.w;
+    }
+    const float w = blockIdx.y ? (Mma<T>::shift > 0.f ? 1.f / 32768.f : 1.f) : a.scale;
+    const typename Mma<T>::v4 v = {(T)(s.x * w), (T)(s.y * w), (T)(s.z * w), (T)(s.w * w)};
+    *reinterpret_cast<typename Mma<T>::v4*>((T*)(blockIdx.y ? a.dv : a.dk) + row * a.D + c) = v;
+}
+
+static bool attn_apart(const tcvom_attn_desc* d) {
+    return d->H > d->Hkv && (long long)d->B * d->Hkv * cdiv(d->Nk, 128) < 2048;
+}
+
 template <class T, int DP>
 static int launch_bwd(AttnArgs a, float* dtable, hipStream_t st) {
     const int last = line_reach(a.bk) + line_right(a.bk);
@@ -384,14 +438,20 @@ static int launch_bwd(AttnArgs a, float* dtable, hipStream_t st) {
     }
     if (a.Nk > 0) {
         a.tiles = cdiv(a.Nk, 128);
-        hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3((unsigned)((long long)a.B * a.Hkv * a.tiles)), dim3(256), sizeof(float) * (last + 1), st, a);
+        const unsigned wgs = (unsigned)((long long)a.B * (a.apart ? a.H : a.Hkv) * a.tiles);
+        hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3(wgs), dim3(256), sizeof(float) * (last + 1), st, a);
+        if (a.apart) {
+            const dim3 grid(cdiv((long long)a.B * a.Nk * a.Hkv * (a.D / 4), 256), 2);
+            hipLaunchKernelGGL(attn_heads_kernel<T>, grid, dim3(256), 0, st, a);
+        }
     }
     return 0;
 }
 
 extern "C" int64_t tcvom_attn_bwd_work(const tcvom_attn_desc* d) {
-    if (!d || d->B <= 0 || d->H <= 0 || d->Nq < 0) return 0;
-    return (int64_t)d->B * d->H * d->Nq + (int64_t)d->B * d->H * cdiv(d->Nq, 128) * d->buckets.num_buckets;
+    if (!d || d->B <= 0 || d->H <= 0 || d->Hkv <= 0 || d->Nq < 0 || d->Nk < 0) return 0;
+    const int64_t rows = (int64_t)d->B * d->H * d->Nq + (int64_t)d->B * d->H * cdiv(d->Nq, 128) * d->buckets.num_buckets;
+    return (rows + 3) / 4 * 4 + (attn_apart(d) ? 2 * (int64_t)d->B * d->Nk * d->H * d->D : 0);
 }
 
 extern "C" int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, const void* out,
@@ -405,7 +465,7 @@ extern "C" int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const voi
                         aligned16(dq) && aligned16(dk) && aligned16(dv), "attn_bwd: tensors start at multiples of 16 bytes");
     TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 32) < (1LL << 30) && (long long)d->B * d->Hkv * cdiv(d->Nk, 32) < (1LL << 30),
                     "attn_bwd: too many rows for one launch");
-    TCVOM_CHECK_ARG(work_floats >= tcvom_attn_bwd_work(d), "attn_bwd: %lld floats of workspace", (long long)work_floats);
+    TCVOM_CHECK_ARG(work_floats == tcvom_attn_bwd_work(d) && aligned16(work), "attn_bwd: %lld floats of workspace", (long long)work_floats);
     for (int n = 0; n < 3; ++n) {
         TCVOM_CHECK_ARG(dout_stride[n] % 8 == 0 && dout_stride[n] >= 0, "attn_bwd: strides are multiples of 8 elements");
         a.dos[n] = dout_stride[n];
@@ -414,6 +474,8 @@ extern "C" int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const voi
     a.dq = dq; a.dk = dk; a.dv = dv;
     a.delta = work;
     a.part = work + (int64_t)d->B * d->H * d->Nq;
+    a.apart = attn_apart(d);
+    if (a.apart) a.partial = work + work_floats - 2 * (int64_t)d->B * d->Nk * d->H * d->D;
     const hipStream_t st = (hipStream_t)stream;
     const int DP = attn_width(d->D);
     if (d->type == TCVOM_TYPE_BF16) {

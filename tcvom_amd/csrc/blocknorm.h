@@ -54,29 +54,13 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* lds, int& slot) 
     }
 }
 
-// the launch table: vector width by alignment, threads by channels (see the head of this file)
-#define NORM_TABLE(TX, TY, LAUNCH)                                     \
-    do {                                                               \
-        if (vec) {                                                     \
-            if (C <= 128) LAUNCH(TX, TY, 8, 16, 16, 1);                \
-            else if (C <= 512) LAUNCH(TX, TY, 8, 64, 4, 1);            \
-            else if (C <= 1024) LAUNCH(TX, TY, 8, 64, 4, 2);           \
-            else if (C <= 2048) LAUNCH(TX, TY, 8, 256, 1, 1);          \
-            else if (C <= 4096) LAUNCH(TX, TY, 8, 256, 1, 2);          \
-            else LAUNCH(TX, TY, 8, 512, 1, 2);                         \
-        } else {                                                       \
-            if (C <= 512) LAUNCH(TX, TY, 1, 64, 4, 8);                 \
-            else if (C <= 4096) LAUNCH(TX, TY, 1, 256, 1, 16);         \
-            else LAUNCH(TX, TY, 1, 512, 1, 16);                        \
-        }                                                              \
-    } while (0)
-#define NORM_TYPES(LAUNCH)                                                                                \
+#define NORM_TYPES(TABLE, LAUNCH)                                                                         \
     do {                                                                                                  \
-        if (x_type == TCVOM_TYPE_F32 && y_type == TCVOM_TYPE_F32) NORM_TABLE(float, float, LAUNCH);                 \
-        else if (x_type == TCVOM_TYPE_F32 && y_type == TCVOM_TYPE_BF16) NORM_TABLE(float, __bf16, LAUNCH);          \
-        else if (x_type == TCVOM_TYPE_F32 && y_type == TCVOM_TYPE_F16) NORM_TABLE(float, _Float16, LAUNCH);         \
-        else if (x_type == TCVOM_TYPE_BF16) NORM_TABLE(__bf16, __bf16, LAUNCH);                                \
-        else NORM_TABLE(_Float16, _Float16, LAUNCH);                                                      \
+        if (x_type == TCVOM_TYPE_F32 && y_type == TCVOM_TYPE_F32) TABLE(float, float, LAUNCH);            \
+        else if (x_type == TCVOM_TYPE_F32 && y_type == TCVOM_TYPE_BF16) TABLE(float, __bf16, LAUNCH);     \
+        else if (x_type == TCVOM_TYPE_F32 && y_type == TCVOM_TYPE_F16) TABLE(float, _Float16, LAUNCH);    \
+        else if (x_type == TCVOM_TYPE_BF16) TABLE(__bf16, __bf16, LAUNCH);                                \
+        else TABLE(_Float16, _Float16, LAUNCH);                                                           \
     } while (0)
 
 static inline bool norm_types_ok(int x_type, int y_type) {

@@ -99,6 +99,23 @@ __global__ __launch_bounds__(TPR * R) void block_norm_fwd_kernel(NormArgs a) {
     }
 }
 
+// vector width by alignment, threads by channels (see blocknorm.h)
+#define FWD_TABLE(TX, TY, LAUNCH)                                      \
+    do {                                                               \
+        if (vec) {                                                     \
+            if (C <= 128) LAUNCH(TX, TY, 8, 16, 16, 1);                \
+            else if (C <= 512) LAUNCH(TX, TY, 8, 64, 4, 1);            \
+            else if (C <= 1024) LAUNCH(TX, TY, 8, 64, 4, 2);           \
+            else if (C <= 2048) LAUNCH(TX, TY, 8, 256, 1, 1);          \
+            else if (C <= 4096) LAUNCH(TX, TY, 8, 256, 1, 2);          \
+            else LAUNCH(TX, TY, 8, 512, 1, 2);                         \
+        } else {                                                       \
+            if (C <= 512) LAUNCH(TX, TY, 1, 64, 4, 8);                 \
+            else if (C <= 4096) LAUNCH(TX, TY, 1, 256, 1, 16);         \
+            else LAUNCH(TX, TY, 1, 512, 1, 16);                        \
+        }                                                              \
+    } while (0)
+
 extern "C" int tcvom_block_norm_fwd(const void* x, const void* y, const float* post_weight, const float* post_bias, const void* gate,
                                     int32_t gate_f32, int64_t gate_rows, const float* pre_weight, const float* pre_bias, float branch_scale,
                                     float residual_scale, float eps, int32_t layer, void* x_out, void* h, float* stats, int64_t T, int32_t C,
@@ -128,7 +145,7 @@ extern "C" int tcvom_block_norm_fwd(const void* x, const void* y, const float* p
         if (layer) hipLaunchKernelGGL((block_norm_fwd_kernel<TX, TY, V, TPR, R, NV, true>), grid, dim3(TPR * R), 0, st, a);  \
         else hipLaunchKernelGGL((block_norm_fwd_kernel<TX, TY, V, TPR, R, NV, false>), grid, dim3(TPR * R), 0, st, a);       \
     } while (0)
-    NORM_TYPES(FWD);
+    NORM_TYPES(FWD_TABLE, FWD);
 #undef FWD
     TCVOM_LAUNCH_CHECK("block_norm_fwd");
     return 0;

@@ -53,6 +53,32 @@ __global__ __launch_bounds__(TPR * R) void block_norm_bwd_kernel(NormArgs a) {
     const long long first = (long long)blockIdx.y * group_rows + (long long)blockIdx.x * a.rows_per_wg;
     const long long end = (long long)(blockIdx.y + 1) * group_rows;
     if (a.gate && !token_gate) load_gate(blockIdx.y);
+    // the next row's loads are in flight while this one's sums wait at their barriers
+    typename RawVec<TX, V>::type rx[NV], rdx[NV];
+    typename RawVec<TY, V>::type ry[NV], rdh[NV];
+    float4 rst;
+    auto fetch = [&](int k) {
+        const long long row = first + k + g;
+        const bool live = k + g < a.rows_per_wg && row < end;
+        const long long base = row * C;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const int c = (n * TPR + lane) * V;
+            rx[n] = (typename RawVec<TX, V>::type)(TX)0.f;
+            rdx[n] = rx[n];
+            ry[n] = (typename RawVec<TY, V>::type)(TY)0.f;
+            rdh[n] = ry[n];
+            if (live && in[n]) {
+                if (pre) rx[n] = load_raw<TX, V>((const TX*)a.x + base + c);
+                if (has_y) ry[n] = load_raw<TY, V>((const TY*)a.y + base + c);
+                if (a.dxo) rdx[n] = load_raw<TX, V>((const TX*)a.dxo + base + c);
+                if (pre) rdh[n] = load_raw<TY, V>((const TY*)a.dh + base + c);
+            }
+        }
+        rst = make_float4(0.f, 1.f, 0.f, 1.f);
+        if (live) rst = *reinterpret_cast<const float4*>(a.stats + row * 4);
+    };
+    fetch(0);
     for (int k = 0; k < a.rows_per_wg; k += R) {
         const long long row = first + k + g;
         const bool live = k + g < a.rows_per_wg && row < end;
@@ -60,19 +86,14 @@ __global__ __launch_bounds__(TPR * R) void block_norm_bwd_kernel(NormArgs a) {
         float x[NV][V], y[NV][V], dX[NV][V], dh[NV][V];
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-            const int c = (n * TPR + lane) * V;
-#pragma unroll
-            for (int j = 0; j < V; ++j) x[n][j] = y[n][j] = dX[n][j] = dh[n][j] = 0.f;
-            if (live && in[n]) {
-                if (pre) load_vec<TX, V>((const TX*)a.x + base + c, x[n]);
-                if (has_y) load_vec<TY, V>((const TY*)a.y + base + c, y[n]);
-                if (a.dxo) load_vec<TX, V>((const TX*)a.dxo + base + c, dX[n]);
-                if (pre) load_vec<TY, V>((const TY*)a.dh + base + c, dh[n]);
-            }
+            raw_to_float<TX, V>(rx[n], x[n]);
+            raw_to_float<TY, V>(ry[n], y[n]);
+            raw_to_float<TX, V>(rdx[n], dX[n]);
+            raw_to_float<TY, V>(rdh[n], dh[n]);
         }
+        const float4 st = rst;
+        if (k + R < a.rows_per_wg) fetch(k + R);
         if (token_gate && live) load_gate(row);
-        float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
-        if (live) st = *reinterpret_cast<const float4*>(a.stats + row * 4);
         const float m1 = st.x, r1 = st.y, m2 = st.z, r2 = st.w;
         // y <- yhat, x <- xhat of x'
 #pragma unroll
@@ -189,6 +210,7 @@ __global__ __launch_bounds__(1024) void block_norm_sums_kernel(const float* part
     const int lo = is_gate ? ((int)blockIdx.y - s.nq) * s.parts : 0, hi = is_gate ? lo + s.parts : s.parts * s.groups;
     float t = 0.f;
     if (c < s.C)
+#pragma unroll 8
         for (int i = lo + slice; i < hi; i += 16) t += part[((long long)i * SUMS + q) * s.C + c];
     red[slice][threadIdx.x & 63] = t;
     __syncthreads();
@@ -212,9 +234,26 @@ static int bwd_wgs(int64_t T, int64_t groups, int R, int threads) {
     return (int)(n < 1 ? 1 : n > most ? most : n);
 }
 static void bwd_shape(int C, bool vec, int* R, int* threads) {
-    *R = vec ? (C <= 128 ? 16 : C <= 1024 ? 4 : 1) : (C <= 512 ? 4 : 1);
-    *threads = C <= 4096 ? 256 : 512;
+    *R = vec ? (C <= 128 ? 16 : C <= 512 ? 4 : C <= 1024 ? 2 : 1) : (C <= 512 ? 4 : 1);
+    *threads = vec ? (C <= 2048 ? 256 : 512) : (C <= 4096 ? 256 : 512);
 }
+// vector width by alignment, threads by channels: 8 channels a thread while the sums of 5 columns each leave room for them (bwd_shape
+// says the same)
+#define BWD_TABLE(TX, TY, LAUNCH)                                      \
+    do {                                                               \
+        if (vec) {                                                     \
+            if (C <= 128) LAUNCH(TX, TY, 8, 16, 16, 1);                \
+            else if (C <= 512) LAUNCH(TX, TY, 8, 64, 4, 1);            \
+            else if (C <= 1024) LAUNCH(TX, TY, 8, 128, 2, 1);          \
+            else if (C <= 2048) LAUNCH(TX, TY, 8, 256, 1, 1);          \
+            else if (C <= 4096) LAUNCH(TX, TY, 8, 512, 1, 1);          \
+            else LAUNCH(TX, TY, 8, 512, 1, 2);                         \
+        } else {                                                       \
+            if (C <= 512) LAUNCH(TX, TY, 1, 64, 4, 8);                 \
+            else if (C <= 4096) LAUNCH(TX, TY, 1, 256, 1, 16);         \
+            else LAUNCH(TX, TY, 1, 512, 1, 16);                        \
+        }                                                              \
+    } while (0)
 
 extern "C" int64_t tcvom_block_norm_bwd_work(int64_t T, int32_t C, int64_t gate_groups) {
     if (T <= 0 || C <= 0 || gate_groups <= 0) return 0;
@@ -275,7 +314,7 @@ extern "C" int tcvom_block_norm_bwd(const void* x, const void* y, const float* p
         if (layer) hipLaunchKernelGGL((block_norm_bwd_kernel<TX, TY, V, TPR, R, NV, true>), grid, dim3(TPR * R), 0, st, a);  \
         else hipLaunchKernelGGL((block_norm_bwd_kernel<TX, TY, V, TPR, R, NV, false>), grid, dim3(TPR * R), 0, st, a);       \
     } while (0)
-    NORM_TYPES(BWD);
+    NORM_TYPES(BWD_TABLE, BWD);
 #undef BWD
     TCVOM_LAUNCH_CHECK("block_norm_bwd");
     if (!a.want) return 0;

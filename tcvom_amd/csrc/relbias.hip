@@ -78,7 +78,7 @@ extern "C" int tcvom_relbias_fwd(const float* table, void* out, const tcvom_rel_
 // rows of the chunk, its key moving one step a row, so that a wave reads consecutive elements; the FAR one (the last) sums what lies
 // past the two ends of the line, which is most of a long matrix, with 16-byte loads.  Each sum is made by one thread, or by a tree of
 // fixed shape, and written once: no atomics, equal calls give equal bits.
-constexpr int BIAS_ROWS = 64;
+constexpr int BIAS_ROWS = 16;
 template <class T>
 __global__ __launch_bounds__(256) void relbias_bwd_kernel(const T* dout, float* part, tcvom_rel_buckets bk, long long Nq, long long Nk,
                                                           long long q_start) {
@@ -122,7 +122,15 @@ __global__ __launch_bounds__(256) void relbias_bwd_kernel(const T* dout, float* 
             if (lane < head) s[0] = (float)row[ja + lane];
             const long long nv = (jb - ja - head) / V;
             const T* vec = row + ja + head;
-            for (long long n = lane; n < nv; n += 64) {
+            long long n = lane;
+            for (; n + 192 < nv; n += 256) {                   // four loads in flight
+                float f[4][V];
+#pragma unroll
+                for (int w = 0; w < 4; ++w) load_vec<T, V>(vec + (n + 64 * w) * V, f[w]);
+#pragma unroll
+                for (int u = 0; u < V; ++u) s[u] += (f[0][u] + f[1][u]) + (f[2][u] + f[3][u]);
+            }
+            for (; n < nv; n += 64) {
                 float f[V];
                 load_vec<T, V>(vec + n * V, f);
 #pragma unroll
@@ -146,24 +154,23 @@ __global__ __launch_bounds__(256) void relbias_bwd_kernel(const T* dout, float* 
     if (threadIdx.x < 2) out[threadIdx.x ? last : 0] = (red[threadIdx.x][0] + red[threadIdx.x][1]) + (red[threadIdx.x][2] + red[threadIdx.x][3]);
 }
 
-// dtable[b][h]: a workgroup a head adds the chunks of every line entry (a thread an entry), then each bucket's entries, in 64 bits
-__global__ __launch_bounds__(1024) void relbias_table_kernel(const float* part, float* dtable, tcvom_rel_buckets bk, int heads, int chunks) {
-    extern __shared__ double sums[];
-    const int h = blockIdx.x, reach = line_reach(bk), last = reach + line_right(bk);
-    const float* p = part + (long long)h * chunks * (last + 1);
-    for (int t = threadIdx.x; t <= last; t += 1024) {
-        double s = 0.;
-        for (int c = 0; c < chunks; ++c) s += (double)p[(long long)c * (last + 1) + t];
-        sums[t] = s;
-    }
+// dtable[b][h]: a workgroup a bucket and head adds the bucket's line entries of every chunk, in 64 bits
+__global__ __launch_bounds__(256) void relbias_table_kernel(const float* part, float* dtable, tcvom_rel_buckets bk, int heads, int chunks) {
+    __shared__ double red[4];
+    const int b = blockIdx.x, h = blockIdx.y, last = line_reach(bk) + line_right(bk);
+    int t0, t1;
+    bucket_entries(bk, b, t0, t1);
+    const int n = t1 - t0;
+    const float* p = part + (long long)h * chunks * (last + 1) + t0;
+    double s = 0.;
+    if (n > 0)
+#pragma unroll 4
+        for (int e = threadIdx.x; e < n * chunks; e += 256) s += (double)p[(long long)(e / n) * (last + 1) + e % n];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    for (int b = threadIdx.x; b < bk.num_buckets; b += 1024) {
-        int t0, t1;
-        bucket_entries(bk, b, t0, t1);
-        double s = 0.;
-        for (int t = t0; t < t1; ++t) s += sums[t];
-        dtable[b * heads + h] = (float)s;
-    }
+    if (threadIdx.x == 0) dtable[b * heads + h] = (float)((red[0] + red[1]) + (red[2] + red[3]));
 }
 
 extern "C" int64_t tcvom_relbias_bwd_work(const tcvom_rel_buckets* buckets, int32_t heads, int64_t q_len) {
@@ -176,7 +183,7 @@ extern "C" int tcvom_relbias_bwd(const void* dout, float* dtable, float* work, i
     TCVOM_CHECK_ARG(dout && dtable && work && heads > 0 && heads <= 65535 && q_len > 0 && k_len > 0,
                     "relbias_bwd: heads=%d q_len=%lld k_len=%lld", heads, (long long)q_len, (long long)k_len);
     TCVOM_CHECK_ARG(type >= TCVOM_TYPE_F32 && type <= TCVOM_TYPE_F16, "relbias_bwd: type %d", type);
-    TCVOM_CHECK_ARG(q_len <= 65535LL * BIAS_ROWS && k_len < (1LL << 31) && q_start < (1LL << 40) && q_start > -(1LL << 40),
+    TCVOM_CHECK_ARG(q_len <= 65535LL * BIAS_ROWS && (int64_t)cdiv(q_len, BIAS_ROWS) * TCVOM_MAX_BUCKET_REACH < (1LL << 31) && k_len < (1LL << 31) && q_start < (1LL << 40) && q_start > -(1LL << 40),
                     "relbias_bwd: lengths");
     if (const int rc = check_buckets("relbias_bwd", buckets)) return rc;
     TCVOM_CHECK_ARG(work_floats >= tcvom_relbias_bwd_work(buckets, heads, q_len), "relbias_bwd: %lld floats of workspace", (long long)work_floats);
@@ -190,7 +197,7 @@ extern "C" int tcvom_relbias_bwd(const void* dout, float* dtable, float* work, i
     else
         hipLaunchKernelGGL(relbias_bwd_kernel<_Float16>, grid, dim3(256), 0, st, (const _Float16*)dout, work, *buckets, q_len, k_len, q_start);
     TCVOM_LAUNCH_CHECK("relbias_bwd");
-    hipLaunchKernelGGL(relbias_table_kernel, dim3(heads), dim3(1024), sizeof(double) * (last + 1), st, work, dtable, *buckets, heads, chunks);
+    hipLaunchKernelGGL(relbias_table_kernel, dim3(buckets->num_buckets, heads), dim3(256), 0, st, work, dtable, *buckets, heads, chunks);
     TCVOM_LAUNCH_CHECK("relbias_table");
     return 0;
 }

@@ -31,6 +31,18 @@ __device__ __forceinline__ void load_vec(const T* p, float (&f)[V]) {
         for (int j = 0; j < V; ++j) f[j] = (float)q[j];
     }
 }
+// the same in two steps, for loads that are issued ahead of their use
+template <class T, int V> struct RawVec { typedef T type __attribute__((ext_vector_type(V))); };
+template <class T> struct RawVec<T, 1> { typedef T type; };
+template <class T, int V>
+__device__ __forceinline__ typename RawVec<T, V>::type load_raw(const T* p) { return *reinterpret_cast<const typename RawVec<T, V>::type*>(p); }
+template <class T, int V>
+__device__ __forceinline__ void raw_to_float(const typename RawVec<T, V>::type& q, float (&f)[V]) {
+    if constexpr (V == 1) f[0] = (float)q;
+    else
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = (float)q[j];
+}
 template <class T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float (&f)[V]) {
     if constexpr (V == 1) {

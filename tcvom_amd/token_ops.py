@@ -25,22 +25,54 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def _check_cuda(name, *tensors):
-    dev = None
+    """Tensors (or None) of one GPU."""
+    index = None
     for t in tensors:
         if t is None:
             continue
-        if not torch.is_tensor(t):
+        if not isinstance(t, torch.Tensor):
             raise TypeError('%s: expected a tensor, got %s' % (name, type(t).__name__))
         if not t.is_cuda:
             raise RuntimeError('tcvom_amd ops run on the GPU through libtcvom_hip.so only (no CPU fallback); %s got a %s tensor'
                                % (name, t.device))
-        if dev is not None and t.device != dev:
-            raise RuntimeError('%s: tensors on %s and %s' % (name, dev, t.device))
-        dev = t.device
+        i = t.get_device()
+        if index is not None and i != index:
+            raise RuntimeError('%s: tensors on cuda:%d and cuda:%d' % (name, index, i))
+        index = i
 
 
 def _c(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _launch(device, name, *args):
+    """An entry point of the library on the current stream of the tensors' device, whatever the current device is.  (The stream's
+    handle is asked for directly: a call's host time is what its smallest sizes cost.)"""
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if torch.cuda.current_device() == device:
+        return L.call(name, *args, stream)
+    with torch.cuda.device(device):
+        return L.call(name, *args, stream)
+
+
+def _first_order(backward):
+    """once_differentiable, whose wrapping is left out of the usual backward (which builds no graph)."""
+    guarded = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
+
+
+def _tracked(*tensors):
+    """Whether autograd has to see the call."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 # =============================================================================================
@@ -71,7 +103,6 @@ def rel_buckets(num_buckets, max_distance, bidirectional):
 
 
 def _check_table(name, table):
-    _check_cuda(name, table)
     if table.dim() != 2 or table.dtype != torch.float32:
         raise ValueError('%s: the table is fp32 [buckets, heads], got %s %s' % (name, table.dtype, tuple(table.shape)))
 
@@ -79,29 +110,32 @@ def _check_table(name, table):
 # =============================================================================================
 # the bias as a matrix
 # =============================================================================================
+def _rel_bias(table, buckets, q_len, k_len, q_start, dtype):
+    heads = table.shape[1]
+    out = torch.empty((heads, q_len, k_len), dtype=dtype, device=table.device)
+    _launch(table.get_device(), 'tcvom_relbias_fwd', _c(table).data_ptr(), out.data_ptr(), C.byref(buckets), heads, q_len, k_len, q_start,
+            _TYPES[dtype])
+    return out
+
+
 class _RelBias(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, buckets, q_len, k_len, q_start, dtype):
-        heads = table.shape[1]
-        with torch.cuda.device(table.device):
-            out = torch.empty((heads, q_len, k_len), dtype=dtype, device=table.device)
-            L.call('tcvom_relbias_fwd', L.ptr(_c(table)), L.ptr(out), C.byref(buckets), heads, q_len, k_len, q_start, _TYPES[dtype],
-                   L.stream_ptr())
-        ctx.args = (buckets, heads, q_len, k_len, q_start, dtype)
-        return out
+    def forward(ctx, table, *args):
+        ctx.args = (table.shape[1],) + args
+        return _rel_bias(table, *args)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
-        buckets, heads, q_len, k_len, q_start, dtype = ctx.args
-        with torch.cuda.device(dout.device):
-            dtable = torch.empty((buckets.num_buckets, heads), dtype=torch.float32, device=dout.device)
-            if q_len == 0 or k_len == 0:
-                return dtable.zero_(), None, None, None, None, None
-            n = L.call('tcvom_relbias_bwd_work', C.byref(buckets), heads, q_len)
-            work = torch.empty(n, dtype=torch.float32, device=dout.device)
-            L.call('tcvom_relbias_bwd', L.ptr(_c(dout)), L.ptr(dtable), L.ptr(work), n, C.byref(buckets), heads, q_len, k_len, q_start,
-                   _TYPES[dtype], L.stream_ptr())
+        heads, buckets, q_len, k_len, q_start, dtype = ctx.args
+        dtable = torch.empty((buckets.num_buckets, heads), dtype=torch.float32, device=dout.device)
+        if q_len == 0 or k_len == 0:
+            return dtable.zero_(), None, None, None, None, None
+        dout = _c(dout)
+        n = L.call('tcvom_relbias_bwd_work', C.byref(buckets), heads, q_len)
+        work = torch.empty(n, dtype=torch.float32, device=dout.device)
+        _launch(dout.get_device(), 'tcvom_relbias_bwd', dout.data_ptr(), dtable.data_ptr(), work.data_ptr(), n, C.byref(buckets), heads,
+                q_len, k_len, q_start, _TYPES[dtype])
         return dtable, None, None, None, None, None
 
 
@@ -112,13 +146,15 @@ def relative_position_bias(table, q_len, k_len, max_distance=128, bidirectional=
     |j - i - q_start|); one-sided: every key after the query counts as distance 0.  The first half of a side's buckets hold one
     distance each, the others grow geometrically up to max_distance (at most 1024), the last holds everything beyond.  q_start:
     position of the first query."""
+    _check_cuda('relative_position_bias', table)
     _check_table('relative_position_bias', table)
     if dtype not in _TYPES:
         raise TypeError('relative_position_bias: dtype %s' % dtype)
     if q_len < 0 or k_len < 0:
         raise ValueError('relative_position_bias: lengths %d, %d' % (q_len, k_len))
     buckets = rel_buckets(table.shape[0], int(max_distance), bool(bidirectional))
-    return _RelBias.apply(table, buckets, int(q_len), int(k_len), int(q_start), dtype)
+    run = _RelBias.apply if _tracked(table) else _rel_bias
+    return run(table, buckets, int(q_len), int(k_len), int(q_start), dtype)
 
 
 # =============================================================================================
@@ -131,64 +167,57 @@ def _rows16(t):
 
 
 def _strides(t):
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape[:3])]
+    a, b, c, _ = t.stride()
+    x, y, z, _ = t.shape
+    return a if x > 1 else 0, b if y > 1 else 0, c if z > 1 else 0
 
 
 def _attn_desc(q, k, v, buckets, causal, scale, k_lens, key_mask, q_start, q_starts):
-    d = L.AttnDesc()
-    d.B, d.Nq, d.H, d.D = q.shape
-    d.Nk, d.Hkv = k.shape[1], k.shape[2]
-    d.type, d.causal, d.scale, d.q_start = _TYPES[q.dtype], int(causal), scale, q_start
-    d.q_stride[:], d.k_stride[:], d.v_stride[:] = _strides(q), _strides(k), _strides(v)
-    d.k_lens = None if k_lens is None else k_lens.data_ptr()
-    d.q_starts = None if q_starts is None else q_starts.data_ptr()
-    d.key_mask = None if key_mask is None else key_mask.data_ptr()
-    d.buckets = buckets
-    return d
+    B, Nq, H, D = q.shape
+    return L.AttnDesc(B, Nq, k.shape[1], H, k.shape[2], D, _TYPES[q.dtype], causal, q_start, scale, _strides(q), _strides(k), _strides(v),
+                      _p(k_lens), _p(q_starts), _p(key_mask), buckets)
+
+
+def _attention(q, k, v, table, train, out_lo, *args):
+    """(out, lse or None) of tensors in the kernels' layout."""
+    d = C.byref(_attn_desc(q, k, v, *args))
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if train else None
+    lo = torch.empty_like(out) if out_lo else None
+    n = L.call('tcvom_attn_fwd_work', d)
+    work = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    _launch(q.get_device(), 'tcvom_attn_fwd', d, q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), out.data_ptr(), _p(lo), _p(lse),
+            _p(work), n)
+    return out, lo, lse
 
 
 class _BiasedAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, buckets, causal, scale, k_lens, key_mask, q_start, q_starts):
+    def forward(ctx, q, k, v, table, *args):
         q, k, v, table = _rows16(q), _rows16(k), _rows16(v), _c(table)
-        train = any(ctx.needs_input_grad[:4])
-        with torch.cuda.device(q.device):
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            lse = out_lo = work = None
-            if train:
-                lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
-                if ctx.needs_input_grad[3]:
-                    out_lo = torch.empty_like(out)
-            d = _attn_desc(q, k, v, buckets, causal, scale, k_lens, key_mask, q_start, q_starts)
-            n = L.call('tcvom_attn_fwd_work', C.byref(d))
-            if n:
-                work = torch.empty(n, dtype=torch.float32, device=q.device)
-            L.call('tcvom_attn_fwd', C.byref(d), L.ptr(q), L.ptr(k), L.ptr(v), L.ptr(table), L.ptr(out), L.ptr(out_lo), L.ptr(lse),
-                   L.ptr(work), n, L.stream_ptr())
-        if train:
-            ctx.save_for_backward(q, k, v, table, out, out_lo, lse, k_lens, key_mask, q_starts)
-            ctx.args = (buckets, causal, scale, q_start)
+        out, out_lo, lse = _attention(q, k, v, table, True, ctx.needs_input_grad[3], *args)
+        buckets, causal, scale, k_lens, key_mask, q_start, q_starts = args
+        ctx.save_for_backward(q, k, v, table, out, out_lo, lse, k_lens, key_mask, q_starts)
+        ctx.args = (buckets, causal, scale, q_start)
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
         q, k, v, table, out, out_lo, lse, k_lens, key_mask, q_starts = ctx.saved_tensors
         buckets, causal, scale, q_start = ctx.args
-        none = (None,) * 7
-        with torch.cuda.device(q.device):
-            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-            dtable = torch.empty_like(table) if ctx.needs_input_grad[3] else None
-            if q.numel() == 0 or k.numel() == 0:
-                return (dq.zero_(), dk.zero_(), dv.zero_(), None if dtable is None else dtable.zero_()) + none
-            dout = _rows16(dout)
-            d = _attn_desc(q, k, v, buckets, causal, scale, k_lens, key_mask, q_start, q_starts)
-            n = L.call('tcvom_attn_bwd_work', C.byref(d))
-            work = torch.empty(n, dtype=torch.float32, device=q.device)
-            L.call('tcvom_attn_bwd', C.byref(d), L.ptr(q), L.ptr(k), L.ptr(v), L.ptr(table), L.ptr(out), L.ptr(out_lo), L.ptr(lse),
-                   L.ptr(dout), (C.c_int64 * 3)(*_strides(dout)), L.ptr(dq), L.ptr(dk), L.ptr(dv), L.ptr(dtable), L.ptr(work), n,
-                   L.stream_ptr())
-        return (dq, dk, dv, dtable) + none
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dtable = torch.empty_like(table) if ctx.needs_input_grad[3] else None
+        if q.numel() == 0 or k.numel() == 0:
+            return (dq.zero_(), dk.zero_(), dv.zero_(), None if dtable is None else dtable.zero_()) + (None,) * 7
+        dout = _rows16(dout)
+        d = C.byref(_attn_desc(q, k, v, buckets, causal, scale, k_lens, key_mask, q_start, q_starts))
+        n = L.call('tcvom_attn_bwd_work', d)
+        work = torch.empty(n, dtype=torch.float32, device=q.device)
+        _launch(q.get_device(), 'tcvom_attn_bwd', d, q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), out.data_ptr(), _p(out_lo),
+                lse.data_ptr(), dout.data_ptr(), (C.c_int64 * 3)(*_strides(dout)), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(dtable),
+                work.data_ptr(), n)
+        return dq, dk, dv, dtable, None, None, None, None, None, None, None
 
 
 def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causal=False, scale=None, k_lens=None, key_mask=None,
@@ -207,7 +236,10 @@ def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causa
     Gradients of q, k, v and table.  Probabilities and their gradients are rounded to the 16-bit type as operands of the matrix
     products, everything else is held in 32 bits."""
     name = 'biased_attention'
-    _check_cuda(name, q, k, v, table, k_lens, key_mask)
+    q_starts = None
+    if isinstance(q_start, torch.Tensor):
+        q_starts, q_start = q_start, 0
+    _check_cuda(name, q, k, v, table, k_lens, key_mask, q_starts)
     _check_table(name, table)
     if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError('%s: q, k, v are all bf16 or all fp16, got %s, %s, %s' % (name, q.dtype, k.dtype, v.dtype))
@@ -224,13 +256,9 @@ def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causa
     scale = D ** -0.5 if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError('%s: scale %g' % (name, scale))
-    q_starts = None
-    if torch.is_tensor(q_start):
-        q_starts, q_start = q_start, 0
     for what, t in (('k_lens', k_lens), ('q_start', q_starts)):
         if t is not None and (t.dtype != torch.int32 or t.shape != (B,)):
             raise ValueError('%s: %s is int32 [%d], got %s %s' % (name, what, B, t.dtype, tuple(t.shape)))
-    _check_cuda(name, q, q_starts)
     if key_mask is not None:
         if key_mask.dtype not in (torch.bool, torch.uint8) or key_mask.shape != (B, Nk):
             raise ValueError('%s: key_mask is bool or uint8 [%d, %d], got %s %s' % (name, B, Nk, key_mask.dtype, tuple(key_mask.shape)))
@@ -238,63 +266,69 @@ def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causa
     if not -(1 << 29) <= int(q_start) <= 1 << 29:
         raise ValueError('%s: q_start %d' % (name, q_start))
     buckets = rel_buckets(table.shape[0], int(max_distance), bool(not causal if bidirectional is None else bidirectional))
-    return _BiasedAttention.apply(q, k, v, table, buckets, bool(causal), scale, _c(k_lens), key_mask, int(q_start), _c(q_starts))
+    args = (buckets, int(causal), scale, _c(k_lens), key_mask, int(q_start), _c(q_starts))
+    if _tracked(q, k, v, table):
+        return _BiasedAttention.apply(q, k, v, table, *args)
+    return _attention(_rows16(q), _rows16(k), _rows16(v), _c(table), False, False, *args)[0]
 
 
 # =============================================================================================
 # norms around a block
 # =============================================================================================
+def _block_norm(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, train, gate_rows, branch_scale, residual_scale, eps, layer):
+    """(x', h, row statistics or None) of contiguous tensors."""
+    channels = x.shape[-1]
+    tokens = x.numel() // channels
+    y_type = x.dtype if y is None else y.dtype
+    xo = None if y is None else torch.empty_like(x)
+    h = None if pre_weight is None else torch.empty_like(x if y is None else y)
+    stats = torch.empty((tokens, 4), dtype=torch.float32, device=x.device) if train else None
+    _launch(x.get_device(), 'tcvom_block_norm_fwd', x.data_ptr(), _p(y), _p(post_weight), _p(post_bias), _p(gate),
+            int(gate is not None and gate.dtype == torch.float32), gate_rows, _p(pre_weight), _p(pre_bias), branch_scale, residual_scale, eps,
+            layer, _p(xo), _p(h), _p(stats), tokens, channels, _TYPES[x.dtype], _TYPES[y_type])
+    return xo, h, stats
+
+
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, y, post_weight, post_bias, gate, pre_weight, pre_bias, gate_rows, branch_scale, residual_scale, eps, layer):
+    def forward(ctx, x, y, post_weight, post_bias, gate, pre_weight, pre_bias, *args):
         ctx.set_materialize_grads(False)
         x, y, post_weight, post_bias, gate, pre_weight, pre_bias = (_c(t) for t in (x, y, post_weight, post_bias, gate, pre_weight, pre_bias))
-        Cc = x.shape[-1]
-        T = x.numel() // Cc
-        y_type = x.dtype if y is None else y.dtype
-        train = any(ctx.needs_input_grad[:7])
-        with torch.cuda.device(x.device):
-            xo = None if y is None else torch.empty_like(x)
-            h = None if pre_weight is None else torch.empty(x.shape, dtype=y_type, device=x.device)
-            stats = torch.empty((T, 4), dtype=torch.float32, device=x.device) if train else None
-            L.call('tcvom_block_norm_fwd', L.ptr(x), L.ptr(y), L.ptr(post_weight), L.ptr(post_bias), L.ptr(gate),
-                   int(gate is not None and gate.dtype == torch.float32), gate_rows, L.ptr(pre_weight), L.ptr(pre_bias), branch_scale,
-                   residual_scale, eps, int(layer), L.ptr(xo), L.ptr(h), L.ptr(stats), T, Cc, _TYPES[x.dtype], _TYPES[y_type],
-                   L.stream_ptr())
-        if train:
-            ctx.save_for_backward(x, y, post_weight, post_bias, gate, pre_weight, stats)
-            ctx.args = (gate_rows, branch_scale, residual_scale, layer, T, Cc, y_type)
+        xo, h, stats = _block_norm(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, True, *args)
+        ctx.save_for_backward(x, y, post_weight, post_bias, gate, pre_weight, stats)
+        ctx.args = args
         return xo, h
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dxo, dh):
         x, y, post_weight, post_bias, gate, pre_weight, stats = ctx.saved_tensors
-        gate_rows, branch_scale, residual_scale, layer, T, Cc, y_type = ctx.args
+        gate_rows, branch_scale, residual_scale, _, layer = ctx.args
         need = ctx.needs_input_grad
         if dxo is None and dh is None:
             return (None,) * 12
-        with torch.cuda.device(x.device):
-            dxo, dh = _c(dxo), _c(dh)
+        dxo, dh = _c(dxo), _c(dh)
 
-            def like(t, wanted=True):
-                return torch.empty_like(t) if t is not None and wanted else None
+        def like(t, wanted=True):
+            return torch.empty_like(t) if t is not None and wanted else None
 
-            pre = dh is not None
-            dx, dy = like(x), like(y)
-            dw1, db1, dg = like(post_weight, need[2]), like(post_bias, need[3]), like(gate, need[4])
-            dw2 = like(pre_weight, need[5] and pre)
-            db2 = torch.empty(Cc, dtype=torch.float32, device=x.device) if need[6] and pre else None
-            if T == 0:
-                return tuple(None if t is None else t.zero_() for t in (dx, dy, dw1, db1, dg, dw2, db2)) + (None,) * 5
-            groups = T // gate_rows if gate is not None and gate_rows > 1 else 1
-            n = L.call('tcvom_block_norm_bwd_work', T, Cc, groups)
-            work = torch.empty(n, dtype=torch.float32, device=x.device)
-            L.call('tcvom_block_norm_bwd', L.ptr(x), L.ptr(y), L.ptr(post_weight), L.ptr(post_bias), L.ptr(gate),
-                   int(gate is not None and gate.dtype == torch.float32), gate_rows, L.ptr(pre_weight), branch_scale, residual_scale,
-                   int(layer), L.ptr(stats), L.ptr(dxo), L.ptr(dh), L.ptr(dx), L.ptr(dy), L.ptr(dw1), L.ptr(db1), L.ptr(dg), L.ptr(dw2),
-                   L.ptr(db2), L.ptr(work), n, T, Cc, _TYPES[x.dtype], _TYPES[y_type], L.stream_ptr())
-        return (dx, dy, dw1, db1, dg, dw2, db2) + (None,) * 5
+        pre = dh is not None
+        channels = x.shape[-1]
+        tokens = x.numel() // channels
+        dx, dy = like(x), like(y)
+        dw1, db1, dg = like(post_weight, need[2]), like(post_bias, need[3]), like(gate, need[4])
+        dw2 = like(pre_weight, need[5] and pre)
+        db2 = torch.empty(channels, dtype=torch.float32, device=x.device) if need[6] and pre else None
+        if tokens == 0:
+            return tuple(None if t is None else t.zero_() for t in (dx, dy, dw1, db1, dg, dw2, db2)) + (None,) * 5
+        groups = tokens // gate_rows if gate is not None and gate_rows > 1 else 1
+        n = L.call('tcvom_block_norm_bwd_work', tokens, channels, groups)
+        work = torch.empty(n, dtype=torch.float32, device=x.device)
+        _launch(x.get_device(), 'tcvom_block_norm_bwd', x.data_ptr(), _p(y), _p(post_weight), _p(post_bias), _p(gate),
+                int(gate is not None and gate.dtype == torch.float32), gate_rows, _p(pre_weight), branch_scale, residual_scale, layer,
+                stats.data_ptr(), _p(dxo), _p(dh), dx.data_ptr(), _p(dy), _p(dw1), _p(db1), _p(dg), _p(dw2), _p(db2), work.data_ptr(), n,
+                tokens, channels, _TYPES[x.dtype], _TYPES[x.dtype if y is None else y.dtype])
+        return dx, dy, dw1, db1, dg, dw2, db2, None, None, None, None, None
 
 
 def _gate_rows(x, gate):
@@ -350,6 +384,7 @@ def block_norm(x, y, post_weight=None, post_bias=None, gate=None, branch_scale=1
         rows = _gate_rows(x, gate)
         if rows > 1 and x.numel() // x.shape[-1] // rows > 32768:
             raise ValueError('%s: %d gate rows of several tokens (at most 32768)' % (name, x.numel() // x.shape[-1] // rows))
-    xo, h = _BlockNorm.apply(x, y, post_weight, post_bias, gate, pre_weight, pre_bias, rows, float(branch_scale), float(residual_scale),
-                             float(eps), kind == 'layer')
+    args = (rows, float(branch_scale), float(residual_scale), float(eps), int(kind == 'layer'))
+    tensors = (x, y, post_weight, post_bias, gate, pre_weight, pre_bias)
+    xo, h = _BlockNorm.apply(*tensors, *args) if _tracked(*tensors) else _block_norm(*(_c(t) for t in tensors), False, *args)[:2]
     return (x if y is None else xo), h
