@@ -71,11 +71,19 @@ __device__ __forceinline__ int seq_start(const AttnArgs& a, int b) {
     return s < -(1 << 29) ? -(1 << 29) : s > (1 << 29) ? (1 << 29) : s;
 }
 
-// workgroup -> work item: the hardware deals workgroups round-robin over the 8 XCDs, each with its own L2; consecutive items (tiles that
-// share keys and values) go to one XCD
-__device__ __forceinline__ int xcd_item(int id, int total) {
-    const int per = total / 8, whole = per * 8;
-    return id < whole ? (id & 7) * per + (id >> 3) : id;
+// workgroup -> (sequence and head, tile).  The hardware deals workgroups round-robin over the 8 XCDs, each with its own L2: the tiles of a
+// head, which share keys and values (or queries), stay on one.  Tiles of causal heads differ in work: all heads' longest ones go
+// first, so that none starts late (2 x 4080 tokens, 16 heads of 128: see attn_dkv_kernel); otherwise head by head, the fewest heads in an L2.
+__device__ __forceinline__ void work_item(const AttnArgs& a, int heads, int& bh, int& tile) {
+    const int id = blockIdx.x, total = gridDim.x;
+    if (a.causal && heads % 8 == 0) {
+        tile = id / heads;
+        bh = id % heads;
+        return;
+    }
+    const int per = total / 8, whole = per * 8, item = id < whole ? (id & 7) * per + (id >> 3) : id;
+    bh = item / a.tiles;
+    tile = item % a.tiles;
 }
 
 // LDS position of 16-byte chunk c of row r, rows of DP elements.  The XOR spreads over the 64 banks (256 bytes) both (a) fragment reads, 16
@@ -88,7 +96,7 @@ template <int DP> __device__ __forceinline__ int chunk_at(int r, int c) {
 
 __device__ __forceinline__ float half_max(float v) {       // maximum over lanes l and l ^ 32
     const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    return __builtin_elementwise_maximum(__uint_as_float(s[0]), __uint_as_float(s[1]));
 }
 __device__ __forceinline__ float half_sum(float v) {
     const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -150,17 +158,57 @@ __device__ __forceinline__ V8 load_or_zero(bool ok, const T* p) {
     if (ok) z = *reinterpret_cast<const V8*>(p);
     return z;
 }
+// One thread's share of moving a tile of ROWS rows from memory to registers and on to LDS (256 threads): rows threadIdx.x / CH + n 256 / CH,
+// 16-byte chunk threadIdx.x % CH.
+template <class T, int DP, int ROWS> struct Mover {
+    static constexpr int CH = DP / 8, STEP = 256 / CH, PER = (ROWS * CH + 255) / 256;
+    u32x4_t reg[PER];
+    // rows `first` .. of the tile whose row 0 is at `base`; `left` of them exist, `ok(row)` says which count; the others are zeros
+    template <class F>
+    __device__ __forceinline__ void load(const T* base, long long stride, int left, int D, bool all, F ok) {
+        const int r0 = threadIdx.x / CH, c = threadIdx.x % CH;
+        const unsigned off = (unsigned)(r0 * (int)stride + c * 8) * 2u;         // strides below 2^24 (attn_check)
+        if (left >= ROWS && D == DP && all && (ROWS * CH) % 256 == 0) {
+#pragma unroll
+            for (int n = 0; n < PER; ++n)
+                reg[n] = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const char*>(base + n * STEP * stride) + off);
+            return;
+        }
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            const int r = r0 + n * STEP;
+            u32x4_t z = {0, 0, 0, 0};
+            if (r < ROWS && r < left && c * 8 < D && (all || ok(r)))
+                z = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const char*>(base + n * STEP * stride) + off);
+            reg[n] = z;
+        }
+    }
+    __device__ __forceinline__ void store(T* tile) const {
+        const int r0 = threadIdx.x / CH, c = threadIdx.x % CH;
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+            const int r = r0 + n * STEP;
+            if ((ROWS * CH) % 256 == 0 || r < ROWS) *reinterpret_cast<u32x4_t*>(&tile[chunk_at<DP>(r, c) * 8]) = reg[n];
+        }
+    }
+};
+// NaN stays NaN; v_maximum3_f32
+__device__ __forceinline__ float max2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ f32x16_t zero16() {
     f32x16_t z;
 #pragma unroll
     for (int r = 0; r < 16; ++r) z[r] = 0.f;
     return z;
 }
-// the line of head h, times log2(e)
+// the line of head h, times log2(e), in line[0 .. last]; its two ends are repeated MARGIN entries outwards, so that a tile of 64 x 64 that
+// crosses the line reads it without clamping
+constexpr int MARGIN = 128;
 __device__ __forceinline__ void fill_line(float* line, const AttnArgs& a, int h, int threads) {
     const int reach = line_reach(a.bk), last = reach + line_right(a.bk);
-    for (int t = threadIdx.x; t <= last; t += threads) line[t] = a.table[rel_bucket(a.bk, t - reach) * a.H + h] * LOG2E;
+    for (int t = (int)threadIdx.x - MARGIN; t <= last + MARGIN; t += threads)
+        line[t] = a.table[rel_bucket(a.bk, min(max(t, 0), last) - reach) * a.H + h] * LOG2E;
 }
+static inline size_t line_bytes(const AttnArgs& a) { return sizeof(float) * (line_reach(a.bk) + line_right(a.bk) + 1 + 2 * MARGIN); }
 
 // host side
 int attn_check(const char* who, const tcvom_attn_desc* d, AttnArgs* a);

@@ -1,5 +1,9 @@
 // Forward of the attention with a relative position bias (attn.h), reached through tcvom_attn_fwd.
 #include "attn.h"
+#include <type_traits>
+
+// a row without a key is zero; a sum that is NaN makes the row NaN
+__device__ __forceinline__ float empty_or(float sum, float v) { return sum == 0.f ? 0.f : v; }
 
 // ---- many queries: a workgroup of 4 waves takes 128 QB queries of one head, a wave 32 QB of them, all through the same tiles of 64 keys.
 // K and V tiles go to LDS through registers (the next tile's loads are in flight during this tile's products), two buffers, one
@@ -7,15 +11,16 @@
 template <class T, int DP, int QB, bool LO>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;
-    constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8, PER = KT * CH / 256;
-    constexpr int BM = 128 * QB;
-    __shared__ __align__(16) T lk[2][KT * DP];
-    __shared__ __align__(16) T lv[2][KT * DP];
-    extern __shared__ float line[];
+    constexpr int KS = DP / 16, DB = DP / 32, BM = 128 * QB, TILE = KT * DP;
+    __shared__ __align__(16) T lk[2 * TILE];
+    __shared__ __align__(16) T lv[2 * TILE];
+    extern __shared__ float line_[];
+    float* line = line_ + MARGIN;
 
-    const int item = xcd_item(blockIdx.x, gridDim.x);
-    const int bh = item / a.tiles, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
-    const int tile = a.causal ? a.tiles - 1 - item % a.tiles : item % a.tiles;          // long causal rows first
+    int bh, tile;
+    work_item(a, a.B * a.H, bh, tile);
+    if (a.causal) tile = a.tiles - 1 - tile;
+    const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
     const int i0 = tile * BM, start = seq_start(a, b), len = seq_keys(a, b);
     // keys any query of the workgroup sees
@@ -30,42 +35,24 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
     const T* V = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
     const unsigned char* mask = a.key_mask ? a.key_mask + (long long)b * a.Nk : nullptr;
 
+    const int w0 = i0 + wave * (32 * QB);                  // the wave's first query
     int qi[QB];
     v8 qf[QB][KS];
 #pragma unroll
     for (int u = 0; u < QB; ++u) {
-        qi[u] = i0 + (wave * QB + u) * 32 + col;
+        qi[u] = w0 + u * 32 + col;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             const int d = s * 16 + half * 8;
-            v8 z = {};
-            qf[u][s] = z;
-            if (qi[u] < a.Nq && d < a.D) qf[u][s] = *reinterpret_cast<const v8*>(Q + (long long)qi[u] * a.qs[1] + d);
+            qf[u][s] = load_or_zero<v8>(qi[u] < a.Nq && d < a.D, Q + (long long)qi[u] * a.qs[1] + d);
         }
     }
-
-    u32x4_t rk[PER], rv[PER];
+    Mover<T, DP, KT> mk, mv;
     auto fetch = [&](int t) {
-#pragma unroll
-        for (int n = 0; n < PER; ++n) {
-            const int idx = n * 256 + threadIdx.x, r = idx / CH, c = idx % CH, key = t * KT + r;
-            u32x4_t z = {0, 0, 0, 0};
-            rk[n] = z;
-            rv[n] = z;
-            if (key < kend && c * 8 < a.D) {
-                rk[n] = *reinterpret_cast<const u32x4_t*>(K + (long long)key * a.ks[1] + c * 8);
-                // values of masked keys count as zero: 0 x inf would not
-                if (!mask || mask[key]) rv[n] = *reinterpret_cast<const u32x4_t*>(V + (long long)key * a.vs[1] + c * 8);
-            }
-        }
-    };
-    auto store = [&](int buf) {
-#pragma unroll
-        for (int n = 0; n < PER; ++n) {
-            const int idx = n * 256 + threadIdx.x, r = idx / CH, c = idx % CH;
-            *reinterpret_cast<u32x4_t*>(&lk[buf][chunk_at<DP>(r, c) * 8]) = rk[n];
-            *reinterpret_cast<u32x4_t*>(&lv[buf][chunk_at<DP>(r, c) * 8]) = rv[n];
-        }
+        const int k0 = t * KT;
+        mk.load(K + k0 * a.ks[1], a.ks[1], kend - k0, a.D, true, [](int) { return true; });
+        // values of masked keys count as zero: 0 x inf would not
+        mv.load(V + k0 * a.vs[1], a.vs[1], kend - k0, a.D, !mask, [&](int r) { return mask[k0 + r] != 0; });
     };
 
     f32x16_t o[QB][DB];
@@ -75,111 +62,118 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
         m[u] = -INFINITY;
         l[u] = 0.f;
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[u][d][r] = 0.f;
+        for (int d = 0; d < DB; ++d) o[u][d] = zero16();
     }
     const float c = a.scale * LOG2E;
     const unsigned rows_at = Tile<T, DP>::rows_at(lane), cols_at = Tile<T, DP>::cols_at(lane);
     if (ntiles > 0) {
         fetch(0);
-        store(0);
+        mk.store(lk);
+        mv.store(lv);
     }
     __syncthreads();
     for (int t = 0; t < ntiles; ++t) {
-        const int buf = t & 1, k0 = t * KT;
-        const unsigned ra = keep(rows_at) + buf * (KT * DP * 2), ca = keep(cols_at) + buf * (KT * DP * 2);
+        const int k0 = t * KT, buf = (t & 1) * TILE;
+        const unsigned ra = keep(rows_at) + buf * 2, ca = keep(cols_at) + buf * 2;
         if (t + 1 < ntiles) fetch(t + 1);
-        unsigned long long bits = ~0ull;
-        if (mask) bits = __ballot(k0 + lane < a.Nk && mask[min(k0 + lane, a.Nk - 1)]);
-#pragma unroll
-        for (int u = 0; u < QB; ++u) {
-            // S^T of 64 keys x 32 queries
-            f32x16_t x[2];
+        // FAR: all relative positions of the tile lie past one end of the line, the bias is the constant `add`
+        auto body = [&](auto far_, float add) {
+            constexpr bool FAR = decltype(far_)::value;
+            f32x16_t x[QB][2];
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) x[kb][r] = 0.f;
+                for (int u = 0; u < QB; ++u) x[u][kb] = zero16();
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    x[kb] = Mma<T>::mma(Tile<T, DP>::rows(lk[0], ra, kb * 32, s), qf[u][s], x[kb]);
+                    const v8 kf = Tile<T, DP>::rows(lk, ra, kb * 32, s);
+#pragma unroll
+                    for (int u = 0; u < QB; ++u) x[u][kb] = Mma<T>::mma(kf, qf[u][s], x[u][kb]);
                 }
             }
-            const int w0 = i0 + (wave * QB + u) * 32;               // the wave's first query of this block
-            const int rel_hi = k0 + KT - 1 - w0 - start, rel_lo = k0 - (w0 + 31) - start;
-            const bool far = rel_hi <= -reach || rel_lo >= right;
-            float add = rel_hi <= -reach ? line[0] : line[last];
-            if (!far) {
-                add = 0.f;
-                int at = k0 + 4 * half - qi[u] - start + reach;       // line index of the lane's first key
+#pragma unroll
+            for (int u = 0; u < QB; ++u) {
+                if constexpr (!FAR) {
+                    const float* at = line + (k0 + 4 * half - qi[u] - start + reach);       // entry of the lane's first key
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x[u][kb][r] = fmaf(x[u][kb][r], c, at[kb * 32 + 8 * (r / 4) + r % 4]);
+                }
+                // keys the lane's query sees: bit n of `see` = key k0 + n
+                if (mask || k0 + KT > min(len, a.causal ? w0 + u * 32 + start + 1 : len)) {
+                    unsigned long long bits = ~0ull;
+                    if (mask) bits = __ballot(k0 + lane < a.Nk && mask[min(k0 + lane, a.Nk - 1)]);
+                    const int lim = min(len, a.causal ? qi[u] + start + 1 : len) - k0;
+                    const unsigned long long see = lim >= 64 ? bits : lim <= 0 ? 0 : bits & ((1ull << lim) - 1);
+                    const unsigned s0 = (unsigned)see >> (4 * half), s1 = (unsigned)(see >> 32) >> (4 * half);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        if (!(s0 >> (8 * (r / 4) + r % 4) & 1)) x[u][0][r] = -INFINITY;
+                        if (!(s1 >> (8 * (r / 4) + r % 4) & 1)) x[u][1][r] = -INFINITY;
+                    }
+                }
+                float top = max2(x[u][0][0], x[u][1][0]);
+#pragma unroll
+                for (int r = 1; r < 16; ++r) top = max2(top, max2(x[u][0][r], x[u][1][r]));
+                top = half_max(top);
+                if constexpr (FAR) top = fmaf(top, c, add);
+                const float mn = max2(m[u], top);
+                if (__any(mn > m[u])) {
+                    const float alpha = exp2_hw(m[u] - (mn == -INFINITY ? 0.f : mn));
+                    l[u] *= alpha;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[u][d][r] *= alpha;
+                    m[u] = mn;
+                }
+                const float sub = Mma<T>::shift - (m[u] == -INFINITY ? 0.f : m[u]) + (FAR ? add : 0.f);
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        const int e = at + kb * 32 + 8 * (r / 4) + r % 4;
-                        x[kb][r] = fmaf(x[kb][r], c, line[min(max(e, 0), last)]);
+                        x[u][kb][r] = exp2_hw(FAR ? fmaf(x[u][kb][r], c, sub) : x[u][kb][r] + sub);
+                        sum[r & 3] += x[u][kb][r];
                     }
+                l[u] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             }
-            const float mul = far ? c : 1.f;
-            // keys the lane's query sees: bit n of `see` = key k0 + n
-            const int lim = min(len, a.causal ? qi[u] + start + 1 : len) - k0;
-            if (bits != ~0ull || k0 + KT > min(len, a.causal ? w0 + start + 1 : len)) {
-                const unsigned long long see = lim >= 64 ? bits : lim <= 0 ? 0 : bits & ((1ull << lim) - 1);
-                const unsigned s0 = (unsigned)see >> (4 * half), s1 = (unsigned)(see >> 32) >> (4 * half);
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    if (!(s0 >> (8 * (r / 4) + r % 4) & 1)) x[0][r] = -INFINITY;
-                    if (!(s1 >> (8 * (r / 4) + r % 4) & 1)) x[1][r] = -INFINITY;
-                }
-            }
-            float top = fmaxf(x[0][0], x[1][0]);
-#pragma unroll
-            for (int r = 1; r < 16; ++r) top = fmaxf(top, fmaxf(x[0][r], x[1][r]));
-            top = half_max(top);
-            top = far ? fmaf(top, c, add) : top;
-            const float mn = fmaxf(m[u], top);
-            if (__any(mn > m[u])) {
-                const float base = mn == -INFINITY ? 0.f : mn;
-                const float alpha = exp2_hw(m[u] - base);
-                l[u] *= alpha;
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[u][d][r] *= alpha;
-                m[u] = mn;
-            }
-            const float sub = add + Mma<T>::shift - (m[u] == -INFINITY ? 0.f : m[u]);
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    x[kb][r] = exp2_hw(fmaf(x[kb][r], mul, sub));
-                    sum[r & 3] += x[kb][r];
-                }
-            l[u] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    const v8 p = pack_step<T>(x[kb], s);
-                    v8 rest;
-                    if constexpr (LO) rest = pack_rest<T>(x[kb], p, s);
+                    v8 p[QB], rest[QB];
+#pragma unroll
+                    for (int u = 0; u < QB; ++u) {
+                        p[u] = pack_step<T>(x[u][kb], s);
+                        if constexpr (LO) rest[u] = pack_rest<T>(x[u][kb], p[u], s);
+                    }
 #pragma unroll
                     for (int d = 0; d < DB; ++d) {
-                        const v8 vf = Tile<T, DP>::cols(lv[0], ca, kb * 32 + s * 16, d);
-                        o[u][d] = Mma<T>::mma(vf, p, o[u][d]);
-                        if constexpr (LO) o[u][d] = Mma<T>::mma(vf, rest, o[u][d]);
+                        const v8 vf = Tile<T, DP>::cols(lv, ca, kb * 32 + s * 16, d);
+#pragma unroll
+                        for (int u = 0; u < QB; ++u) {
+                            o[u][d] = Mma<T>::mma(vf, p[u], o[u][d]);
+                            if constexpr (LO) o[u][d] = Mma<T>::mma(vf, rest[u], o[u][d]);
+                        }
                     }
                 }
+        };
+        const int rel_hi = k0 + KT - 1 - w0 - start, rel_lo = k0 - (w0 + 32 * QB - 1) - start;
+        if (rel_hi <= -reach) body(std::true_type(), line[0]);
+        else if (rel_lo >= right) body(std::true_type(), line[last]);
+        else body(std::false_type(), 0.f);
+        if (t + 1 < ntiles) {
+            mk.store(lk + (TILE - buf));
+            mv.store(lv + (TILE - buf));
         }
-        if (t + 1 < ntiles) store(buf ^ 1);
         __syncthreads();
     }
 #pragma unroll
     for (int u = 0; u < QB; ++u) {
         const float sum = half_sum(l[u]);
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const float inv = 1.f / sum;
         if (qi[u] >= a.Nq) continue;
         const long long row = ((long long)b * a.Nq + qi[u]) * a.H + h;
 #pragma unroll
@@ -191,7 +185,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
                 typename Mma<T>::v4 w, lo;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float f = sum > 0.f ? o[u][d][4 * g + j] * inv : 0.f;
+                    const float f = empty_or(sum, o[u][d][4 * g + j] * inv);
                     w[j] = (T)f;
                     lo[j] = (T)(f - (float)w[j]);
                 }
@@ -199,7 +193,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
                 if (LO) *reinterpret_cast<typename Mma<T>::v4*>((T*)a.out_lo + row * a.D + at) = lo;
             }
         if (a.lse && half == 0)
-            a.lse[((long long)b * a.H + h) * a.Nq + qi[u]] = sum > 0.f ? m[u] + log2f(sum) - Mma<T>::shift : -INFINITY;
+            a.lse[((long long)b * a.H + h) * a.Nq + qi[u]] = sum == 0.f ? -INFINITY : m[u] + log2f(sum) - Mma<T>::shift;
     }
 }
 
@@ -312,8 +306,8 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
         }
         float top = x[0];
 #pragma unroll
-        for (int r = 1; r < 16; ++r) top = fmaxf(top, x[r]);
-        const float mn = fmaxf(m, half_max(top));
+        for (int r = 1; r < 16; ++r) top = max2(top, x[r]);
+        const float mn = max2(m, half_max(top));
         const float base = mn == -INFINITY ? 0.f : mn;
         if (__any(mn > m)) {
             const float alpha = exp2_hw(m - base);
@@ -375,7 +369,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     if (wave != 0 || !live) return;
     const long long out_row = ((long long)b * a.Nq + i) * a.H + h;
     if (a.splits == 1) {
-        const float inv = L > 0.f ? 1.f / L : 0.f;
+        const float inv = 1.f / L;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -384,10 +378,10 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
                 if (at >= a.D) continue;
                 typename Mma<T>::v4 w;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = (T)(L > 0.f ? o[d][4 * q + j] * inv : 0.f);
+                for (int j = 0; j < 4; ++j) w[j] = (T)empty_or(L, o[d][4 * q + j] * inv);
                 *reinterpret_cast<typename Mma<T>::v4*>((T*)a.out + out_row * a.D + at) = w;
             }
-        if (a.lse && half == 0) a.lse[((long long)b * a.H + h) * a.Nq + i] = L > 0.f ? M + log2f(L) - Mma<T>::shift : -INFINITY;
+        if (a.lse && half == 0) a.lse[((long long)b * a.H + h) * a.Nq + i] = L == 0.f ? -INFINITY : M + log2f(L) - Mma<T>::shift;
         return;
     }
     // partial [split][out_row][D + 2]: output, maximum, sum
@@ -430,14 +424,14 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
             o1 += w * f.y;
         }
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = 1.f / L;
     if (d < a.D) {
-        typename Mma<T>::v2 w = {(T)(L > 0.f ? o0 * inv : 0.f), (T)(L > 0.f ? o1 * inv : 0.f)};
+        typename Mma<T>::v2 w = {(T)empty_or(L, o0 * inv), (T)empty_or(L, o1 * inv)};
         *reinterpret_cast<typename Mma<T>::v2*>((T*)a.out + row * a.D + d) = w;
     }
     if (a.lse && lane == 0) {
         const long long b = row / ((long long)a.Nq * a.H), i = row / a.H % a.Nq, h = row % a.H;
-        a.lse[(b * a.H + h) * a.Nq + i] = L > 0.f ? M + log2f(L) - Mma<T>::shift : -INFINITY;
+        a.lse[(b * a.H + h) * a.Nq + i] = L == 0.f ? -INFINITY : M + log2f(L) - Mma<T>::shift;
     }
 }
 
@@ -453,6 +447,7 @@ int attn_check(const char* who, const tcvom_attn_desc* d, AttnArgs* a) {
     for (int n = 0; n < 3; ++n)
         TCVOM_CHECK_ARG(d->q_stride[n] % 8 == 0 && d->k_stride[n] % 8 == 0 && d->v_stride[n] % 8 == 0 && d->q_stride[n] >= 0 &&
                             d->k_stride[n] >= 0 && d->v_stride[n] >= 0, "%s: strides are multiples of 8 elements", who);
+    TCVOM_CHECK_ARG(d->q_stride[1] < (1 << 24) && d->k_stride[1] < (1 << 24) && d->v_stride[1] < (1 << 24), "%s: tokens 2^24 elements apart", who);
     if (const int rc = check_buckets(who, &d->buckets)) return rc;
     *a = AttnArgs();
     a->B = d->B; a->Nq = d->Nq; a->Nk = d->Nk; a->H = d->H; a->Hkv = d->Hkv; a->D = d->D;
@@ -496,7 +491,7 @@ static void launch_fwd(AttnArgs a, const tcvom_attn_desc* d, hipStream_t st) {
     constexpr int QB = 1;
     a.tiles = cdiv(a.Nq, 128 * QB);
     const dim3 grid((unsigned)((long long)a.B * a.H * a.tiles));
-    const size_t lds = sizeof(float) * (last + 1);
+    const size_t lds = line_bytes(a);
     if (a.out_lo) hipLaunchKernelGGL((attn_fwd_kernel<T, DP, QB, true>), grid, dim3(256), lds, st, a);
     else hipLaunchKernelGGL((attn_fwd_kernel<T, DP, QB, false>), grid, dim3(256), lds, st, a);
 }

@@ -8,23 +8,28 @@
 //
 // Rounding to 16 bits: p and ds as operands of the matrix products, as the forward rounds p.  The bucket sums take ds in 32 bits.
 #include "attn.h"
+#include <type_traits>
 
 // ---- dq, delta, bucket sums: a wave owns 32 queries of one head (S^T and dP^T as in the forward), the workgroup walks tiles of 64 keys.
-// Bucket sums: a tile past an end of the line adds to one register a lane; in a tile that crosses the line every element is added to
-// the entry of its relative position in LDS.  Each half wave has its own copy of the line, within which the 32 lanes of a step (one
-// key, 32 queries) have different entries, so that every entry is a sum in program order: equal calls give equal bits.
+// Bucket sums: a tile past an end of the line adds to one register a lane.  A 32 x 32 block that crosses it is written to LDS skewed, key
+// row n, query column c at [n][n - c + 31], where each of the 63 diagonals is a column that one lane adds up (the rest of the 64
+// columns was zeroed once and never written), then onto the wave's own line of sums.  Every sum is made in program order: equal calls
+// give equal bits.  (Adding the elements with LDS atomics took 53 cycles an instruction, one lane after the other: 16 of them a block
+// were as long as its matrix products.)
 template <class T, int DP, bool TABLE>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;
     constexpr int KT = DP == 128 ? 32 : 64;                 // keys a tile: two waves a SIMD fit the registers
-    constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8, PER = KT * CH / 256, BM = 128;
-    __shared__ __align__(16) T lk[2][KT * DP];
-    __shared__ __align__(16) T lv[2][KT * DP];
-    extern __shared__ float line[];
+    constexpr int KS = DP / 16, DB = DP / 32, BM = 128, TILE = KT * DP;
+    __shared__ __align__(16) T lk[2 * TILE];
+    __shared__ __align__(16) T lv[2 * TILE];
+    extern __shared__ float line_[];
+    float* line = line_ + MARGIN;
 
-    const int item = xcd_item(blockIdx.x, gridDim.x);
-    const int bh = item / a.tiles, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
-    const int tile = a.causal ? a.tiles - 1 - item % a.tiles : item % a.tiles;
+    int bh, tile;
+    work_item(a, a.B * a.H, bh, tile);
+    if (a.causal) tile = a.tiles - 1 - tile;
+    const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
     const int i0 = tile * BM, start = seq_start(a, b), len = seq_keys(a, b);
     const int i_last = min(i0 + BM, a.Nq) - 1;
@@ -32,10 +37,17 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     const int ntiles = (kend + KT - 1) / KT;
     const int reach = line_reach(a.bk), right = line_right(a.bk), last = reach + right;
     fill_line(line, a, h, 256);
-    float* sums = line + last + 1;                          // [8][last + 1]: half waves
-    if (TABLE)
-        for (int t = threadIdx.x; t < 8 * (last + 1); t += 256) sums[t] = 0.f;
-    float* mine = sums + (wave * 2 + half) * (last + 1);
+    // [4][last + 1 + 2 MARGIN]: a line of sums for each wave, with margins as the bias has
+    const int pitch = last + 1 + 2 * MARGIN;
+    float* sums = line_ + pitch;
+    __shared__ float skew[TABLE ? 4 * 32 * 64 : 1];
+    if (TABLE) {
+        for (int t = threadIdx.x; t < 4 * pitch; t += 256) sums[t] = 0.f;
+        for (int t = threadIdx.x; t < 4 * 32 * 64; t += 256) skew[t] = 0.f;
+    }
+    float* mine = sums + wave * pitch + MARGIN;
+    float* put = skew + (TABLE ? wave * (32 * 64) + 4 * half * 65 - col + 31 : 0);
+    const float* get = skew + (TABLE ? wave * (32 * 64) + lane : 0);
 
     const T* Q = (const T*)a.q + b * a.qs[0] + h * a.qs[2];
     const T* K = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
@@ -64,23 +76,12 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     delta = half_sum(delta);
     if (half == 0 && qi < a.Nq) a.delta[stat] = delta;
 
-    u32x4_t rk[PER], rv[PER];
+    Mover<T, DP, KT> mk, mv;
     auto fetch = [&](int t) {
-#pragma unroll
-        for (int n = 0; n < PER; ++n) {
-            const int idx = n * 256 + threadIdx.x, r = idx / CH, c = idx % CH, key = t * KT + r;
-            const bool ok = key < kend && c * 8 < a.D && (!mask || mask[key]);
-            rk[n] = load_or_zero<u32x4_t>(ok, K + (long long)key * a.ks[1] + c * 8);
-            rv[n] = load_or_zero<u32x4_t>(ok, V + (long long)key * a.vs[1] + c * 8);
-        }
-    };
-    auto store = [&](int buf) {
-#pragma unroll
-        for (int n = 0; n < PER; ++n) {
-            const int idx = n * 256 + threadIdx.x, r = idx / CH, c = idx % CH;
-            *reinterpret_cast<u32x4_t*>(&lk[buf][chunk_at<DP>(r, c) * 8]) = rk[n];
-            *reinterpret_cast<u32x4_t*>(&lv[buf][chunk_at<DP>(r, c) * 8]) = rv[n];
-        }
+        const int k0 = t * KT;
+        auto ok = [&](int r) { return mask[k0 + r] != 0; };
+        mk.load(K + k0 * a.ks[1], a.ks[1], kend - k0, a.D, !mask, ok);
+        mv.load(V + k0 * a.vs[1], a.vs[1], kend - k0, a.D, !mask, ok);
     };
     f32x16_t acc[DB];
 #pragma unroll
@@ -90,71 +91,78 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     const unsigned rows_at = Tile<T, DP>::rows_at(lane), cols_at = Tile<T, DP>::cols_at(lane);
     if (ntiles > 0) {
         fetch(0);
-        store(0);
+        mk.store(lk);
+        mv.store(lv);
     }
     __syncthreads();
     for (int t = 0; t < ntiles; ++t) {
-        const int buf = t & 1, k0 = t * KT;
-        const unsigned ra = keep(rows_at) + buf * (KT * DP * 2), ca = keep(cols_at) + buf * (KT * DP * 2);
+        const int k0 = t * KT, buf = (t & 1) * TILE;
+        const unsigned ra = keep(rows_at) + buf * 2, ca = keep(cols_at) + buf * 2;
         if (t + 1 < ntiles) fetch(t + 1);
-        unsigned long long bits = ~0ull;
-        if (mask) bits = __ballot(k0 + lane < a.Nk && mask[min(k0 + lane, a.Nk - 1)]);
-        const int lim = min(len, a.causal ? qi + start + 1 : len) - k0;
-        const bool holes = bits != ~0ull || k0 + KT > min(len, a.causal ? w0 + start + 1 : len);
-        const unsigned long long see = lim >= 64 ? bits : lim <= 0 ? 0 : bits & ((1ull << lim) - 1);
-        const int rel_hi = k0 + KT - 1 - w0 - start, rel_lo = k0 - (w0 + 31) - start;
-        const bool far = rel_hi <= -reach || rel_lo >= right;
+        const bool holes = mask || i0 + BM > a.Nq || k0 + KT > min(len, a.causal ? w0 + start + 1 : len);
+        // (as in the forward; far sums are taken by the caller from the returned sum of the lane's elements)
+        auto body = [&](auto far_, float add) {
+            constexpr bool FAR = decltype(far_)::value;
+            float total = 0.f;
+            unsigned long long see = 0;
+            if (holes) {                                    // (the whole wave: the ballot is over its 64 lanes)
+                unsigned long long bits = ~0ull;
+                if (mask) bits = __ballot(k0 + lane < a.Nk && mask[min(k0 + lane, a.Nk - 1)]);
+                const int lim = live ? min(len, a.causal ? qi + start + 1 : len) - k0 : 0;
+                see = lim >= 64 ? bits : lim <= 0 ? 0 : bits & ((1ull << lim) - 1);
+            }
 #pragma unroll
-        for (int kb = 0; kb < KT / 32; ++kb) {
-            f32x16_t x = zero16(), g = zero16();
+            for (int kb = 0; kb < KT / 32; ++kb) {
+                f32x16_t x = zero16(), g = zero16();
 #pragma unroll
-            for (int s = 0; s < KS; ++s) x = Mma<T>::mma(Tile<T, DP>::rows(lk[0], ra, kb * 32, s), qf[s], x);
+                for (int s = 0; s < KS; ++s) x = Mma<T>::mma(Tile<T, DP>::rows(lk, ra, kb * 32, s), qf[s], x);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) g = Mma<T>::mma(Tile<T, DP>::rows(lv[0], ra, kb * 32, s), gf[s], g);
-            const int at = k0 + kb * 32 + 4 * half - qi - start + reach;
-            if (far) {
-                const float add = (rel_hi <= -reach ? line[0] : line[last]) - lse;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = exp2_hw(fmaf(x[r], c, add));
-            } else {
+                for (int s = 0; s < KS; ++s) g = Mma<T>::mma(Tile<T, DP>::rows(lv, ra, kb * 32, s), gf[s], g);
+                const int e0 = k0 + kb * 32 + 4 * half - qi - start + reach;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int e = at + 8 * (r / 4) + r % 4;
-                    x[r] = exp2_hw(fmaf(x[r], c, line[min(max(e, 0), last)] - lse));
+                    const float b2 = FAR ? add - lse : line[e0 + 8 * (r / 4) + r % 4] - lse;
+                    x[r] = exp2_hw(fmaf(x[r], c, b2)) * (g[r] - delta);
                 }
-            }
+                if (holes) {
+                    const unsigned w = (unsigned)(see >> (32 * kb)) >> (4 * half);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] *= g[r] - delta;
-            if (holes || !live) {
-                const unsigned w = live ? (unsigned)(see >> (32 * kb)) >> (4 * half) : 0u;
+                    for (int r = 0; r < 16; ++r)
+                        if (!(w >> (8 * (r / 4) + r % 4) & 1)) x[r] = 0.f;
+                }
+                if (TABLE) {
+                    if constexpr (FAR) {
+                        float s[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!(w >> (8 * (r / 4) + r % 4) & 1)) x[r] = 0.f;
-            }
-            if (TABLE) {
-                if (far) {
-                    float s = 0.f;
+                        for (int r = 4; r < 16; ++r) s[r & 3] += x[r];
+                        total += (s[0] + s[1]) + (s[2] + s[3]);
+                    } else {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) s += x[r];
-                    if (rel_hi <= -reach) far_lo += s; else far_hi += s;
-                } else {
+                        for (int r = 0; r < 16; ++r) put[(8 * (r / 4) + r % 4) * 65] = x[r];
+                        float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int e = at + 8 * (r / 4) + r % 4;
-                        if (e <= 0) far_lo += x[r];
-                        else if (e >= last) far_hi += x[r];
-                        else atomicAdd(mine + e, x[r]);
+                        for (int n = 0; n < 32; ++n) s[n & 3] += get[n * 64];
+                        // diagonal key - query = lane - 31 of the block (lane 63: none, zero)
+                        mine[k0 + kb * 32 - w0 - start + reach + lane - 31] += (s[0] + s[1]) + (s[2] + s[3]);
                     }
                 }
-            }
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const v8 p = pack_step<T>(x, s);
+                for (int s = 0; s < 2; ++s) {
+                    const v8 p = pack_step<T>(x, s);
 #pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::mma(Tile<T, DP>::cols(lk[0], ca, kb * 32 + s * 16, d), p, acc[d]);
+                    for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::mma(Tile<T, DP>::cols(lk, ca, kb * 32 + s * 16, d), p, acc[d]);
+                }
             }
+            return total;
+        };
+        const int rel_hi = k0 + KT - 1 - w0 - start, rel_lo = k0 - (w0 + 31) - start;
+        if (rel_hi <= -reach) far_lo += body(std::true_type(), line[0]);
+        else if (rel_lo >= right) far_hi += body(std::true_type(), line[last]);
+        else body(std::false_type(), 0.f);
+        if (t + 1 < ntiles) {
+            mk.store(lk + (TILE - buf));
+            mv.store(lv + (TILE - buf));
         }
-        if (t + 1 < ntiles) store(buf ^ 1);
         __syncthreads();
     }
     if (qi < a.Nq) {
@@ -171,7 +179,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
             }
     }
     if (!TABLE) return;
-    // the half waves' lines become one (in place of the bias), with the far sums at its two ends, then the buckets' sums
+    // the waves' lines become one, entry by entry in order (in place of the bias); what lies past its ends -- whole tiles and the
+    // margins -- belongs to the end entries
     __shared__ float ends[2][4];
     const float lo = wave_sum(far_lo), hi = wave_sum(far_hi);
     if (lane == 0) {
@@ -179,22 +188,27 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
         ends[1][wave] = hi;
     }
     __syncthreads();
-    for (int t = threadIdx.x; t <= last; t += 256) {
+    for (int t = threadIdx.x; t < pitch; t += 256) {
         float s = 0.f;
-        if (t == 0 || t == last) {
-            const float* e = ends[t ? 1 : 0];
-            s = (e[0] + e[1]) + (e[2] + e[3]);
-        } else {
 #pragma unroll
-            for (int n = 0; n < 8; ++n) s += sums[n * (last + 1) + t];
-        }
-        line[t] = s;
+        for (int n = 0; n < 4; ++n) s += sums[n * pitch + t];
+        line_[t] = s;
     }
     __syncthreads();
     for (int n = threadIdx.x; n < a.bk.num_buckets; n += 256) {
         int t0, t1;
         bucket_entries(a.bk, n, t0, t1);
         float s = 0.f;
+        if (t0 < t1) {
+            if (t0 == 0) {
+                s = (ends[0][0] + ends[0][1]) + (ends[0][2] + ends[0][3]);
+                t0 = -MARGIN;
+            }
+            if (t1 == last + 1) {
+                s += (ends[1][0] + ends[1][1]) + (ends[1][2] + ends[1][3]);
+                t1 = last + 1 + MARGIN;
+            }
+        }
         for (int t = t0; t < t1; ++t) s += line[t];
         a.part[(((long long)h * a.B + b) * a.tiles + tile) * a.bk.num_buckets + n] = s;
     }
@@ -225,16 +239,18 @@ __global__ __launch_bounds__(1024) void attn_table_kernel(const float* part, flo
 template <class T, int DP>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;
-    constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8, QT = 32, PER = (QT * CH + 255) / 256, BN = 128;
-    __shared__ __align__(16) T lq[2][QT * DP];
-    __shared__ __align__(16) T lg[2][QT * DP];
+    constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8, QT = 32, BN = 128, TILE = QT * DP;
+    __shared__ __align__(16) T lq[2 * TILE];
+    __shared__ __align__(16) T lg[2 * TILE];
     __shared__ __align__(16) T lv[BN * DP];                 // this workgroup's values, operand B of dP = dO V^T: no registers left for them
     __shared__ __align__(16) float ls[2][QT], ld[2][QT];
-    extern __shared__ float line[];
+    extern __shared__ float line_[];
+    float* line = line_ + MARGIN;
 
-    const int item = xcd_item(blockIdx.x, gridDim.x);           // (tile 0 of a causal head, with most queries, comes first)
     const int heads = a.apart ? a.H : a.Hkv, G = a.apart ? 1 : a.H / a.Hkv;      // of the grid, and of a workgroup
-    const int bh = item / a.tiles, b = bh / heads, h0 = bh % heads * G, hk = h0 / (a.H / a.Hkv), tile = item % a.tiles;
+    int bh, tile;
+    work_item(a, a.B * heads, bh, tile);
+    const int b = bh / heads, h0 = bh % heads * G, hk = h0 / (a.H / a.Hkv);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
     const int start = seq_start(a, b), len = seq_keys(a, b);
     const int j0 = tile * BN, w0 = j0 + wave * 32, key = w0 + col;
@@ -262,57 +278,66 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     // queries that see a key of this workgroup: from i >= j0 - start on if causal, none if the keys do not exist
     const int i_first = a.causal ? max(0, j0 - start) / QT * QT : 0;
     const int nt = j0 < len && i_first < a.Nq ? (a.Nq - i_first + QT - 1) / QT : 0;
-    u32x4_t rq[PER], rg[PER];
-    float rs = 0.f, rd = 0.f;
-    auto fetch = [&](int t) {                               // t counts the query tiles of all heads of the group
-        const int h = h0 + t / nt, i0 = i_first + t % nt * QT;
-        const T* Q = (const T*)a.q + b * a.qs[0] + h * a.qs[2];
-        const T* dO = (const T*)a.dout + b * a.dos[0] + h * a.dos[2];
-        const long long stat = ((long long)b * a.H + h) * a.Nq;
+    Mover<T, DP, QT> mq, mg;
+    constexpr int PER = Mover<T, DP, QT>::PER, STEP = Mover<T, DP, QT>::STEP;
+    float rl[PER], rs = 0.f, rd = 0.f;
+    int fh = h0, fi = i_first;                              // head and first query of the next tile
+    auto fetch = [&]() {
+        const T* Q = (const T*)a.q + b * a.qs[0] + fh * a.qs[2] + fi * a.qs[1];
+        const T* dO = (const T*)a.dout + b * a.dos[0] + fh * a.dos[2] + fi * a.dos[1];
+        const float* lse = a.lse + ((long long)b * a.H + fh) * a.Nq + fi;
+        const float* delta = a.delta + ((long long)b * a.H + fh) * a.Nq + fi;
+        const int left = a.Nq - fi;
+        auto ok = [](int) { return true; };
+        mq.load(Q, a.qs[1], left, a.D, true, ok);
+        mg.load(dO, a.dos[1], left, a.D, true, ok);
 #pragma unroll
         for (int n = 0; n < PER; ++n) {
-            const int idx = n * 256 + threadIdx.x, r = idx / CH, ch = idx % CH, i = i0 + r;
-            const bool ok = r < QT && i < a.Nq && ch * 8 < a.D && a.lse[stat + i] != -INFINITY;
-            rq[n] = load_or_zero<u32x4_t>(ok, Q + (long long)i * a.qs[1] + ch * 8);
-            rg[n] = load_or_zero<u32x4_t>(ok, dO + (long long)i * a.dos[1] + ch * 8);
+            const int r = threadIdx.x / CH + n * STEP;
+            rl[n] = r < left ? lse[r] : -INFINITY;
         }
         if (threadIdx.x < QT) {
-            const int i = i0 + threadIdx.x;
-            const float l = i < a.Nq ? a.lse[stat + i] : -INFINITY;
-            rs = l == -INFINITY ? INFINITY : l - Mma<T>::shift;             // p = 0 for rows that are empty or past the end
-            rd = i < a.Nq ? a.delta[stat + i] * small : 0.f;
+            rs = (int)threadIdx.x < left ? lse[threadIdx.x] : -INFINITY;
+            rd = (int)threadIdx.x < left ? delta[threadIdx.x] : 0.f;
+        }
+        fi += QT;
+        if (fi >= a.Nq) {
+            fi = i_first;
+            ++fh;
         }
     };
     auto store = [&](int buf) {
+        // a row without a key has no gradient, whatever its dout holds: 0 x inf would not vanish in the products
 #pragma unroll
-        for (int n = 0; n < PER; ++n) {
-            const int idx = n * 256 + threadIdx.x, r = idx / CH, ch = idx % CH;
-            if (r >= QT) continue;
-            *reinterpret_cast<u32x4_t*>(&lq[buf][chunk_at<DP>(r, ch) * 8]) = rq[n];
-            *reinterpret_cast<u32x4_t*>(&lg[buf][chunk_at<DP>(r, ch) * 8]) = rg[n];
-        }
+        for (int n = 0; n < PER; ++n)
+            if (rl[n] == -INFINITY) mg.reg[n] = (u32x4_t){0, 0, 0, 0};
+        mq.store(lq + buf * TILE);
+        mg.store(lg + buf * TILE);
         if (threadIdx.x < QT) {
-            ls[buf][threadIdx.x] = rs;
-            ld[buf][threadIdx.x] = rd;
+            ls[buf][threadIdx.x] = rs == -INFINITY ? INFINITY : rs - Mma<T>::shift;         // p = 0 in rows that are empty or past the end
+            ld[buf][threadIdx.x] = rd * small;
         }
     };
     const int total = nt * G;
     if (total > 0) {
-        fetch(0);
+        fetch();
         store(0);
     }
+    int i0 = i_first - QT, h = h0 - 1;
     for (int t = 0; t < total; ++t) {
-        const int buf = t & 1, i0 = i_first + t % nt * QT;
+        const int buf = t & 1;
+        i0 += QT;
         const unsigned va = keep(rows_at), ra = va + buf * (QT * DP * 2), ca = keep(cols_at) + buf * (QT * DP * 2);
-        if (t % nt == 0) {                                   // another head's bias
+        if (t == 0 || i0 >= a.Nq) {                          // another head's bias
+            i0 = i_first;
             __syncthreads();
-            fill_line(line, a, h0 + t / nt, 256);
+            fill_line(line, a, ++h, 256);
             __syncthreads();
         }
-        if (t + 1 < total) fetch(t + 1);
+        if (t + 1 < total) fetch();
         f32x16_t x = zero16();
 #pragma unroll
-        for (int s = 0; s < KS; ++s) x = Mma<T>::mma(Tile<T, DP>::rows(lq[0], ra, 0, s), kf[s], x);
+        for (int s = 0; s < KS; ++s) x = Mma<T>::mma(Tile<T, DP>::rows(lq, ra, 0, s), kf[s], x);
         const int rel_hi = w0 + 31 - i0 - start, rel_lo = w0 - (i0 + QT - 1) - start;
         const bool far = rel_hi <= -reach || rel_lo >= right;
         float sub[16];
@@ -326,12 +351,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = exp2_hw(fmaf(x[r], c, add - sub[r]));
         } else {
-            const int at = key - i0 - 4 * half - start + reach;
+            const float* at = line + (key - i0 - 4 * half - start + reach);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int e = at - 8 * (r / 4) - r % 4;
-                x[r] = exp2_hw(fmaf(x[r], c, line[min(max(e, 0), last)] - sub[r]));
-            }
+            for (int r = 0; r < 16; ++r) x[r] = exp2_hw(fmaf(x[r], c, at[-8 * (r / 4) - r % 4] - sub[r]));
         }
         const int first = a.causal ? key - start - i0 - 4 * half : -1 << 30;     // the first row of the tile that sees the key, less 4 half
         if (!seen || first > -4) {
@@ -344,12 +366,12 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
         for (int s = 0; s < 2; ++s) {
             const v8 p = pack_step<T>(x, s);
 #pragma unroll
-            for (int d = 0; d < DB; ++d) dv[d] = Mma<T>::mma(Tile<T, DP>::cols(lg[0], ca, s * 16, d), p, dv[d]);
+            for (int d = 0; d < DB; ++d) dv[d] = Mma<T>::mma(Tile<T, DP>::cols(lg, ca, s * 16, d), p, dv[d]);
         }
         if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);      // (the next product's operands would not fit beside this one's)
         f32x16_t g = zero16();
 #pragma unroll
-        for (int s = 0; s < KS; ++s) g = Mma<T>::mma(Tile<T, DP>::rows(lg[0], ra, 0, s), Tile<T, DP>::rows(lv + wave * 32 * DP, va, 0, s), g);
+        for (int s = 0; s < KS; ++s) g = Mma<T>::mma(Tile<T, DP>::rows(lg, ra, 0, s), Tile<T, DP>::rows(lv + wave * 32 * DP, va, 0, s), g);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const float4 d4 = *reinterpret_cast<const float4*>(&ld[buf][8 * q + 4 * half]);
@@ -362,7 +384,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
         for (int s = 0; s < 2; ++s) {
             const v8 p = pack_step<T>(x, s);
 #pragma unroll
-            for (int d = 0; d < DB; ++d) dk[d] = Mma<T>::mma(Tile<T, DP>::cols(lq[0], ca, s * 16, d), p, dk[d]);
+            for (int d = 0; d < DB; ++d) dk[d] = Mma<T>::mma(Tile<T, DP>::cols(lq, ca, s * 16, d), p, dk[d]);
         }
         if (t + 1 < total) store(buf ^ 1);
         __syncthreads();
@@ -425,21 +447,20 @@ static bool attn_apart(const tcvom_attn_desc* d) {
 
 template <class T, int DP>
 static int launch_bwd(AttnArgs a, float* dtable, hipStream_t st) {
-    const int last = line_reach(a.bk) + line_right(a.bk);
     if (a.Nq > 0) {
         a.tiles = cdiv(a.Nq, 128);
         const dim3 grid((unsigned)((long long)a.B * a.H * a.tiles));
         if (dtable) {
-            hipLaunchKernelGGL((attn_dq_kernel<T, DP, true>), grid, dim3(256), sizeof(float) * 9 * (last + 1), st, a);
+            hipLaunchKernelGGL((attn_dq_kernel<T, DP, true>), grid, dim3(256), 5 * line_bytes(a), st, a);
             hipLaunchKernelGGL(attn_table_kernel, dim3(a.H), dim3(1024), 0, st, a.part, dtable, a.bk.num_buckets, a.H, (long long)a.B * a.tiles);
         } else {
-            hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), sizeof(float) * (last + 1), st, a);
+            hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), line_bytes(a), st, a);
         }
     }
     if (a.Nk > 0) {
         a.tiles = cdiv(a.Nk, 128);
         const unsigned wgs = (unsigned)((long long)a.B * (a.apart ? a.H : a.Hkv) * a.tiles);
-        hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3(wgs), dim3(256), sizeof(float) * (last + 1), st, a);
+        hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3(wgs), dim3(256), line_bytes(a), st, a);
         if (a.apart) {
             const dim3 grid(cdiv((long long)a.B * a.Nk * a.Hkv * (a.D / 4), 256), 2);
             hipLaunchKernelGGL(attn_heads_kernel<T>, grid, dim3(256), 0, st, a);
@@ -467,7 +488,8 @@ extern "C" int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const voi
                     "attn_bwd: too many rows for one launch");
     TCVOM_CHECK_ARG(work_floats == tcvom_attn_bwd_work(d) && aligned16(work), "attn_bwd: %lld floats of workspace", (long long)work_floats);
     for (int n = 0; n < 3; ++n) {
-        TCVOM_CHECK_ARG(dout_stride[n] % 8 == 0 && dout_stride[n] >= 0, "attn_bwd: strides are multiples of 8 elements");
+        TCVOM_CHECK_ARG(dout_stride[n] % 8 == 0 && dout_stride[n] >= 0 && dout_stride[1] < (1 << 24), "attn_bwd: stride %lld of dout",
+                        (long long)dout_stride[n]);
         a.dos[n] = dout_stride[n];
     }
     a.q = q; a.k = k; a.v = v; a.table = table; a.out = (void*)out; a.out_lo = (void*)out_lo; a.lse = (float*)lse; a.dout = dout;

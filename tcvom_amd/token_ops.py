@@ -161,9 +161,12 @@ def relative_position_bias(table, q_len, k_len, max_distance=128, bidirectional=
 # attention with the bias inside
 # =============================================================================================
 def _rows16(t):
-    """[B, N, heads, width] as the kernels read it: innermost stride 1, the others multiples of 8, 16-byte aligned; a copy if not."""
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s, n in zip(t.stride()[:3], t.shape[:3]) if n > 1)
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    """[B, N, heads, width] as the kernels read it: innermost stride 1, the others multiples of 8, tokens less than 2^24 elements apart,
+    16-byte aligned; a copy if not."""
+    a, b, c, d = t.stride()
+    if d == 1 and (a | b | c) % 8 == 0 and b < 1 << 24 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t):
