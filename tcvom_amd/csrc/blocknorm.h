@@ -3,9 +3,9 @@
 // N = RMSNorm (t r w, r = 1 / sqrt(mean t^2 + eps)) or LayerNorm ((t - m) r w + b).  Bound: HBM bytes -- x, y in and x', h out once
 // forward (x, y, dx', dh in and dx, dy out backward), everything between in registers.
 //
-// One row belongs to TPR threads, each with NV vectors of V channels: 16 lanes at <= 128 channels, a wave up to 1024, 256 threads
-// up to 4096, 512 up to 8192 (V = 8, 16-byte loads); channel counts that are no multiple of 8, and pointers that are not 16-byte
-// aligned, take V = 1.  A workgroup has R such row groups and walks its rows with the weights in registers.
+// One row belongs to TPR threads, each with NV vectors of 8 channels: 16 lanes at <= 128 channels, up to 512 threads at 8192.  A
+// workgroup has R such row groups and walks its rows with the weights in registers.  TAIL: the channels are no multiple of 8; rows
+// then start at any address, which 16-byte accesses allow, and the last vector of a row is moved element by element.
 #pragma once
 #include "token_common.h"
 
@@ -27,14 +27,42 @@ struct NormArgs {
     void* dgate;                         // backward, gate of every token: its gradient, in the gate's type
 };
 
+constexpr int V = 8;                     // channels a vector
+// vector at channel c of a row of C channels at p, zeros past the end
+template <class T, bool TAIL>
+__device__ __forceinline__ typename RawVec<T, V>::type row_load(const T* p, int c, int C) {
+    return !TAIL || c + V <= C ? load_raw<T, V>(p + c) : load_first<T, V>(p + c, C - c);
+}
+template <class T, bool TAIL>
+__device__ __forceinline__ void row_load_f(const T* p, int c, int C, float (&f)[V]) { raw_to_float<T, V>(row_load<T, TAIL>(p, c, C), f); }
+template <class T, bool TAIL>
+__device__ __forceinline__ void row_store(T* p, int c, int C, const float (&f)[V]) {
+    if (!TAIL || c + V <= C) store_vec<T, V>(p + c, f);
+    else store_first<T, V>(p + c, f, C - c);
+}
+
+// sums over 16 lanes and over a wave, in every lane, on the vector unit (a shuffle through LDS takes over 100 cycles a stage, and a row of
+// the backward waits for 12 of them)
+__device__ __forceinline__ float row_sum(float v) {
+    v += H16_DPP(v, 0xB1);                  // lane ^ 1
+    v += H16_DPP(v, 0x4E);                  // lane ^ 2
+    v += H16_DPP(v, 0x124);                 // row_ror:4
+    return v + H16_DPP(v, 0x128);           // row_ror:8
+}
+__device__ __forceinline__ float full_sum(float v) {
+    v = row_sum(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 // sums over the TPR threads of a row group.  TPR > 64: one barrier a call, two LDS slots in turn (the barrier of call n + 1 is after
 // every thread's read of call n, so call n + 2 may reuse its slot).
 template <int TPR, int R, int K>
 __device__ __forceinline__ void group_sum(float (&v)[K], float* lds, int& slot) {
 #pragma unroll
-    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1)
-#pragma unroll
-        for (int k = 0; k < K; ++k) v[k] += __shfl_xor(v[k], o, 64);
+    for (int k = 0; k < K; ++k) v[k] = TPR == 16 ? row_sum(v[k]) : full_sum(v[k]);
     if constexpr (TPR > 64) {
         constexpr int W = TPR / 64;
         float* s = lds + slot * (R * W * 2);
@@ -54,6 +82,7 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float* lds, int& slot) 
     }
 }
 
+// element types and the form of a launch table
 #define NORM_TYPES(TABLE, LAUNCH)                                                                         \
     do {                                                                                                  \
         if (x_type == TCVOM_TYPE_F32 && y_type == TCVOM_TYPE_F32) TABLE(float, float, LAUNCH);            \

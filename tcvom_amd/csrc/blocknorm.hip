@@ -1,7 +1,7 @@
 // Forward of the norms around a block (blocknorm.h), reached through tcvom_block_norm_fwd.
 #include "blocknorm.h"
 
-template <class TX, class TY, int V, int TPR, int R, int NV, bool LAYER>
+template <class TX, class TY, int TPR, int R, int NV, bool TAIL, bool LAYER>
 __global__ __launch_bounds__(TPR * R) void block_norm_fwd_kernel(NormArgs a) {
     __shared__ float lds[TPR > 64 ? 4 * R * (TPR / 64) : 1];
     int slot = 0;
@@ -16,12 +16,12 @@ __global__ __launch_bounds__(TPR * R) void block_norm_fwd_kernel(NormArgs a) {
         const int c = (n * TPR + lane) * V;
         in[n] = c < C;
 #pragma unroll
-        for (int j = 0; j < V; ++j) { w1[n][j] = 1.f; b1[n][j] = 0.f; w2[n][j] = 1.f; b2[n][j] = 0.f; gt[n][j] = 1.f; }
+        for (int j = 0; j < V; ++j) { w1[n][j] = !TAIL || c + j < C ? 1.f : 0.f; b1[n][j] = 0.f; w2[n][j] = 1.f; b2[n][j] = 0.f; gt[n][j] = 1.f; }
         if (!in[n]) continue;
-        if (post) load_vec<float, V>(a.w1 + c, w1[n]);
-        if (LAYER && post && a.b1) load_vec<float, V>(a.b1 + c, b1[n]);
-        if (pre) load_vec<float, V>(a.w2 + c, w2[n]);
-        if (LAYER && pre && a.b2) load_vec<float, V>(a.b2 + c, b2[n]);
+        if (post) row_load_f<float, TAIL>(a.w1, c, C, w1[n]);
+        if (LAYER && post && a.b1) row_load_f<float, TAIL>(a.b1, c, C, b1[n]);
+        if (pre) row_load_f<float, TAIL>(a.w2, c, C, w2[n]);
+        if (LAYER && pre && a.b2) row_load_f<float, TAIL>(a.b2, c, C, b2[n]);
     }
     long long grow = -1;
     const long long r0 = (long long)blockIdx.x * a.rows_per_wg;
@@ -36,8 +36,8 @@ __global__ __launch_bounds__(TPR * R) void block_norm_fwd_kernel(NormArgs a) {
 #pragma unroll
             for (int j = 0; j < V; ++j) x[n][j] = y[n][j] = 0.f;
             if (live && in[n]) {
-                load_vec<TX, V>((const TX*)a.x + base + c, x[n]);
-                if (has_y) load_vec<TY, V>((const TY*)a.y + base + c, y[n]);
+                row_load_f<TX, TAIL>((const TX*)a.x + base, c, C, x[n]);
+                if (has_y) row_load_f<TY, TAIL>((const TY*)a.y + base, c, C, y[n]);
             }
         }
         if (a.gate && live && row / a.gate_rows != grow) {
@@ -46,8 +46,8 @@ __global__ __launch_bounds__(TPR * R) void block_norm_fwd_kernel(NormArgs a) {
             for (int n = 0; n < NV; ++n) {
                 const int c = (n * TPR + lane) * V;
                 if (!in[n]) continue;
-                if (a.gate_f32) load_vec<float, V>((const float*)a.gate + grow * C + c, gt[n]);
-                else load_vec<TY, V>((const TY*)a.gate + grow * C + c, gt[n]);
+                if (a.gate_f32) row_load_f<float, TAIL>((const float*)a.gate + grow * C, c, C, gt[n]);
+                else row_load_f<TY, TAIL>((const TY*)a.gate + grow * C, c, C, gt[n]);
             }
         }
         float m1 = 0.f, r1 = 1.f, m2 = 0.f, r2 = 1.f;
@@ -66,7 +66,10 @@ __global__ __launch_bounds__(TPR * R) void block_norm_fwd_kernel(NormArgs a) {
             for (int n = 0; n < NV; ++n)
                 if (in[n])
 #pragma unroll
-                    for (int j = 0; j < V; ++j) { const float d = t[n][j] - (LAYER ? m : 0.f); s[0] += d * d; }
+                    for (int j = 0; j < V; ++j) {
+                        const float d = t[n][j] - (LAYER ? m : 0.f);
+                        if (!(TAIL && LAYER) || (n * TPR + lane) * V + j < C) s[0] += d * d;
+                    }
             group_sum<TPR, R, 1>(s, lds, slot);
             r = 1.f / sqrtf(s[0] * inv + a.eps);
         };
@@ -77,8 +80,10 @@ __global__ __launch_bounds__(TPR * R) void block_norm_fwd_kernel(NormArgs a) {
                 if (in[n])
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
-                        const float t = post ? (y[n][j] - m1) * r1 * w1[n][j] + b1[n][j] : y[n][j];
-                        x[n][j] = a.rs * x[n][j] + a.bs * gt[n][j] * t;
+                        // (an absent post norm is one of weight 1 on rows of mean 0 and deviation 1)
+                        const float z = (LAYER ? y[n][j] - m1 : y[n][j]) * r1;
+                        const float t = LAYER ? fmaf(z, w1[n][j], b1[n][j]) : z * w1[n][j];
+                        x[n][j] = fmaf(a.bs * gt[n][j], t, a.rs * x[n][j]);
                     }
         }
         if (pre) moments(x, m2, r2);
@@ -87,33 +92,30 @@ __global__ __launch_bounds__(TPR * R) void block_norm_fwd_kernel(NormArgs a) {
         for (int n = 0; n < NV; ++n) {
             const int c = (n * TPR + lane) * V;
             if (!in[n]) continue;
-            if (has_y) store_vec<TX, V>((TX*)a.xo + base + c, x[n]);
+            if (has_y) row_store<TX, TAIL>((TX*)a.xo + base, c, C, x[n]);
             if (pre) {
                 float h[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) h[j] = (x[n][j] - m2) * r2 * w2[n][j] + b2[n][j];
-                store_vec<TY, V>((TY*)a.h + base + c, h);
+                for (int j = 0; j < V; ++j) {
+                    const float z = (LAYER ? x[n][j] - m2 : x[n][j]) * r2;
+                    h[j] = LAYER ? fmaf(z, w2[n][j], b2[n][j]) : z * w2[n][j];
+                }
+                row_store<TY, TAIL>((TY*)a.h + base, c, C, h);
             }
         }
         if (a.stats && lane == 0) *reinterpret_cast<float4*>(a.stats + row * 4) = make_float4(m1, r1, m2, r2);
     }
 }
 
-// vector width by alignment, threads by channels (see blocknorm.h)
-#define FWD_TABLE(TX, TY, LAUNCH)                                      \
-    do {                                                               \
-        if (vec) {                                                     \
-            if (C <= 128) LAUNCH(TX, TY, 8, 16, 16, 1);                \
-            else if (C <= 512) LAUNCH(TX, TY, 8, 64, 4, 1);            \
-            else if (C <= 1024) LAUNCH(TX, TY, 8, 64, 4, 2);           \
-            else if (C <= 2048) LAUNCH(TX, TY, 8, 256, 1, 1);          \
-            else if (C <= 4096) LAUNCH(TX, TY, 8, 256, 1, 2);          \
-            else LAUNCH(TX, TY, 8, 512, 1, 2);                         \
-        } else {                                                       \
-            if (C <= 512) LAUNCH(TX, TY, 1, 64, 4, 8);                 \
-            else if (C <= 4096) LAUNCH(TX, TY, 1, 256, 1, 16);         \
-            else LAUNCH(TX, TY, 1, 512, 1, 16);                        \
-        }                                                              \
+// threads by channels (see blocknorm.h)
+#define FWD_TABLE(TX, TY, LAUNCH)                      \
+    do {                                               \
+        if (C <= 128) LAUNCH(TX, TY, 16, 16, 1);       \
+        else if (C <= 512) LAUNCH(TX, TY, 64, 4, 1);   \
+        else if (C <= 1024) LAUNCH(TX, TY, 64, 4, 2);  \
+        else if (C <= 2048) LAUNCH(TX, TY, 256, 1, 1); \
+        else if (C <= 4096) LAUNCH(TX, TY, 256, 1, 2); \
+        else LAUNCH(TX, TY, 512, 1, 2);                \
     } while (0)
 
 extern "C" int tcvom_block_norm_fwd(const void* x, const void* y, const float* post_weight, const float* post_bias, const void* gate,
@@ -134,19 +136,23 @@ extern "C" int tcvom_block_norm_fwd(const void* x, const void* y, const float* p
     a.gate = gate; a.gate_f32 = gate_f32; a.gate_rows = gate_rows > 0 ? gate_rows : 1;
     a.bs = branch_scale; a.rs = residual_scale; a.eps = eps; a.T = T; a.C = C;
     a.xo = x_out; a.h = h; a.stats = stats;
-    const bool vec = C % 8 == 0 && aligned16(x) && aligned16(y) && aligned16(post_weight) && aligned16(post_bias) && aligned16(gate) &&
-                     aligned16(pre_weight) && aligned16(pre_bias) && aligned16(x_out) && aligned16(h);
     const hipStream_t st = (hipStream_t)stream;
-#define FWD(TX, TY, V, TPR, R, NV)                                                                                      \
-    do {                                                                                                                \
-        const int wgs = 256 * (2048 / (TPR * R));                                                                       \
-        a.rows_per_wg = cdiv(cdiv(T, R), wgs) * R;                                                                      \
-        const dim3 grid(cdiv(T, a.rows_per_wg));                                                                        \
-        if (layer) hipLaunchKernelGGL((block_norm_fwd_kernel<TX, TY, V, TPR, R, NV, true>), grid, dim3(TPR * R), 0, st, a);  \
-        else hipLaunchKernelGGL((block_norm_fwd_kernel<TX, TY, V, TPR, R, NV, false>), grid, dim3(TPR * R), 0, st, a);       \
+#define FWD_LAUNCH(TX, TY, TPR, R, NV, TAIL)                                                                                   \
+    do {                                                                                                                      \
+        if (layer) hipLaunchKernelGGL((block_norm_fwd_kernel<TX, TY, TPR, R, NV, TAIL, true>), grid, dim3(TPR * R), 0, st, a);  \
+        else hipLaunchKernelGGL((block_norm_fwd_kernel<TX, TY, TPR, R, NV, TAIL, false>), grid, dim3(TPR * R), 0, st, a);       \
+    } while (0)
+#define FWD(TX, TY, TPR, R, NV)                                           \
+    do {                                                                  \
+        const int wgs = 256 * (2048 / (TPR * R));                         \
+        a.rows_per_wg = cdiv(cdiv(T, R), wgs) * R;                        \
+        const dim3 grid(cdiv(T, a.rows_per_wg));                          \
+        if (C % V) FWD_LAUNCH(TX, TY, TPR, R, NV, true);                  \
+        else FWD_LAUNCH(TX, TY, TPR, R, NV, false);                       \
     } while (0)
     NORM_TYPES(FWD_TABLE, FWD);
 #undef FWD
+#undef FWD_LAUNCH
     TCVOM_LAUNCH_CHECK("block_norm_fwd");
     return 0;
 }

@@ -10,8 +10,8 @@
 
 enum { SUM_W1 = 0, SUM_B1, SUM_W2, SUM_B2, SUM_G, SUMS };
 
-template <class TX, class TY, int V, int TPR, int R, int NV, bool LAYER>
-__global__ __launch_bounds__(TPR * R) void block_norm_bwd_kernel(NormArgs a) {
+template <class TX, class TY, int TPR, int R, int NV, bool TAIL, bool LAYER>
+__global__ __launch_bounds__(TPR * R, 2) void block_norm_bwd_kernel(NormArgs a) {
     constexpr int RED = TPR > 64 ? 4 * R * (TPR / 64) : 1;
     constexpr int COLS = R > 1 ? TPR * R * V : 1;
     __shared__ float lds[RED];
@@ -31,21 +31,23 @@ __global__ __launch_bounds__(TPR * R) void block_norm_bwd_kernel(NormArgs a) {
         in[n] = c < C;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            w1[n][j] = 1.f; b1[n][j] = 0.f; w2[n][j] = 1.f; gt[n][j] = 1.f;
+            w1[n][j] = !TAIL || c + j < C ? 1.f : 0.f; b1[n][j] = 0.f; w2[n][j] = 1.f; gt[n][j] = a.bs;
             s_w1[n][j] = s_b1[n][j] = s_w2[n][j] = s_b2[n][j] = s_g[n][j] = 0.f;
         }
         if (!in[n]) continue;
-        if (post) load_vec<float, V>(a.w1 + c, w1[n]);
-        if (LAYER && post && a.b1) load_vec<float, V>(a.b1 + c, b1[n]);
-        if (pre) load_vec<float, V>(a.w2 + c, w2[n]);
+        if (post) row_load_f<float, TAIL>(a.w1, c, C, w1[n]);
+        if (LAYER && post && a.b1) row_load_f<float, TAIL>(a.b1, c, C, b1[n]);
+        if (pre) row_load_f<float, TAIL>(a.w2, c, C, w2[n]);
     }
     auto load_gate = [&](long long grow) {
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             const int c = (n * TPR + lane) * V;
             if (!in[n]) continue;
-            if (a.gate_f32) load_vec<float, V>((const float*)a.gate + grow * C + c, gt[n]);
-            else load_vec<TY, V>((const TY*)a.gate + grow * C + c, gt[n]);
+            if (a.gate_f32) row_load_f<float, TAIL>((const float*)a.gate + grow * C, c, C, gt[n]);
+            else row_load_f<TY, TAIL>((const TY*)a.gate + grow * C, c, C, gt[n]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) gt[n][j] *= a.bs;
         }
     };
     // blockIdx.y = gate row (its tokens' sums stay apart), blockIdx.x = workgroup among its tokens
@@ -53,77 +55,83 @@ __global__ __launch_bounds__(TPR * R) void block_norm_bwd_kernel(NormArgs a) {
     const long long first = (long long)blockIdx.y * group_rows + (long long)blockIdx.x * a.rows_per_wg;
     const long long end = (long long)(blockIdx.y + 1) * group_rows;
     if (a.gate && !token_gate) load_gate(blockIdx.y);
-    // the next row's loads are in flight while this one's sums wait at their barriers
-    typename RawVec<TX, V>::type rx[NV], rdx[NV];
-    typename RawVec<TY, V>::type ry[NV], rdh[NV];
-    float4 rst;
-    auto fetch = [&](int k) {
+    // the next DEPTH rows' loads are in flight while this one's sums wait at their barriers
+    constexpr int DEPTH = NV == 1 ? 2 : 1;
+    struct Raw {
+        typename RawVec<TX, V>::type x[NV], dx[NV];
+        typename RawVec<TY, V>::type y[NV], dh[NV];
+        float4 st;
+    } raw[DEPTH];
+    auto fetch = [&](int k, Raw& r) {
         const long long row = first + k + g;
         const bool live = k + g < a.rows_per_wg && row < end;
         const long long base = row * C;
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             const int c = (n * TPR + lane) * V;
-            rx[n] = (typename RawVec<TX, V>::type)(TX)0.f;
-            rdx[n] = rx[n];
-            ry[n] = (typename RawVec<TY, V>::type)(TY)0.f;
-            rdh[n] = ry[n];
+            r.x[n] = (typename RawVec<TX, V>::type)(TX)0.f;
+            r.dx[n] = r.x[n];
+            r.y[n] = (typename RawVec<TY, V>::type)(TY)0.f;
+            r.dh[n] = r.y[n];
             if (live && in[n]) {
-                if (pre) rx[n] = load_raw<TX, V>((const TX*)a.x + base + c);
-                if (has_y) ry[n] = load_raw<TY, V>((const TY*)a.y + base + c);
-                if (a.dxo) rdx[n] = load_raw<TX, V>((const TX*)a.dxo + base + c);
-                if (pre) rdh[n] = load_raw<TY, V>((const TY*)a.dh + base + c);
+                if (pre) r.x[n] = row_load<TX, TAIL>((const TX*)a.x + base, c, C);
+                if (has_y) r.y[n] = row_load<TY, TAIL>((const TY*)a.y + base, c, C);
+                if (a.dxo) r.dx[n] = row_load<TX, TAIL>((const TX*)a.dxo + base, c, C);
+                if (pre) r.dh[n] = row_load<TY, TAIL>((const TY*)a.dh + base, c, C);
             }
         }
-        rst = make_float4(0.f, 1.f, 0.f, 1.f);
-        if (live) rst = *reinterpret_cast<const float4*>(a.stats + row * 4);
+        r.st = make_float4(0.f, 1.f, 0.f, 1.f);
+        if (live) r.st = *reinterpret_cast<const float4*>(a.stats + row * 4);
     };
-    fetch(0);
-    for (int k = 0; k < a.rows_per_wg; k += R) {
+    auto step = [&](int k, Raw& r) {
         const long long row = first + k + g;
         const bool live = k + g < a.rows_per_wg && row < end;
         const long long base = row * C;
         float x[NV][V], y[NV][V], dX[NV][V], dh[NV][V];
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
-            raw_to_float<TX, V>(rx[n], x[n]);
-            raw_to_float<TY, V>(ry[n], y[n]);
-            raw_to_float<TX, V>(rdx[n], dX[n]);
-            raw_to_float<TY, V>(rdh[n], dh[n]);
+            raw_to_float<TX, V>(r.x[n], x[n]);
+            raw_to_float<TY, V>(r.y[n], y[n]);
+            raw_to_float<TX, V>(r.dx[n], dX[n]);
+            raw_to_float<TY, V>(r.dh[n], dh[n]);
         }
-        const float4 st = rst;
-        if (k + R < a.rows_per_wg) fetch(k + R);
+        const float4 st = r.st;
+        if (k + DEPTH * R < a.rows_per_wg) fetch(k + DEPTH * R, r);
         if (token_gate && live) load_gate(row);
         const float m1 = st.x, r1 = st.y, m2 = st.z, r2 = st.w;
-        // y <- yhat, x <- xhat of x'
+        // y <- yhat, x <- xhat of x'.  (An absent post norm is one of weight 1 on rows of mean 0 and deviation 1, an absent y is zero.)
 #pragma unroll
         for (int n = 0; n < NV; ++n)
             if (in[n])
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    if (post) y[n][j] = (y[n][j] - m1) * r1;
-                    const float t = post ? y[n][j] * w1[n][j] + b1[n][j] : y[n][j];
-                    const float x1 = has_y ? a.rs * x[n][j] + a.bs * gt[n][j] * t : x[n][j];
-                    x[n][j] = (x1 - m2) * r2;
+                    y[n][j] = (LAYER ? y[n][j] - m1 : y[n][j]) * r1;
+                    const float t = LAYER ? fmaf(y[n][j], w1[n][j], b1[n][j]) : y[n][j] * w1[n][j];
+                    const float x1 = fmaf(gt[n][j], t, a.rs * x[n][j]);
+                    x[n][j] = (LAYER ? x1 - m2 : x1) * r2;
                 }
+        constexpr int K = LAYER ? 2 : 1;
         if (pre) {
-            float s[2] = {0.f, 0.f};
+            float s[K] = {};
 #pragma unroll
             for (int n = 0; n < NV; ++n)
                 if (in[n])
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
-                        if (live) { s_w2[n][j] += dh[n][j] * x[n][j]; s_b2[n][j] += dh[n][j]; }
+                        // (rows past the end hold zeros: they add nothing)
+                        s_w2[n][j] = fmaf(dh[n][j], x[n][j], s_w2[n][j]);
+                        if (LAYER) s_b2[n][j] += dh[n][j];
                         dh[n][j] *= w2[n][j];
-                        s[0] += dh[n][j] * x[n][j];
-                        s[1] += dh[n][j];
+                        s[0] = fmaf(dh[n][j], x[n][j], s[0]);
+                        if (LAYER) s[K - 1] += dh[n][j];
                     }
-            group_sum<TPR, R, 2>(s, lds, slot);
-            const float p = s[0] * inv, q = LAYER ? s[1] * inv : 0.f;
+            group_sum<TPR, R, K>(s, lds, slot);
+            const float p = s[0] * inv * r2, q = LAYER ? s[K - 1] * inv : 0.f;
 #pragma unroll
             for (int n = 0; n < NV; ++n)
 #pragma unroll
-                for (int j = 0; j < V; ++j) dX[n][j] += r2 * (dh[n][j] - q - x[n][j] * p);
+                for (int j = 0; j < V; ++j)
+                    dX[n][j] = fmaf(r2, LAYER ? dh[n][j] - q : dh[n][j], fmaf(-p, x[n][j], dX[n][j]));
         }
         if (live)
 #pragma unroll
@@ -132,45 +140,57 @@ __global__ __launch_bounds__(TPR * R) void block_norm_bwd_kernel(NormArgs a) {
                 if (!in[n]) continue;
                 float o[V];
 #pragma unroll
-                for (int j = 0; j < V; ++j) o[j] = has_y ? a.rs * dX[n][j] : dX[n][j];
-                store_vec<TX, V>((TX*)a.dx + base + c, o);
+                for (int j = 0; j < V; ++j) o[j] = a.rs * dX[n][j];
+                row_store<TX, TAIL>((TX*)a.dx + base, c, C, o);
             }
-        if (!has_y) continue;
-        float s[2] = {0.f, 0.f};
+        if (!has_y) return;
+        float s[K] = {};
         float dg[NV][V];
 #pragma unroll
         for (int n = 0; n < NV; ++n)
             if (in[n])
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float t = post ? y[n][j] * w1[n][j] + b1[n][j] : y[n][j];
-                    dg[n][j] = a.bs * t * dX[n][j];
-                    const float dn = a.bs * gt[n][j] * dX[n][j];
-                    if (live) { s_g[n][j] += dg[n][j]; s_w1[n][j] += dn * y[n][j]; s_b1[n][j] += dn; }
+                    const float t = LAYER ? fmaf(y[n][j], w1[n][j], b1[n][j]) : y[n][j] * w1[n][j];
+                    dg[n][j] = t * dX[n][j];
+                    const float dn = live ? gt[n][j] * dX[n][j] : 0.f;
+                    s_g[n][j] += live ? dg[n][j] : 0.f;
+                    s_w1[n][j] = fmaf(dn, y[n][j], s_w1[n][j]);
+                    if (LAYER) s_b1[n][j] += dn;
                     dX[n][j] = dn * w1[n][j];
-                    s[0] += dX[n][j] * y[n][j];
-                    s[1] += dX[n][j];
+                    s[0] = fmaf(dX[n][j], y[n][j], s[0]);
+                    if (LAYER) s[K - 1] += dX[n][j];
                 }
         float p = 0.f, q = 0.f;
         if (post) {
-            group_sum<TPR, R, 2>(s, lds, slot);
-            p = s[0] * inv;
-            q = LAYER ? s[1] * inv : 0.f;
+            group_sum<TPR, R, K>(s, lds, slot);
+            p = s[0] * inv * r1;
+            q = LAYER ? s[K - 1] * inv : 0.f;
         }
-        if (!live) continue;
+        if (!live) return;
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             const int c = (n * TPR + lane) * V;
             if (!in[n]) continue;
             float o[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) o[j] = post ? r1 * (dX[n][j] - q - y[n][j] * p) : dX[n][j];
-            store_vec<TY, V>((TY*)a.dy + base + c, o);
+            for (int j = 0; j < V; ++j) o[j] = fmaf(r1, LAYER ? dX[n][j] - q : dX[n][j], -p * y[n][j]);
+            row_store<TY, TAIL>((TY*)a.dy + base, c, C, o);
             if (token_gate && a.dgate) {
-                if (a.gate_f32) store_vec<float, V>((float*)a.dgate + base + c, dg[n]);
-                else store_vec<TY, V>((TY*)a.dgate + base + c, dg[n]);
+#pragma unroll
+                for (int j = 0; j < V; ++j) dg[n][j] *= a.bs;
+                if (a.gate_f32) row_store<float, TAIL>((float*)a.dgate + base, c, C, dg[n]);
+                else row_store<TY, TAIL>((TY*)a.dgate + base, c, C, dg[n]);
             }
         }
+    };
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i)
+        if (i * R < a.rows_per_wg) fetch(i * R, raw[i]);
+    for (int k = 0; k < a.rows_per_wg; k += DEPTH * R) {
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i)
+            if (k + i * R < a.rows_per_wg) step(k + i * R, raw[i]);
     }
     float* part = a.part + ((long long)blockIdx.y * gridDim.x + blockIdx.x) * SUMS * C;
     auto flush = [&](int q, float (&t)[NV][V]) {
@@ -188,7 +208,7 @@ __global__ __launch_bounds__(TPR * R) void block_norm_bwd_kernel(NormArgs a) {
 #pragma unroll
                         for (int j = 0; j < V; ++j) t[n][j] += cols[(i * TPR + lane) * V + j];
             }
-            if (g == 0 && in[n]) store_vec<float, V>(part + (long long)q * C + c, t[n]);
+            if (g == 0 && in[n]) row_store<float, TAIL>(part + (long long)q * C, c, C, t[n]);
         }
     };
     flush(SUM_W1, s_w1);
@@ -197,6 +217,10 @@ __global__ __launch_bounds__(TPR * R) void block_norm_bwd_kernel(NormArgs a) {
         flush(SUM_B1, s_b1);
         flush(SUM_B2, s_b2);
     }
+#pragma unroll
+    for (int n = 0; n < NV; ++n)
+#pragma unroll
+        for (int j = 0; j < V; ++j) s_g[n][j] *= a.bs;
     flush(SUM_G, s_g);
 }
 
@@ -225,47 +249,26 @@ __global__ __launch_bounds__(1024) void block_norm_sums_kernel(const float* part
     else ((float*)s.dgate)[at] = t;
 }
 
-// workgroups of a launch: at most this many partial rows in all (two workgroups a CU), at least one a gate row
-static int bwd_wgs(int64_t T, int64_t groups, int R, int threads) {
-    const int64_t rows = T / groups;
-    const int64_t want = (int64_t)256 * (threads > 256 ? 1 : 2);
-    int64_t n = (want + groups - 1) / groups;
-    const int64_t most = (rows + R - 1) / R;
-    return (int)(n < 1 ? 1 : n > most ? most : n);
+static int bwd_groups(int C) { return C <= 128 ? 16 : C <= 512 ? 4 : C <= 1024 ? 2 : 1; }       // row groups of a workgroup (BWD_TABLE's R)
+// workgroups a gate row (or in all): as many as fit the chip at once -- two of 256 threads a CU, one of 512 -- no more than there are rows for
+static int bwd_wgs(int64_t T, int64_t groups, int C) {
+    const int64_t n = ((C > 2048 ? 256 : 512) + groups - 1) / groups, most = (T / groups + bwd_groups(C) - 1) / bwd_groups(C);
+    return (int)(n > most ? most : n);
 }
-static void bwd_shape(int C, bool vec, int* R, int* threads) {
-    *R = vec ? (C <= 128 ? 16 : C <= 512 ? 4 : C <= 1024 ? 2 : 1) : (C <= 512 ? 4 : 1);
-    *threads = vec ? (C <= 2048 ? 256 : 512) : (C <= 4096 ? 256 : 512);
-}
-// vector width by alignment, threads by channels: 8 channels a thread while the sums of 5 columns each leave room for them (bwd_shape
-// says the same)
-#define BWD_TABLE(TX, TY, LAUNCH)                                      \
-    do {                                                               \
-        if (vec) {                                                     \
-            if (C <= 128) LAUNCH(TX, TY, 8, 16, 16, 1);                \
-            else if (C <= 512) LAUNCH(TX, TY, 8, 64, 4, 1);            \
-            else if (C <= 1024) LAUNCH(TX, TY, 8, 128, 2, 1);          \
-            else if (C <= 2048) LAUNCH(TX, TY, 8, 256, 1, 1);          \
-            else if (C <= 4096) LAUNCH(TX, TY, 8, 512, 1, 1);          \
-            else LAUNCH(TX, TY, 8, 512, 1, 2);                         \
-        } else {                                                       \
-            if (C <= 512) LAUNCH(TX, TY, 1, 64, 4, 8);                 \
-            else if (C <= 4096) LAUNCH(TX, TY, 1, 256, 1, 16);         \
-            else LAUNCH(TX, TY, 1, 512, 1, 16);                        \
-        }                                                              \
+// threads by channels: 8 channels a thread while the sums of 5 columns each leave room for them
+#define BWD_TABLE(TX, TY, LAUNCH)                      \
+    do {                                               \
+        if (C <= 128) LAUNCH(TX, TY, 16, 16, 1);       \
+        else if (C <= 512) LAUNCH(TX, TY, 64, 4, 1);   \
+        else if (C <= 1024) LAUNCH(TX, TY, 128, 2, 1); \
+        else if (C <= 2048) LAUNCH(TX, TY, 256, 1, 1); \
+        else if (C <= 4096) LAUNCH(TX, TY, 512, 1, 1); \
+        else LAUNCH(TX, TY, 512, 1, 2);                \
     } while (0)
 
 extern "C" int64_t tcvom_block_norm_bwd_work(int64_t T, int32_t C, int64_t gate_groups) {
     if (T <= 0 || C <= 0 || gate_groups <= 0) return 0;
-    // the larger of the aligned and the unaligned form: the caller need not know which one runs
-    int64_t most = 0;
-    for (int v = 0; v < 2; ++v) {
-        int R, threads;
-        bwd_shape(C, v, &R, &threads);
-        const int64_t n = (int64_t)bwd_wgs(T, gate_groups, R, threads) * gate_groups;
-        most = n > most ? n : most;
-    }
-    return most * SUMS * C;
+    return (int64_t)bwd_wgs(T, gate_groups, C) * gate_groups * SUMS * C;
 }
 
 extern "C" int tcvom_block_norm_bwd(const void* x, const void* y, const float* post_weight, const float* post_bias, const void* gate,
@@ -292,30 +295,31 @@ extern "C" int tcvom_block_norm_bwd(const void* x, const void* y, const float* p
     NormArgs a = {};
     a.x = x; a.y = y; a.w1 = post_weight; a.b1 = post_bias; a.w2 = pre_weight;
     a.gate = gate; a.gate_f32 = gate_f32; a.gate_rows = gate ? (token_gate ? 1 : gate_rows) : 1;
-    a.bs = branch_scale; a.rs = residual_scale; a.T = T; a.C = C;
+    a.bs = y ? branch_scale : 0.f; a.rs = y ? residual_scale : 1.f; a.T = T; a.C = C;
     a.stats = (float*)stats; a.dxo = dx_out; a.dh = dh; a.dx = dx; a.dy = dy; a.part = work;
     a.dgate = token_gate ? dgate : nullptr;
     a.want = (dpost_weight ? 1 << SUM_W1 : 0) | (dpost_bias ? 1 << SUM_B1 : 0) | (dpre_weight ? 1 << SUM_W2 : 0) |
              (dpre_bias ? 1 << SUM_B2 : 0) | (dgate && !token_gate ? 1 << SUM_G : 0);
-    const bool vec = C % 8 == 0 && aligned16(x) && aligned16(y) && aligned16(post_weight) && aligned16(post_bias) && aligned16(gate) &&
-                     aligned16(pre_weight) && aligned16(dx_out) && aligned16(dh) && aligned16(dx) && aligned16(dy) && aligned16(a.dgate) &&
-                     aligned16(work);
-    int R0, threads0;
-    bwd_shape(C, vec, &R0, &threads0);
-    const int wgs = bwd_wgs(T, groups, R0, threads0);
+    const int R0 = bwd_groups(C), wgs = bwd_wgs(T, groups, C);
     const int64_t rows = T / groups;
     const hipStream_t st = (hipStream_t)stream;
     const int per = cdiv(cdiv(rows, wgs), R0) * R0;
     const int used = cdiv(rows, per);                        // <= wgs: rounding up to whole row groups can leave some without rows
     a.rows_per_wg = per;
-#define BWD(TX, TY, V, TPR, R, NV)                                                                                      \
-    do {                                                                                                                \
-        const dim3 grid(used, (unsigned)groups);                                                                        \
-        if (layer) hipLaunchKernelGGL((block_norm_bwd_kernel<TX, TY, V, TPR, R, NV, true>), grid, dim3(TPR * R), 0, st, a);  \
-        else hipLaunchKernelGGL((block_norm_bwd_kernel<TX, TY, V, TPR, R, NV, false>), grid, dim3(TPR * R), 0, st, a);       \
+    const dim3 grid(used, (unsigned)groups);
+#define BWD_LAUNCH(TX, TY, TPR, R, NV, TAIL)                                                                                   \
+    do {                                                                                                                      \
+        if (layer) hipLaunchKernelGGL((block_norm_bwd_kernel<TX, TY, TPR, R, NV, TAIL, true>), grid, dim3(TPR * R), 0, st, a);  \
+        else hipLaunchKernelGGL((block_norm_bwd_kernel<TX, TY, TPR, R, NV, TAIL, false>), grid, dim3(TPR * R), 0, st, a);       \
+    } while (0)
+#define BWD(TX, TY, TPR, R, NV)                                 \
+    do {                                                        \
+        if (C % V) BWD_LAUNCH(TX, TY, TPR, R, NV, true);        \
+        else BWD_LAUNCH(TX, TY, TPR, R, NV, false);             \
     } while (0)
     NORM_TYPES(BWD_TABLE, BWD);
 #undef BWD
+#undef BWD_LAUNCH
     TCVOM_LAUNCH_CHECK("block_norm_bwd");
     if (!a.want) return 0;
     NormSums s = {};

@@ -11,56 +11,44 @@ template <> struct Elem<float> { static constexpr int kind = TCVOM_TYPE_F32; };
 template <> struct Elem<__bf16> { static constexpr int kind = TCVOM_TYPE_BF16; };
 template <> struct Elem<_Float16> { static constexpr int kind = TCVOM_TYPE_F16; };
 
-// V consecutive elements at p as floats / from floats.  V > 1: p is 16-byte aligned for V = 8 (32 bytes of fp32 as two loads).
+// V consecutive elements at p as floats / from floats.  The types carry the alignment of one element: rows of an odd length start anywhere,
+// and global memory takes 16-byte accesses at any address.
+template <class T, int V> struct RawVec {
+    typedef T type __attribute__((ext_vector_type(V)));
+    typedef type any __attribute__((aligned(sizeof(T))));
+};
 template <class T, int V>
-__device__ __forceinline__ void load_vec(const T* p, float (&f)[V]) {
-    if constexpr (V == 1) {
-        f[0] = (float)p[0];
-    } else if constexpr (sizeof(T) == 4) {
-        typedef __attribute__((ext_vector_type(4))) float f4_t;
-#pragma unroll
-        for (int i = 0; i < V; i += 4) {
-            const f4_t q = *reinterpret_cast<const f4_t*>(p + i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) f[i + j] = q[j];
-        }
-    } else {
-        typedef __attribute__((ext_vector_type(V))) T v_t;
-        const v_t q = *reinterpret_cast<const v_t*>(p);
-#pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = (float)q[j];
-    }
+__device__ __forceinline__ typename RawVec<T, V>::type load_raw(const T* p) {
+    return *reinterpret_cast<const typename RawVec<T, V>::any*>(p);
 }
-// the same in two steps, for loads that are issued ahead of their use
-template <class T, int V> struct RawVec { typedef T type __attribute__((ext_vector_type(V))); };
-template <class T> struct RawVec<T, 1> { typedef T type; };
-template <class T, int V>
-__device__ __forceinline__ typename RawVec<T, V>::type load_raw(const T* p) { return *reinterpret_cast<const typename RawVec<T, V>::type*>(p); }
 template <class T, int V>
 __device__ __forceinline__ void raw_to_float(const typename RawVec<T, V>::type& q, float (&f)[V]) {
-    if constexpr (V == 1) f[0] = (float)q;
-    else
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = (float)q[j];
+    for (int j = 0; j < V; ++j) f[j] = (float)q[j];
 }
 template <class T, int V>
+__device__ __forceinline__ void load_vec(const T* p, float (&f)[V]) { raw_to_float<T, V>(load_raw<T, V>(p), f); }
+template <class T, int V>
 __device__ __forceinline__ void store_vec(T* p, const float (&f)[V]) {
-    if constexpr (V == 1) {
-        p[0] = (T)f[0];
-    } else if constexpr (sizeof(T) == 4) {
-        typedef __attribute__((ext_vector_type(4))) float f4_t;
+    typename RawVec<T, V>::type q;
 #pragma unroll
-        for (int i = 0; i < V; i += 4) {
-            const f4_t q = {f[i], f[i + 1], f[i + 2], f[i + 3]};
-            *reinterpret_cast<f4_t*>(p + i) = q;
-        }
-    } else {
-        typedef __attribute__((ext_vector_type(V))) T v_t;
-        v_t q;
+    for (int j = 0; j < V; ++j) q[j] = (T)f[j];
+    *reinterpret_cast<typename RawVec<T, V>::any*>(p) = q;
+}
+// the first n of them (n <= V), the others zero / left alone
+template <class T, int V>
+__device__ __forceinline__ typename RawVec<T, V>::type load_first(const T* p, int n) {
+    typename RawVec<T, V>::type q = (typename RawVec<T, V>::type)(T)0.f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) q[j] = (T)f[j];
-        *reinterpret_cast<v_t*>(p) = q;
-    }
+    for (int j = 0; j < V; ++j)
+        if (j < n) q[j] = p[j];
+    return q;
+}
+template <class T, int V>
+__device__ __forceinline__ void store_first(T* p, const float (&f)[V], int n) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (j < n) p[j] = (T)f[j];
 }
 
 // ---- buckets of relative positions (tcvom_rel_buckets, include/tcvom_hip.h)
