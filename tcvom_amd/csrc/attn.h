@@ -194,6 +194,17 @@ template <class T, int DP, int ROWS> struct Mover {
 };
 // NaN stays NaN; v_maximum3_f32
 __device__ __forceinline__ float max2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float max3(float a, float b, float c) { return max2(max2(a, b), c); }
+__device__ __forceinline__ float max16(const f32x16_t& x) {
+    return max3(max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[8])),
+                max3(max3(x[9], x[10], x[11]), x[12], x[13]), max2(x[14], x[15]));
+}
+// x where the bit of `see` is set, else `other`; register r of a block stands for bit 8 (r / 4) + r % 4
+__device__ __forceinline__ float pick(unsigned see, int r, float x, float other) {
+    const unsigned m = (unsigned)__builtin_amdgcn_sbfe((int)see, 8 * (r / 4) + r % 4, 1);
+    return __uint_as_float((__float_as_uint(x) & m) | (__float_as_uint(other) & ~m));
+}
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }      // (a scalar: branches on it are uniform)
 __device__ __forceinline__ f32x16_t zero16() {
     f32x16_t z;
 #pragma unroll

@@ -1,17 +1,16 @@
 // Forward of the attention with a relative position bias (attn.h), reached through tcvom_attn_fwd.
 #include "attn.h"
-#include <type_traits>
 
 // a row without a key is zero; a sum that is NaN makes the row NaN
 __device__ __forceinline__ float empty_or(float sum, float v) { return sum == 0.f ? 0.f : v; }
 
-// ---- many queries: a workgroup of 4 waves takes 128 QB queries of one head, a wave 32 QB of them, all through the same tiles of 64 keys.
+// ---- many queries: a workgroup of 4 waves takes 128 queries of one head, a wave 32 of them, all through the same tiles of 64 keys.
 // K and V tiles go to LDS through registers (the next tile's loads are in flight during this tile's products), two buffers, one
 // barrier a tile.
-template <class T, int DP, int QB, bool LO>
+template <class T, int DP, bool LO>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;
-    constexpr int KS = DP / 16, DB = DP / 32, BM = 128 * QB, TILE = KT * DP;
+    constexpr int KS = DP / 16, DB = DP / 32, BM = 128, TILE = KT * DP;
     __shared__ __align__(16) T lk[2 * TILE];
     __shared__ __align__(16) T lv[2 * TILE];
     extern __shared__ float line_[];
@@ -21,7 +20,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
     work_item(a, a.B * a.H, bh, tile);
     if (a.causal) tile = a.tiles - 1 - tile;
     const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+    const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5, col = lane & 31;
     const int i0 = tile * BM, start = seq_start(a, b), len = seq_keys(a, b);
     // keys any query of the workgroup sees
     const int i_last = min(i0 + BM, a.Nq) - 1;
@@ -35,17 +34,13 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
     const T* V = (const T*)a.v + b * a.vs[0] + hk * a.vs[2];
     const unsigned char* mask = a.key_mask ? a.key_mask + (long long)b * a.Nk : nullptr;
 
-    const int w0 = i0 + wave * (32 * QB);                  // the wave's first query
-    int qi[QB];
-    v8 qf[QB][KS];
+    const int w0 = i0 + wave * 32, qi = w0 + col;          // the wave's first query, the lane's
+    const int first_limit = min(len, a.causal ? w0 + start + 1 : len), my_limit = min(len, a.causal ? qi + start + 1 : len);
+    v8 qf[KS];
 #pragma unroll
-    for (int u = 0; u < QB; ++u) {
-        qi[u] = w0 + u * 32 + col;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const int d = s * 16 + half * 8;
-            qf[u][s] = load_or_zero<v8>(qi[u] < a.Nq && d < a.D, Q + (long long)qi[u] * a.qs[1] + d);
-        }
+    for (int s = 0; s < KS; ++s) {
+        const int d = s * 16 + half * 8;
+        qf[s] = load_or_zero<v8>(qi < a.Nq && d < a.D, Q + (long long)qi * a.qs[1] + d);
     }
     Mover<T, DP, KT> mk, mv;
     auto fetch = [&](int t) {
@@ -55,15 +50,10 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
         mv.load(V + k0 * a.vs[1], a.vs[1], kend - k0, a.D, !mask, [&](int r) { return mask[k0 + r] != 0; });
     };
 
-    f32x16_t o[QB][DB];
-    float m[QB], l[QB];
+    f32x16_t o[DB];
 #pragma unroll
-    for (int u = 0; u < QB; ++u) {
-        m[u] = -INFINITY;
-        l[u] = 0.f;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) o[u][d] = zero16();
-    }
+    for (int d = 0; d < DB; ++d) o[d] = zero16();
+    float m = -INFINITY, l = 0.f;
     const float c = a.scale * LOG2E;
     const unsigned rows_at = Tile<T, DP>::rows_at(lane), cols_at = Tile<T, DP>::cols_at(lane);
     if (ntiles > 0) {
@@ -76,125 +66,100 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
         const int k0 = t * KT, buf = (t & 1) * TILE;
         const unsigned ra = keep(rows_at) + buf * 2, ca = keep(cols_at) + buf * 2;
         if (t + 1 < ntiles) fetch(t + 1);
-        // FAR: all relative positions of the tile lie past one end of the line, the bias is the constant `add`
-        auto body = [&](auto far_, float add) {
-            constexpr bool FAR = decltype(far_)::value;
-            f32x16_t x[QB][2];
+        f32x16_t x[2];
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
+        for (int kb = 0; kb < 2; ++kb) {
+            x[kb] = zero16();
 #pragma unroll
-                for (int u = 0; u < QB; ++u) x[u][kb] = zero16();
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const v8 kf = Tile<T, DP>::rows(lk, ra, kb * 32, s);
-#pragma unroll
-                    for (int u = 0; u < QB; ++u) x[u][kb] = Mma<T>::mma(kf, qf[u][s], x[u][kb]);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < QB; ++u) {
-                if constexpr (!FAR) {
-                    const float* at = line + (k0 + 4 * half - qi[u] - start + reach);       // entry of the lane's first key
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) x[u][kb][r] = fmaf(x[u][kb][r], c, at[kb * 32 + 8 * (r / 4) + r % 4]);
-                }
-                // keys the lane's query sees: bit n of `see` = key k0 + n
-                if (mask || k0 + KT > min(len, a.causal ? w0 + u * 32 + start + 1 : len)) {
-                    unsigned long long bits = ~0ull;
-                    if (mask) bits = __ballot(k0 + lane < a.Nk && mask[min(k0 + lane, a.Nk - 1)]);
-                    const int lim = min(len, a.causal ? qi[u] + start + 1 : len) - k0;
-                    const unsigned long long see = lim >= 64 ? bits : lim <= 0 ? 0 : bits & ((1ull << lim) - 1);
-                    const unsigned s0 = (unsigned)see >> (4 * half), s1 = (unsigned)(see >> 32) >> (4 * half);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        if (!(s0 >> (8 * (r / 4) + r % 4) & 1)) x[u][0][r] = -INFINITY;
-                        if (!(s1 >> (8 * (r / 4) + r % 4) & 1)) x[u][1][r] = -INFINITY;
-                    }
-                }
-                float top = max2(x[u][0][0], x[u][1][0]);
-#pragma unroll
-                for (int r = 1; r < 16; ++r) top = max2(top, max2(x[u][0][r], x[u][1][r]));
-                top = half_max(top);
-                if constexpr (FAR) top = fmaf(top, c, add);
-                const float mn = max2(m[u], top);
-                if (__any(mn > m[u])) {
-                    const float alpha = exp2_hw(m[u] - (mn == -INFINITY ? 0.f : mn));
-                    l[u] *= alpha;
-#pragma unroll
-                    for (int d = 0; d < DB; ++d)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) o[u][d][r] *= alpha;
-                    m[u] = mn;
-                }
-                const float sub = Mma<T>::shift - (m[u] == -INFINITY ? 0.f : m[u]) + (FAR ? add : 0.f);
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        x[u][kb][r] = exp2_hw(FAR ? fmaf(x[u][kb][r], c, sub) : x[u][kb][r] + sub);
-                        sum[r & 3] += x[u][kb][r];
-                    }
-                l[u] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            }
+            for (int s = 0; s < KS; ++s) x[kb] = Mma<T>::mma(Tile<T, DP>::rows(lk, ra, kb * 32, s), qf[s], x[kb]);
+        }
+        // base-2 logits are mul x + add: one bias for a tile past an end of the line, else x takes its bias in place.  (One body for both:
+        // two would cost a copy of the accumulators where they meet.)
+        const int rel_hi = k0 + KT - 1 - w0 - start, rel_lo = k0 - (w0 + 31) - start;
+        float mul = c, add = rel_hi <= -reach ? line[0] : line[last];
+        if (rel_hi > -reach && rel_lo < right) {
+            mul = 1.f;
+            add = 0.f;
+            const float* at = line + (k0 + 4 * half - qi - start + reach);          // entry of the lane's first key
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    v8 p[QB], rest[QB];
+                for (int r = 0; r < 16; ++r) x[kb][r] = fmaf(x[kb][r], c, at[kb * 32 + 8 * (r / 4) + r % 4]);
+        }
+        // keys the lane's query sees: bit n of `see` = key k0 + n
+        if (mask || k0 + KT > first_limit) {
+            unsigned long long bits = ~0ull;
+            if (mask) bits = __ballot(k0 + lane < a.Nk && mask[min(k0 + lane, a.Nk - 1)]);
+            const int lim = my_limit - k0;
+            const unsigned long long see = lim >= 64 ? bits : lim <= 0 ? 0 : bits & ((1ull << lim) - 1);
+            const unsigned s0 = (unsigned)see >> (4 * half), s1 = (unsigned)(see >> 32) >> (4 * half);
 #pragma unroll
-                    for (int u = 0; u < QB; ++u) {
-                        p[u] = pack_step<T>(x[u][kb], s);
-                        if constexpr (LO) rest[u] = pack_rest<T>(x[u][kb], p[u], s);
-                    }
+            for (int r = 0; r < 16; ++r) {
+                x[0][r] = pick(s0, r, x[0][r], -INFINITY);
+                x[1][r] = pick(s1, r, x[1][r], -INFINITY);
+            }
+        }
+        const float mn = max2(m, fmaf(half_max(max2(max16(x[0]), max16(x[1]))), mul, add));
+        if (__any(mn > m)) {
+            const float alpha = exp2_hw(m - (mn == -INFINITY ? 0.f : mn));
+            l *= alpha;
 #pragma unroll
-                    for (int d = 0; d < DB; ++d) {
-                        const v8 vf = Tile<T, DP>::cols(lv, ca, kb * 32 + s * 16, d);
+            for (int d = 0; d < DB; ++d)
 #pragma unroll
-                        for (int u = 0; u < QB; ++u) {
-                            o[u][d] = Mma<T>::mma(vf, p[u], o[u][d]);
-                            if constexpr (LO) o[u][d] = Mma<T>::mma(vf, rest[u], o[u][d]);
-                        }
-                    }
+                for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+            m = mn;
+        }
+        const float sub = Mma<T>::shift - (m == -INFINITY ? 0.f : m) + add;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                x[kb][r] = exp2_hw(fmaf(x[kb][r], mul, sub));
+                sum[r & 3] += x[kb][r];
+            }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const v8 p = pack_step<T>(x[kb], s);
+                v8 rest;
+                if constexpr (LO) rest = pack_rest<T>(x[kb], p, s);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) {
+                    const v8 vf = Tile<T, DP>::cols(lv, ca, kb * 32 + s * 16, d);
+                    o[d] = Mma<T>::mma(vf, p, o[d]);
+                    if constexpr (LO) o[d] = Mma<T>::mma(vf, rest, o[d]);
                 }
-        };
-        const int rel_hi = k0 + KT - 1 - w0 - start, rel_lo = k0 - (w0 + 32 * QB - 1) - start;
-        if (rel_hi <= -reach) body(std::true_type(), line[0]);
-        else if (rel_lo >= right) body(std::true_type(), line[last]);
-        else body(std::false_type(), 0.f);
+            }
         if (t + 1 < ntiles) {
             mk.store(lk + (TILE - buf));
             mv.store(lv + (TILE - buf));
         }
         __syncthreads();
     }
+    const float sum = half_sum(l);
+    const float inv = 1.f / sum;
+    if (qi >= a.Nq) return;
+    const long long row = ((long long)b * a.Nq + qi) * a.H + h;
 #pragma unroll
-    for (int u = 0; u < QB; ++u) {
-        const float sum = half_sum(l[u]);
-        const float inv = 1.f / sum;
-        if (qi[u] >= a.Nq) continue;
-        const long long row = ((long long)b * a.Nq + qi[u]) * a.H + h;
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int g = 0; g < 4; ++g) {
+            const int at = d * 32 + g * 8 + half * 4;
+            if (at >= a.D) continue;
+            typename Mma<T>::v4 w, lo;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const int at = d * 32 + g * 8 + half * 4;
-                if (at >= a.D) continue;
-                typename Mma<T>::v4 w, lo;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float f = empty_or(sum, o[u][d][4 * g + j] * inv);
-                    w[j] = (T)f;
-                    lo[j] = (T)(f - (float)w[j]);
-                }
-                *reinterpret_cast<typename Mma<T>::v4*>((T*)a.out + row * a.D + at) = w;
-                if (LO) *reinterpret_cast<typename Mma<T>::v4*>((T*)a.out_lo + row * a.D + at) = lo;
+            for (int j = 0; j < 4; ++j) {
+                const float f = empty_or(sum, o[d][4 * g + j] * inv);
+                w[j] = (T)f;
+                lo[j] = (T)(f - (float)w[j]);
             }
-        if (a.lse && half == 0)
-            a.lse[((long long)b * a.H + h) * a.Nq + qi[u]] = sum == 0.f ? -INFINITY : m[u] + log2f(sum) - Mma<T>::shift;
-    }
+            *reinterpret_cast<typename Mma<T>::v4*>((T*)a.out + row * a.D + at) = w;
+            if (LO) *reinterpret_cast<typename Mma<T>::v4*>((T*)a.out_lo + row * a.D + at) = lo;
+        }
+    if (a.lse && half == 0) a.lse[((long long)b * a.H + h) * a.Nq + qi] = sum == 0.f ? -INFINITY : m + log2f(sum) - Mma<T>::shift;
 }
 
 // ---- few queries (single tokens): bound by reading K and V once.  The G = H / Hkv heads that share keys times the queries are the 32
@@ -214,7 +179,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     unsigned char* bucket = (unsigned char*)(tab + a.bk.num_buckets * G);
     const int split = blockIdx.x % a.splits, rt = blockIdx.x / a.splits % a.tiles, bh = blockIdx.x / (a.splits * a.tiles);
     const int b = bh / a.Hkv, hk = bh % a.Hkv;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+    const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5, col = lane & 31;
     const int start = seq_start(a, b), len = seq_keys(a, b);
     const int kend = a.causal ? max(0, min(len, a.Nq + start)) : len;
     // this split's keys: an equal share of the existing ones, in whole rounds of 128
@@ -301,13 +266,9 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
         if (mask || k0 + 32 > kz || (a.causal && k0 + 32 > start + 1)) {
             const unsigned see = (lim >= 32 ? bits : lim <= 0 ? 0 : bits & ((1u << lim) - 1)) >> (4 * half);
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (!(see >> (8 * (r / 4) + r % 4) & 1)) x[r] = -INFINITY;
+            for (int r = 0; r < 16; ++r) x[r] = pick(see, r, x[r], -INFINITY);
         }
-        float top = x[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) top = max2(top, x[r]);
-        const float mn = max2(m, half_max(top));
+        const float mn = max2(m, half_max(max16(x)));
         const float base = mn == -INFINITY ? 0.f : mn;
         if (__any(mn > m)) {
             const float alpha = exp2_hw(m - base);
@@ -488,12 +449,11 @@ static void launch_fwd(AttnArgs a, const tcvom_attn_desc* d, hipStream_t st) {
             hipLaunchKernelGGL((attn_join_kernel<T>), dim3(cdiv((long long)a.B * a.Nq * a.H, 4)), dim3(256), 0, st, a);
         return;
     }
-    constexpr int QB = 1;
-    a.tiles = cdiv(a.Nq, 128 * QB);
+    a.tiles = cdiv(a.Nq, 128);
     const dim3 grid((unsigned)((long long)a.B * a.H * a.tiles));
     const size_t lds = line_bytes(a);
-    if (a.out_lo) hipLaunchKernelGGL((attn_fwd_kernel<T, DP, QB, true>), grid, dim3(256), lds, st, a);
-    else hipLaunchKernelGGL((attn_fwd_kernel<T, DP, QB, false>), grid, dim3(256), lds, st, a);
+    if (a.out_lo) hipLaunchKernelGGL((attn_fwd_kernel<T, DP, true>), grid, dim3(256), lds, st, a);
+    else hipLaunchKernelGGL((attn_fwd_kernel<T, DP, false>), grid, dim3(256), lds, st, a);
 }
 
 extern "C" int tcvom_attn_fwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, void* out,

@@ -8,7 +8,6 @@
 //
 // Rounding to 16 bits: p and ds as operands of the matrix products, as the forward rounds p.  The bucket sums take ds in 32 bits.
 #include "attn.h"
-#include <type_traits>
 
 // ---- dq, delta, bucket sums: a wave owns 32 queries of one head (S^T and dP^T as in the forward), the workgroup walks tiles of 64 keys.
 // Bucket sums: a tile past an end of the line adds to one register a lane.  A 32 x 32 block that crosses it is written to LDS skewed, key
@@ -30,7 +29,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     work_item(a, a.B * a.H, bh, tile);
     if (a.causal) tile = a.tiles - 1 - tile;
     const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+    const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5, col = lane & 31;
     const int i0 = tile * BM, start = seq_start(a, b), len = seq_keys(a, b);
     const int i_last = min(i0 + BM, a.Nq) - 1;
     const int kend = a.causal ? max(0, min(len, i_last + start + 1)) : len;
@@ -100,65 +99,60 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
         const unsigned ra = keep(rows_at) + buf * 2, ca = keep(cols_at) + buf * 2;
         if (t + 1 < ntiles) fetch(t + 1);
         const bool holes = mask || i0 + BM > a.Nq || k0 + KT > min(len, a.causal ? w0 + start + 1 : len);
-        // (as in the forward; far sums are taken by the caller from the returned sum of the lane's elements)
-        auto body = [&](auto far_, float add) {
-            constexpr bool FAR = decltype(far_)::value;
-            float total = 0.f;
-            unsigned long long see = 0;
-            if (holes) {                                    // (the whole wave: the ballot is over its 64 lanes)
-                unsigned long long bits = ~0ull;
-                if (mask) bits = __ballot(k0 + lane < a.Nk && mask[min(k0 + lane, a.Nk - 1)]);
-                const int lim = live ? min(len, a.causal ? qi + start + 1 : len) - k0 : 0;
-                see = lim >= 64 ? bits : lim <= 0 ? 0 : bits & ((1ull << lim) - 1);
-            }
-#pragma unroll
-            for (int kb = 0; kb < KT / 32; ++kb) {
-                f32x16_t x = zero16(), g = zero16();
-#pragma unroll
-                for (int s = 0; s < KS; ++s) x = Mma<T>::mma(Tile<T, DP>::rows(lk, ra, kb * 32, s), qf[s], x);
-#pragma unroll
-                for (int s = 0; s < KS; ++s) g = Mma<T>::mma(Tile<T, DP>::rows(lv, ra, kb * 32, s), gf[s], g);
-                const int e0 = k0 + kb * 32 + 4 * half - qi - start + reach;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float b2 = FAR ? add - lse : line[e0 + 8 * (r / 4) + r % 4] - lse;
-                    x[r] = exp2_hw(fmaf(x[r], c, b2)) * (g[r] - delta);
-                }
-                if (holes) {
-                    const unsigned w = (unsigned)(see >> (32 * kb)) >> (4 * half);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (!(w >> (8 * (r / 4) + r % 4) & 1)) x[r] = 0.f;
-                }
-                if (TABLE) {
-                    if constexpr (FAR) {
-                        float s[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                        for (int r = 4; r < 16; ++r) s[r & 3] += x[r];
-                        total += (s[0] + s[1]) + (s[2] + s[3]);
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) put[(8 * (r / 4) + r % 4) * 65] = x[r];
-                        float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int n = 0; n < 32; ++n) s[n & 3] += get[n * 64];
-                        // diagonal key - query = lane - 31 of the block (lane 63: none, zero)
-                        mine[k0 + kb * 32 - w0 - start + reach + lane - 31] += (s[0] + s[1]) + (s[2] + s[3]);
-                    }
-                }
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const v8 p = pack_step<T>(x, s);
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::mma(Tile<T, DP>::cols(lk, ca, kb * 32 + s * 16, d), p, acc[d]);
-                }
-            }
-            return total;
-        };
+        unsigned long long see = 0;
+        if (holes) {
+            unsigned long long bits = ~0ull;
+            if (mask) bits = __ballot(k0 + lane < a.Nk && mask[min(k0 + lane, a.Nk - 1)]);
+            const int lim = live ? min(len, a.causal ? qi + start + 1 : len) - k0 : 0;
+            see = lim >= 64 ? bits : lim <= 0 ? 0 : bits & ((1ull << lim) - 1);
+        }
         const int rel_hi = k0 + KT - 1 - w0 - start, rel_lo = k0 - (w0 + 31) - start;
-        if (rel_hi <= -reach) far_lo += body(std::true_type(), line[0]);
-        else if (rel_lo >= right) far_hi += body(std::true_type(), line[last]);
-        else body(std::false_type(), 0.f);
+        const bool left = rel_hi <= -reach, near = !left && rel_lo < right;
+        const float mul = near ? 1.f : c, add = (near ? 0.f : left ? line[0] : line[last]) - lse;
+        float total = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < KT / 32; ++kb) {
+            f32x16_t x = zero16(), g = zero16();
+#pragma unroll
+            for (int s = 0; s < KS; ++s) x = Mma<T>::mma(Tile<T, DP>::rows(lk, ra, kb * 32, s), qf[s], x);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) g = Mma<T>::mma(Tile<T, DP>::rows(lv, ra, kb * 32, s), gf[s], g);
+            if (near) {
+                const float* at = line + (k0 + kb * 32 + 4 * half - qi - start + reach);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], c, at[8 * (r / 4) + r % 4]);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = exp2_hw(fmaf(x[r], mul, add)) * (g[r] - delta);
+            if (holes) {
+                const unsigned w = (unsigned)(see >> (32 * kb)) >> (4 * half);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = pick(w, r, x[r], 0.f);
+            }
+            if (TABLE) {
+                float s[4] = {0.f, 0.f, 0.f, 0.f};
+                if (near) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) put[(8 * (r / 4) + r % 4) * 65] = x[r];
+#pragma unroll
+                    for (int n = 0; n < 32; ++n) s[n & 3] += get[n * 64];
+                    // diagonal key - query = lane - 31 of the block (lane 63: none, zero)
+                    mine[k0 + kb * 32 - w0 - start + reach + lane - 31] += (s[0] + s[1]) + (s[2] + s[3]);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[r & 3] += x[r];
+                    total += (s[0] + s[1]) + (s[2] + s[3]);
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const v8 p = pack_step<T>(x, s);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::mma(Tile<T, DP>::cols(lk, ca, kb * 32 + s * 16, d), p, acc[d]);
+            }
+        }
+        far_lo += left ? total : 0.f;
+        far_hi += left ? 0.f : total;
         if (t + 1 < ntiles) {
             mk.store(lk + (TILE - buf));
             mv.store(lv + (TILE - buf));
@@ -251,7 +245,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     int bh, tile;
     work_item(a, a.B * heads, bh, tile);
     const int b = bh / heads, h0 = bh % heads * G, hk = h0 / (a.H / a.Hkv);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+    const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5, col = lane & 31;
     const int start = seq_start(a, b), len = seq_keys(a, b);
     const int j0 = tile * BN, w0 = j0 + wave * 32, key = w0 + col;
     const int reach = line_reach(a.bk), right = line_right(a.bk), last = reach + right;
