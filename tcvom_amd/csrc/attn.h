@@ -125,9 +125,13 @@ __device__ __forceinline__ typename Mma<T>::v8 pack_rest(const f32x16_t& p, type
     return r;
 }
 
+// v, computed here: not hoisted out of a loop into a register of its own
+__device__ __forceinline__ unsigned keep(unsigned v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 // Operands from an LDS tile of rows of DP elements (layout: chunk_at).  A lane's byte offset differs between steps by an XOR of a few low
-// bits and a constant, so that one register and one instruction a step address them all; `keep` stops the compiler from holding
-// every step's address in a register of its own across the loop.
+// bits and a constant, so that one register and one instruction a step address them all.
 template <class T, int DP> struct Tile {
     typedef typename Mma<T>::v8 v8;
     static constexpr int ROW = DP * 2;
@@ -147,10 +151,6 @@ template <class T, int DP> struct Tile {
                        Mma<T>::tr(reinterpret_cast<const T*>(p + (off ^ (d << 6) ^ 32) + 8 * ROW)));
     }
 };
-__device__ __forceinline__ unsigned keep(unsigned v) {
-    asm volatile("" : "+v"(v));
-    return v;
-}
 // 16 bytes of a row, zeros where `ok` is false
 template <class V8, class T>
 __device__ __forceinline__ V8 load_or_zero(bool ok, const T* p) {
@@ -166,7 +166,8 @@ template <class T, int DP, int ROWS> struct Mover {
     // rows `first` .. of the tile whose row 0 is at `base`; `left` of them exist, `ok(row)` says which count; the others are zeros
     template <class F>
     __device__ __forceinline__ void load(const T* base, long long stride, int left, int D, bool all, F ok) {
-        const int r0 = threadIdx.x / CH, c = threadIdx.x % CH;
+        const unsigned tid = DP == 128 ? keep(threadIdx.x) : threadIdx.x;        // (the widest kernels have no registers to hold offsets in)
+        const int r0 = tid / CH, c = tid % CH;
         const unsigned off = (unsigned)(r0 * (int)stride + c * 8) * 2u;         // strides below 2^24 (attn_check)
         if (left >= ROWS && D == DP && all && (ROWS * CH) % 256 == 0) {
 #pragma unroll
@@ -184,7 +185,8 @@ template <class T, int DP, int ROWS> struct Mover {
         }
     }
     __device__ __forceinline__ void store(T* tile) const {
-        const int r0 = threadIdx.x / CH, c = threadIdx.x % CH;
+        const unsigned tid = DP == 128 ? keep(threadIdx.x) : threadIdx.x;
+        const int r0 = tid / CH, c = tid % CH;
 #pragma unroll
         for (int n = 0; n < PER; ++n) {
             const int r = r0 + n * STEP;

@@ -27,7 +27,6 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
     const int kend = a.causal ? max(0, min(len, i_last + start + 1)) : len;
     const int ntiles = (kend + KT - 1) / KT;
     const int reach = line_reach(a.bk), right = line_right(a.bk), last = reach + right;
-    fill_line(line, a, h, 256);
 
     const T* Q = (const T*)a.q + b * a.qs[0] + h * a.qs[2];
     const T* K = (const T*)a.k + b * a.ks[0] + hk * a.ks[2];
@@ -56,8 +55,9 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
     float m = -INFINITY, l = 0.f;
     const float c = a.scale * LOG2E;
     const unsigned rows_at = Tile<T, DP>::rows_at(lane), cols_at = Tile<T, DP>::cols_at(lane);
+    if (ntiles > 0) fetch(0);
+    fill_line(line, a, h, 256);                            // (the first tile's loads are in flight)
     if (ntiles > 0) {
-        fetch(0);
         mk.store(lk);
         mv.store(lv);
     }
@@ -185,10 +185,6 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     // this split's keys: an equal share of the existing ones, in whole rounds of 128
     const int share = (kend + a.splits * 128 - 1) / (a.splits * 128) * 128;
     const int ka = min(kend, split * share), kz = min(kend, ka + share);
-    for (int t = threadIdx.x; t < a.bk.num_buckets * G; t += 256)
-        tab[t] = a.table[(long long)(t / G) * a.H + hk * G + t % G] * LOG2E;
-    for (int t = threadIdx.x; t <= last; t += 256) bucket[t] = (unsigned char)rel_bucket(a.bk, t - reach);
-
     const int row = rt * 32 + col, g = min(row, rows - 1) / a.Nq, i = min(row, rows - 1) % a.Nq, h = hk * G + g;
     const bool live = row < rows;
     const T* Q = (const T*)a.q + b * a.qs[0] + h * a.qs[2] + (long long)i * a.qs[1];
@@ -233,6 +229,10 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     const unsigned cols_at = Tile<T, DP>::cols_at(lane);
     int k0 = ka + wave * 32;
     if (k0 < kz) fetch(k0);
+    // (the first keys' loads are in flight)
+    for (int t = threadIdx.x; t < a.bk.num_buckets * G; t += 256)
+        tab[t] = a.table[(long long)(t / G) * a.H + hk * G + t % G] * LOG2E;
+    for (int t = threadIdx.x; t <= last; t += 256) bucket[t] = (unsigned char)rel_bucket(a.bk, t - reach);
     __syncthreads();
     const float bias_lo = tab[bucket[0] * G + g], bias_hi = tab[bucket[last] * G + g];
     for (; k0 < kz; k0 += 128) {
@@ -360,31 +360,39 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     }
 }
 
-// joins the splits of a row: a wave a row, a lane 2 channels (D <= 128)
+// joins the splits of a row: a workgroup a row, a wave every fourth split, a lane 2 channels (D <= 128); all of a wave's loads are in
+// flight at once, the waves meet in LDS
 template <class T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-    const int lane = threadIdx.x & 63;
-    const long long rows = (long long)a.B * a.Nq * a.H, row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= rows) return;
-    const int ld = a.D + 4;
+    __shared__ float red[4][64 * 2 + 1];
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    const long long rows = (long long)a.B * a.Nq * a.H, row = blockIdx.x;
+    const int ld = a.D + 4, d = lane * 2;
     const float* p = a.partial + row * ld;
     const long long step = rows * ld;
     float M = -INFINITY;
-    for (int s = lane; s < a.splits; s += 64) M = fmaxf(M, p[s * step + a.D]);
-    M = wave_max(M);
+    for (int s = lane; s < a.splits; s += 64) M = max2(M, p[s * step + a.D]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) M = max2(M, __shfl_xor(M, o, 64));
     const float base = M == -INFINITY ? 0.f : M;
     float L = 0.f, o0 = 0.f, o1 = 0.f;
-    const int d = lane * 2;
-#pragma unroll 4
-    for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 8
+    for (int s = wave; s < a.splits; s += 4) {
         const float w = exp2_hw(p[s * step + a.D] - base);
+        float2 f = make_float2(0.f, 0.f);
+        if (d < a.D) f = *reinterpret_cast<const float2*>(p + s * step + d);
         L += w * p[s * step + a.D + 1];
-        if (d < a.D) {
-            const float2 f = *reinterpret_cast<const float2*>(p + s * step + d);
-            o0 += w * f.x;
-            o1 += w * f.y;
-        }
+        o0 += w * f.x;
+        o1 += w * f.y;
     }
+    red[wave][d] = o0;
+    red[wave][d + 1] = o1;
+    if (lane == 0) red[wave][128] = L;
+    __syncthreads();
+    if (wave) return;
+    L = (red[0][128] + red[1][128]) + (red[2][128] + red[3][128]);
+    o0 = (red[0][d] + red[1][d]) + (red[2][d] + red[3][d]);
+    o1 = (red[0][d + 1] + red[1][d + 1]) + (red[2][d + 1] + red[3][d + 1]);
     const float inv = 1.f / L;
     if (d < a.D) {
         typename Mma<T>::v2 w = {(T)empty_or(L, o0 * inv), (T)empty_or(L, o1 * inv)};
@@ -413,7 +421,7 @@ int attn_check(const char* who, const tcvom_attn_desc* d, AttnArgs* a) {
     *a = AttnArgs();
     a->B = d->B; a->Nq = d->Nq; a->Nk = d->Nk; a->H = d->H; a->Hkv = d->Hkv; a->D = d->D;
     a->causal = d->causal; a->q_start = d->q_start; a->scale = d->scale;
-    a->k_lens = d->k_lens; a->q_starts = d->q_starts; a->key_mask = d->key_mask; a->bk = d->buckets;
+    a->k_lens = d->k_lens; a->q_starts = d->q_starts; a->key_mask = d->key_mask; a->bk = pad_buckets(d->buckets);
     for (int n = 0; n < 3; ++n) { a->qs[n] = d->q_stride[n]; a->ks[n] = d->k_stride[n]; a->vs[n] = d->v_stride[n]; }
     return 0;
 }
@@ -446,7 +454,7 @@ static void launch_fwd(AttnArgs a, const tcvom_attn_desc* d, hipStream_t st) {
         const dim3 grid((unsigned)((long long)a.B * a.Hkv * a.tiles * a.splits));
         hipLaunchKernelGGL((attn_few_kernel<T, DP>), grid, dim3(256), lds, st, a);
         if (a.splits > 1)
-            hipLaunchKernelGGL((attn_join_kernel<T>), dim3(cdiv((long long)a.B * a.Nq * a.H, 4)), dim3(256), 0, st, a);
+            hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((long long)a.B * a.Nq * a.H)), dim3(256), 0, st, a);
         return;
     }
     a.tiles = cdiv(a.Nq, 128);

@@ -35,7 +35,6 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     const int kend = a.causal ? max(0, min(len, i_last + start + 1)) : len;
     const int ntiles = (kend + KT - 1) / KT;
     const int reach = line_reach(a.bk), right = line_right(a.bk), last = reach + right;
-    fill_line(line, a, h, 256);
     // [4][last + 1 + 2 MARGIN]: a line of sums for each wave, with margins as the bias has
     const int pitch = last + 1 + 2 * MARGIN;
     float* sums = line_ + pitch;
@@ -57,20 +56,26 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     const int w0 = i0 + wave * 32, qi = w0 + col;
     const long long stat = ((long long)b * a.H + h) * a.Nq + qi, orow = (((long long)b * a.Nq + qi) * a.H + h) * a.D;
     const float raw = qi < a.Nq ? a.lse[stat] : -INFINITY;
-    const bool live = raw != -INFINITY;                     // a row without a key has no gradient, whatever its dout holds
-    const float lse = live ? raw : 0.f;
     v8 qf[KS], gf[KS];
     float delta = 0.f;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
         const int d = s * 16 + half * 8;
-        const bool ok = live && d < a.D;
+        const bool ok = qi < a.Nq && d < a.D;
         qf[s] = load_or_zero<v8>(ok, Q + (long long)qi * a.qs[1] + d);
         gf[s] = load_or_zero<v8>(ok, dO + (long long)qi * a.dos[1] + d);
         const v8 hi = load_or_zero<v8>(ok, (const T*)a.out + orow + d);
         const v8 lo = load_or_zero<v8>(ok && a.out_lo, (const T*)a.out_lo + orow + d);
 #pragma unroll
         for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[s][j], (float)hi[j] + (float)lo[j], delta);
+    }
+    // a row without a key has no gradient, whatever its dout holds
+    const bool live = raw != -INFINITY;
+    const float lse = live ? raw : 0.f;
+    if (!live) {
+        delta = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) gf[s] = qf[s] = v8{};
     }
     delta = half_sum(delta);
     if (half == 0 && qi < a.Nq) a.delta[stat] = delta;
@@ -88,8 +93,9 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     float far_lo = 0.f, far_hi = 0.f;
     const float c = a.scale * LOG2E;
     const unsigned rows_at = Tile<T, DP>::rows_at(lane), cols_at = Tile<T, DP>::cols_at(lane);
+    if (ntiles > 0) fetch(0);
+    fill_line(line, a, h, 256);
     if (ntiles > 0) {
-        fetch(0);
         mk.store(lk);
         mv.store(lv);
     }
@@ -236,8 +242,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8, QT = 32, BN = 128, TILE = QT * DP;
     __shared__ __align__(16) T lq[2 * TILE];
     __shared__ __align__(16) T lg[2 * TILE];
-    __shared__ __align__(16) T lv[BN * DP];                 // this workgroup's values, operand B of dP = dO V^T: no registers left for them
-    __shared__ __align__(16) float ls[2][QT], ld[2][QT];
+    constexpr bool VREG = DP < 128;                         // values, operand B of dP = dO V^T, in registers; width 128 has none left
+    __shared__ __align__(16) T lv[VREG ? 8 : BN * DP];
+    __shared__ __align__(16) float ls[4][QT], ld[4][QT];    // log-sums and deltas of the tiles: written two tiles ahead
     extern __shared__ float line_[];
     float* line = line_ + MARGIN;
 
@@ -253,12 +260,13 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     const bool seen = key < len && (!mask || mask[key]);
     const T* K = (const T*)a.k + b * a.ks[0] + hk * a.ks[2] + (long long)key * a.ks[1];
     const T* V = (const T*)a.v + b * a.vs[0] + hk * a.vs[2] + (long long)key * a.vs[1];
-    v8 kf[KS];
+    v8 kf[KS], vf[KS];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
         const int d = s * 16 + half * 8;
         kf[s] = load_or_zero<v8>(seen && d < a.D, K + d);
-        *reinterpret_cast<v8*>(&lv[chunk_at<DP>(wave * 32 + col, s * 2 + half) * 8]) = load_or_zero<v8>(seen && d < a.D, V + d);
+        vf[s] = load_or_zero<v8>(seen && d < a.D, V + d);
+        if constexpr (!VREG) *reinterpret_cast<v8*>(&lv[chunk_at<DP>(wave * 32 + col, s * 2 + half) * 8]) = vf[s];
     }
     f32x16_t dk[DB], dv[DB];
 #pragma unroll
@@ -274,61 +282,79 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     const int nt = j0 < len && i_first < a.Nq ? (a.Nq - i_first + QT - 1) / QT : 0;
     Mover<T, DP, QT> mq, mg;
     constexpr int PER = Mover<T, DP, QT>::PER, STEP = Mover<T, DP, QT>::STEP;
-    float rl[PER], rs = 0.f, rd = 0.f;
-    int fh = h0, fi = i_first;                              // head and first query of the next tile
-    auto fetch = [&]() {
-        const T* Q = (const T*)a.q + b * a.qs[0] + fh * a.qs[2] + fi * a.qs[1];
-        const T* dO = (const T*)a.dout + b * a.dos[0] + fh * a.dos[2] + fi * a.dos[1];
-        const float* lse = a.lse + ((long long)b * a.H + fh) * a.Nq + fi;
-        const float* delta = a.delta + ((long long)b * a.H + fh) * a.Nq + fi;
-        const int left = a.Nq - fi;
-        auto ok = [](int) { return true; };
-        mq.load(Q, a.qs[1], left, a.D, true, ok);
-        mg.load(dO, a.dos[1], left, a.D, true, ok);
-#pragma unroll
-        for (int n = 0; n < PER; ++n) {
-            const int r = threadIdx.x / CH + n * STEP;
-            rl[n] = r < left ? lse[r] : -INFINITY;
-        }
-        if (threadIdx.x < QT) {
-            rs = (int)threadIdx.x < left ? lse[threadIdx.x] : -INFINITY;
-            rd = (int)threadIdx.x < left ? delta[threadIdx.x] : 0.f;
-        }
-        fi += QT;
-        if (fi >= a.Nq) {
-            fi = i_first;
-            ++fh;
+    // head and first query of the tile that is fetched next: from the last queries back to the first, so that the workgroups of a causal
+    // head, which end at different ones, start together
+    const int i_last = i_first + (nt - 1) * QT;
+    struct Place { int h, i; } at_q = {h0, i_last}, at_s = {h0, i_last};
+    auto advance = [&](Place& p) {
+        p.i -= QT;
+        if (p.i < i_first) {
+            p.i = i_last;
+            ++p.h;
         }
     };
-    auto store = [&](int buf) {
+    float rs = 0.f, rd = 0.f;
+    auto fetch_stats = [&]() {
+        if (threadIdx.x < QT) {
+            const long long stat = ((long long)b * a.H + at_s.h) * a.Nq + at_s.i + threadIdx.x;
+            const bool ok = at_s.i + (int)threadIdx.x < a.Nq;
+            rs = ok ? a.lse[stat] : -INFINITY;
+            rd = ok ? a.delta[stat] : 0.f;
+        }
+        advance(at_s);
+    };
+    auto store_stats = [&](int t) {
+        if (threadIdx.x < QT) {
+            ls[t & 3][threadIdx.x] = rs == -INFINITY ? INFINITY : rs - Mma<T>::shift;       // p = 0 in rows that are empty or past the end
+            ld[t & 3][threadIdx.x] = rd * small;
+        }
+    };
+    auto all = [](int) { return true; };
+    auto fetch_q = [&]() {
+        mq.load((const T*)a.q + b * a.qs[0] + at_q.h * a.qs[2] + at_q.i * a.qs[1], a.qs[1], a.Nq - at_q.i, a.D, true, all);
+    };
+    auto fetch_g = [&]() {
+        mg.load((const T*)a.dout + b * a.dos[0] + at_q.h * a.dos[2] + at_q.i * a.dos[1], a.dos[1], a.Nq - at_q.i, a.D, true, all);
+        advance(at_q);
+    };
+    auto store_g = [&](int t) {
         // a row without a key has no gradient, whatever its dout holds: 0 x inf would not vanish in the products
 #pragma unroll
         for (int n = 0; n < PER; ++n)
-            if (rl[n] == -INFINITY) mg.reg[n] = (u32x4_t){0, 0, 0, 0};
-        mq.store(lq + buf * TILE);
-        mg.store(lg + buf * TILE);
-        if (threadIdx.x < QT) {
-            ls[buf][threadIdx.x] = rs == -INFINITY ? INFINITY : rs - Mma<T>::shift;         // p = 0 in rows that are empty or past the end
-            ld[buf][threadIdx.x] = rd * small;
-        }
+            if (ls[t & 3][(threadIdx.x / CH + n * STEP) % QT] == INFINITY) mg.reg[n] = (u32x4_t){0, 0, 0, 0};
+        mg.store(lg + (t & 1) * TILE);
     };
     const int total = nt * G;
     if (total > 0) {
-        fetch();
-        store(0);
+        fetch_q();
+        fetch_g();
+        fetch_stats();
+        store_stats(0);
+        if (total > 1) {
+            fetch_stats();
+            store_stats(1);
+        }
+        mq.store(lq);
+        __syncthreads();
+        store_g(0);
     }
-    int i0 = i_first - QT, h = h0 - 1;
+    int i0 = i_first, h = h0 - 1;
     for (int t = 0; t < total; ++t) {
         const int buf = t & 1;
-        i0 += QT;
+        i0 -= QT;
         const unsigned va = keep(rows_at), ra = va + buf * (QT * DP * 2), ca = keep(cols_at) + buf * (QT * DP * 2);
-        if (t == 0 || i0 >= a.Nq) {                          // another head's bias
-            i0 = i_first;
+        if (i0 < i_first) {                                  // another head's bias
+            i0 = i_last;
             __syncthreads();
             fill_line(line, a, ++h, 256);
             __syncthreads();
         }
-        if (t + 1 < total) fetch();
+        // the next tile: at width 128 its dO is fetched once its Q has left the registers
+        if (t + 2 < total) fetch_stats();
+        if (t + 1 < total) {
+            fetch_q();
+            if (DP < 128) fetch_g();
+        }
         f32x16_t x = zero16();
 #pragma unroll
         for (int s = 0; s < KS; ++s) x = Mma<T>::mma(Tile<T, DP>::rows(lq, ra, 0, s), kf[s], x);
@@ -337,7 +363,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
         float sub[16];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const float4 s4 = *reinterpret_cast<const float4*>(&ls[buf][8 * q + 4 * half]);
+            const float4 s4 = *reinterpret_cast<const float4*>(&ls[t & 3][8 * q + 4 * half]);
             sub[4 * q] = s4.x; sub[4 * q + 1] = s4.y; sub[4 * q + 2] = s4.z; sub[4 * q + 3] = s4.w;
         }
         if (far) {
@@ -362,13 +388,19 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) dv[d] = Mma<T>::mma(Tile<T, DP>::cols(lg, ca, s * 16, d), p, dv[d]);
         }
-        if constexpr (DP == 128) __builtin_amdgcn_sched_barrier(0);      // (the next product's operands would not fit beside this one's)
+        if constexpr (DP == 128) {
+            __builtin_amdgcn_sched_barrier(0);               // (the next product's operands would not fit beside this one's)
+            if (t + 1 < total) {
+                mq.store(lq + (buf ^ 1) * TILE);
+                fetch_g();
+            }
+        }
         f32x16_t g = zero16();
 #pragma unroll
-        for (int s = 0; s < KS; ++s) g = Mma<T>::mma(Tile<T, DP>::rows(lg, ra, 0, s), Tile<T, DP>::rows(lv + wave * 32 * DP, va, 0, s), g);
+        for (int s = 0; s < KS; ++s) g = Mma<T>::mma(Tile<T, DP>::rows(lg, ra, 0, s), VREG ? vf[s] : Tile<T, DP>::rows(lv + wave * 32 * DP, va, 0, s), g);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const float4 d4 = *reinterpret_cast<const float4*>(&ld[buf][8 * q + 4 * half]);
+            const float4 d4 = *reinterpret_cast<const float4*>(&ld[t & 3][8 * q + 4 * half]);
             x[4 * q] *= fmaf(g[4 * q], small, -d4.x);
             x[4 * q + 1] *= fmaf(g[4 * q + 1], small, -d4.y);
             x[4 * q + 2] *= fmaf(g[4 * q + 2], small, -d4.z);
@@ -380,7 +412,11 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
 #pragma unroll
             for (int d = 0; d < DB; ++d) dk[d] = Mma<T>::mma(Tile<T, DP>::cols(lq, ca, s * 16, d), p, dk[d]);
         }
-        if (t + 1 < total) store(buf ^ 1);
+        if (t + 1 < total) {
+            if (DP < 128) mq.store(lq + (buf ^ 1) * TILE);
+            store_g(t + 1);
+        }
+        if (t + 2 < total) store_stats(t + 2);
         __syncthreads();
     }
     if (key >= a.Nk) return;

@@ -53,6 +53,7 @@ extern "C" int tcvom_relbias_fwd(const float* table, void* out, const tcvom_rel_
     TCVOM_CHECK_ARG(type >= TCVOM_TYPE_F32 && type <= TCVOM_TYPE_F16, "relbias_fwd: type %d", type);
     TCVOM_CHECK_ARG(q_len < (1LL << 31) && k_len < (1LL << 31) && q_start < (1LL << 40) && q_start > -(1LL << 40), "relbias_fwd: lengths");
     if (const int rc = check_buckets("relbias_fwd", buckets)) return rc;
+    const tcvom_rel_buckets bk = pad_buckets(*buckets);
     if (q_len == 0 || k_len == 0) return 0;
     // 64 KB of output and more a workgroup, but at least 8 workgroups a CU while there are rows for it
     int64_t rows = cdiv(65536, k_len * (type == TCVOM_TYPE_F32 ? 4 : 2));
@@ -64,11 +65,11 @@ extern "C" int tcvom_relbias_fwd(const float* table, void* out, const tcvom_rel_
     const size_t lds = sizeof(float) * (line_reach(*buckets) + line_right(*buckets) + 1);
     const hipStream_t st = (hipStream_t)stream;
     if (type == TCVOM_TYPE_F32)
-        hipLaunchKernelGGL(relbias_fwd_kernel<float>, grid, dim3(256), lds, st, table, (float*)out, *buckets, heads, q_len, k_len, q_start, (int)rows);
+        hipLaunchKernelGGL(relbias_fwd_kernel<float>, grid, dim3(256), lds, st, table, (float*)out, bk, heads, q_len, k_len, q_start, (int)rows);
     else if (type == TCVOM_TYPE_BF16)
-        hipLaunchKernelGGL(relbias_fwd_kernel<__bf16>, grid, dim3(256), lds, st, table, (__bf16*)out, *buckets, heads, q_len, k_len, q_start, (int)rows);
+        hipLaunchKernelGGL(relbias_fwd_kernel<__bf16>, grid, dim3(256), lds, st, table, (__bf16*)out, bk, heads, q_len, k_len, q_start, (int)rows);
     else
-        hipLaunchKernelGGL(relbias_fwd_kernel<_Float16>, grid, dim3(256), lds, st, table, (_Float16*)out, *buckets, heads, q_len, k_len, q_start, (int)rows);
+        hipLaunchKernelGGL(relbias_fwd_kernel<_Float16>, grid, dim3(256), lds, st, table, (_Float16*)out, bk, heads, q_len, k_len, q_start, (int)rows);
     TCVOM_LAUNCH_CHECK("relbias_fwd");
     return 0;
 }
@@ -92,15 +93,16 @@ __global__ __launch_bounds__(256) void relbias_bwd_kernel(const T* dout, float* 
         const int t = 1 + (int)blockIdx.x * 256 + threadIdx.x;             // inner entry: rel = t - reach
         if (t >= last) return;
         const long long off = t - reach + q_start;                         // its key in row i is i + off
-        long long a = -off > i0 ? -off : i0, b = Nk - off < i1 ? Nk - off : i1;
-        float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        const T* p = plane + a * Nk + a + off;
-        long long i = a;
-        for (; i + 8 <= b; i += 8, p += 8 * (Nk + 1))
+        const long long a = -off > i0 ? -off : i0, b = Nk - off < i1 ? Nk - off : i1;     // rows whose key exists
+        const T* p = plane + i0 * Nk + i0 + off;
+        float s[BIAS_ROWS];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) s[u] += (float)p[u * (Nk + 1)];
-        for (; i < b; ++i, p += Nk + 1) s[0] += (float)*p;
-        out[t] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+        for (int u = 0; u < BIAS_ROWS; ++u) s[u] = i0 + u >= a && i0 + u < b ? (float)p[u * (Nk + 1)] : 0.f;
+#pragma unroll
+        for (int o = BIAS_ROWS / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int u = 0; u < o; ++u) s[u] += s[u + o];
+        out[t] = s[0];
         return;
     }
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -111,38 +113,46 @@ __global__ __launch_bounds__(256) void relbias_bwd_kernel(const T* dout, float* 
         long long jl = i + q_start - reach + 1, jr = i + q_start - reach + last;
         jl = jl < 0 ? 0 : jl > Nk ? Nk : jl;
         jr = jr < 0 ? 0 : jr > Nk ? Nk : jr;
+        // both sides together, four vectors of each in flight
+        const T* vec[2];
+        int nv[2];
+        float s[2][V];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             const long long ja = w ? jr : 0, jb = w ? Nk : jl;
             long long head = ((16 - ((uintptr_t)(row + ja) & 15)) & 15) / sizeof(T);
             if (head > jb - ja) head = jb - ja;
-            float s[V];
+            nv[w] = (int)((jb - ja - head) / V);
+            vec[w] = row + ja + head;
 #pragma unroll
-            for (int u = 0; u < V; ++u) s[u] = 0.f;
-            if (lane < head) s[0] = (float)row[ja + lane];
-            const long long nv = (jb - ja - head) / V;
-            const T* vec = row + ja + head;
-            long long n = lane;
-            for (; n + 192 < nv; n += 256) {                   // four loads in flight
-                float f[4][V];
+            for (int u = 0; u < V; ++u) s[w][u] = 0.f;
+            if (lane < head) s[w][0] = (float)row[ja + lane];
+            const long long j = ja + head + (long long)nv[w] * V + lane;
+            if (j < jb) s[w][V - 1] += (float)row[j];
+        }
+        for (int n = lane; n < max(nv[0], nv[1]); n += 256) {
+            typename RawVec<T, V>::type f[2][4];
 #pragma unroll
-                for (int w = 0; w < 4; ++w) load_vec<T, V>(vec + (n + 64 * w) * V, f[w]);
+            for (int w = 0; w < 2; ++w)
 #pragma unroll
-                for (int u = 0; u < V; ++u) s[u] += (f[0][u] + f[1][u]) + (f[2][u] + f[3][u]);
-            }
-            for (; n < nv; n += 64) {
-                float f[V];
-                load_vec<T, V>(vec + n * V, f);
+                for (int k = 0; k < 4; ++k) {
+                    f[w][k] = (typename RawVec<T, V>::type)(T)0.f;
+                    if (n + 64 * k < nv[w]) f[w][k] = load_raw<T, V>(vec[w] + (long long)(n + 64 * k) * V);
+                }
 #pragma unroll
-                for (int u = 0; u < V; ++u) s[u] += f[u];
-            }
-            const long long j = ja + head + nv * V + lane;
-            if (j < jb) s[V - 1] += (float)row[j];
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int u = 0; u < V; ++u) s[w][u] += (float)f[w][k][u];
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
 #pragma unroll
             for (int o = V / 2; o > 0; o >>= 1)
 #pragma unroll
-                for (int u = 0; u < o; ++u) s[u] += s[u + o];
-            side[w] += s[0];
+                for (int u = 0; u < o; ++u) s[w][u] += s[w][u + o];
+            side[w] += s[w][0];
         }
     }
 #pragma unroll
@@ -186,18 +196,19 @@ extern "C" int tcvom_relbias_bwd(const void* dout, float* dtable, float* work, i
     TCVOM_CHECK_ARG(q_len <= 65535LL * BIAS_ROWS && (int64_t)cdiv(q_len, BIAS_ROWS) * TCVOM_MAX_BUCKET_REACH < (1LL << 31) && k_len < (1LL << 31) && q_start < (1LL << 40) && q_start > -(1LL << 40),
                     "relbias_bwd: lengths");
     if (const int rc = check_buckets("relbias_bwd", buckets)) return rc;
+    const tcvom_rel_buckets bk = pad_buckets(*buckets);
     TCVOM_CHECK_ARG(work_floats >= tcvom_relbias_bwd_work(buckets, heads, q_len), "relbias_bwd: %lld floats of workspace", (long long)work_floats);
     const int last = line_reach(*buckets) + line_right(*buckets), chunks = cdiv(q_len, BIAS_ROWS);
     const dim3 grid(cdiv(last - 1, 256) + 1, chunks, heads);
     const hipStream_t st = (hipStream_t)stream;
     if (type == TCVOM_TYPE_F32)
-        hipLaunchKernelGGL(relbias_bwd_kernel<float>, grid, dim3(256), 0, st, (const float*)dout, work, *buckets, q_len, k_len, q_start);
+        hipLaunchKernelGGL(relbias_bwd_kernel<float>, grid, dim3(256), 0, st, (const float*)dout, work, bk, q_len, k_len, q_start);
     else if (type == TCVOM_TYPE_BF16)
-        hipLaunchKernelGGL(relbias_bwd_kernel<__bf16>, grid, dim3(256), 0, st, (const __bf16*)dout, work, *buckets, q_len, k_len, q_start);
+        hipLaunchKernelGGL(relbias_bwd_kernel<__bf16>, grid, dim3(256), 0, st, (const __bf16*)dout, work, bk, q_len, k_len, q_start);
     else
-        hipLaunchKernelGGL(relbias_bwd_kernel<_Float16>, grid, dim3(256), 0, st, (const _Float16*)dout, work, *buckets, q_len, k_len, q_start);
+        hipLaunchKernelGGL(relbias_bwd_kernel<_Float16>, grid, dim3(256), 0, st, (const _Float16*)dout, work, bk, q_len, k_len, q_start);
     TCVOM_LAUNCH_CHECK("relbias_bwd");
-    hipLaunchKernelGGL(relbias_table_kernel, dim3(buckets->num_buckets, heads), dim3(256), 0, st, work, dtable, *buckets, heads, chunks);
+    hipLaunchKernelGGL(relbias_table_kernel, dim3(buckets->num_buckets, heads), dim3(256), 0, st, work, dtable, bk, heads, chunks);
     TCVOM_LAUNCH_CHECK("relbias_table");
     return 0;
 }

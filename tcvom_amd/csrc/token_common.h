@@ -56,17 +56,25 @@ __device__ __forceinline__ void store_first(T* p, const float (&f)[V], int n) {
 // the kernels work on the "line" of values at rel = -reach .. right (reach = starts[n_starts - 1], right = reach if bidirectional else 0).
 __host__ __device__ __forceinline__ int line_reach(const tcvom_rel_buckets& b) { return b.starts[b.n_starts - 1]; }
 __host__ __device__ __forceinline__ int line_right(const tcvom_rel_buckets& b) { return b.bidirectional ? line_reach(b) : 0; }
-// bucket of rel: a uniform loop over the borders (scalar loads from the kernel arguments), run once per line entry and workgroup
+// bucket of rel: a uniform loop over the borders, 16 at a time (one scalar load of the kernel arguments; pad_buckets fills the last 16)
 __device__ __forceinline__ int rel_bucket(const tcvom_rel_buckets& b, int rel) {
     const int d = rel < 0 ? -rel : (b.bidirectional ? rel : 0);
     int n = d;
-    if (d >= b.exact) {
-        n = b.exact - 1;
-        for (int k = 0; k < b.n_starts; ++k) n += d >= b.starts[k];
+    if (d >= b.exact) n = b.exact - 1;
+    for (int k = 0; k < b.n_starts; k += 16) {
+        int more = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) more += d >= b.starts[k + i];
+        n += more;                                            // (a distance below `exact` is below every border)
     }
     return n + (b.bidirectional && rel > 0 ? b.num_buckets / 2 : 0);
 }
-
+static_assert(TCVOM_MAX_BUCKET_STARTS % 16 == 0, "rel_bucket reads the borders 16 at a time");
+static inline tcvom_rel_buckets pad_buckets(const tcvom_rel_buckets& b) {
+    tcvom_rel_buckets p = b;
+    for (int k = b.n_starts; k < TCVOM_MAX_BUCKET_STARTS; ++k) p.starts[k] = 1 << 30;
+    return p;
+}
 // the line entries of bucket b: t0 <= t < t1 (possibly none)
 __device__ __forceinline__ void bucket_entries(const tcvom_rel_buckets& bk, int b, int& t0, int& t1) {
     const int side = bk.bidirectional ? bk.num_buckets / 2 : bk.num_buckets, reach = line_reach(bk);

@@ -184,7 +184,7 @@ def _attn_desc(q, k, v, buckets, causal, scale, k_lens, key_mask, q_start, q_sta
 def _attention(q, k, v, table, train, out_lo, *args):
     """(out, lse or None) of tensors in the kernels' layout."""
     d = C.byref(_attn_desc(q, k, v, *args))
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if train else None
     lo = torch.empty_like(out) if out_lo else None
     n = L.call('tcvom_attn_fwd_work', d)
@@ -209,7 +209,7 @@ class _BiasedAttention(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, table, out, out_lo, lse, k_lens, key_mask, q_starts = ctx.saved_tensors
         buckets, causal, scale, q_start = ctx.args
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
         dtable = torch.empty_like(table) if ctx.needs_input_grad[3] else None
         if q.numel() == 0 or k.numel() == 0:
             return (dq.zero_(), dk.zero_(), dv.zero_(), None if dtable is None else dtable.zero_()) + (None,) * 7
