@@ -405,6 +405,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------- host side
+static_assert(sizeof(tcvom_attn_desc) == 664, "tcvom_amd/_lib.py: AttnDesc");
 int attn_check(const char* who, const tcvom_attn_desc* d, AttnArgs* a) {
     if (!d) return tcvom_fail(TCVOM_ERR_ARG, "%s: null description", who);
     TCVOM_CHECK_ARG(d->type == TCVOM_TYPE_BF16 || d->type == TCVOM_TYPE_F16, "%s: type %d", who, d->type);
@@ -426,8 +427,8 @@ int attn_check(const char* who, const tcvom_attn_desc* d, AttnArgs* a) {
     return 0;
 }
 
-// few queries: see attn_few_kernel; a single tile of 32 columns then serves all heads of a group
-static bool attn_few(const tcvom_attn_desc* d) { return d->Nq <= 32; }
+// few queries: attn_few_kernel, whose LDS holds the biases of up to 64 heads that share keys
+static bool attn_few(const tcvom_attn_desc* d) { return d->Nq <= 32 && d->H / d->Hkv <= 64; }
 static void few_shape(const tcvom_attn_desc* d, int* tiles, int* splits) {
     *tiles = cdiv((long long)d->H / d->Hkv * d->Nq, 32);
     const long long wgs = (long long)d->B * d->Hkv * *tiles;
@@ -447,8 +448,8 @@ extern "C" int64_t tcvom_attn_fwd_work(const tcvom_attn_desc* d) {
 
 template <class T, int DP>
 static void launch_fwd(AttnArgs a, const tcvom_attn_desc* d, hipStream_t st) {
-    const int last = line_reach(a.bk) + line_right(a.bk);
     if (attn_few(d) && !a.out_lo) {
+        const int last = line_reach(a.bk) + line_right(a.bk);
         few_shape(d, &a.tiles, &a.splits);
         const size_t lds = sizeof(float) * a.bk.num_buckets * (a.H / a.Hkv) + last + 1;
         const dim3 grid((unsigned)((long long)a.B * a.Hkv * a.tiles * a.splits));
@@ -471,8 +472,7 @@ extern "C" int tcvom_attn_fwd(const tcvom_attn_desc* d, const void* q, const voi
     if (d->B == 0 || d->Nq == 0) return 0;
     TCVOM_CHECK_ARG(q && table && out && (d->Nk == 0 || (k && v)), "attn_fwd: null tensor");
     TCVOM_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_lo), "attn_fwd: tensors start at multiples of 16 bytes");
-    TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 32) < (1LL << 30), "attn_fwd: too many queries for one launch");
-    TCVOM_CHECK_ARG(d->H / d->Hkv <= 64 || d->Nq > 32, "attn_fwd: %d heads share keys (at most 64)", d->H / d->Hkv);
+    TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 128) <= ATTN_MAX_WGS, "attn_fwd: %d sequences x %d heads x %d queries", d->B, d->H, d->Nq);
     TCVOM_CHECK_ARG(work_floats >= tcvom_attn_fwd_work(d) && (work || tcvom_attn_fwd_work(d) == 0), "attn_fwd: %lld floats of workspace",
                     (long long)work_floats);
     a.q = q; a.k = k; a.v = v; a.table = table; a.out = out; a.out_lo = out_lo; a.lse = lse; a.partial = work;

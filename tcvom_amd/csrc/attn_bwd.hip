@@ -514,9 +514,9 @@ extern "C" int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const voi
     TCVOM_CHECK_ARG(q && k && v && table && out && lse && dout && dout_stride && dq && dk && dv && work, "attn_bwd: null tensor");
     TCVOM_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_lo) && aligned16(dout) &&
                         aligned16(dq) && aligned16(dk) && aligned16(dv), "attn_bwd: tensors start at multiples of 16 bytes");
-    TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 32) < (1LL << 30) && (long long)d->B * d->Hkv * cdiv(d->Nk, 32) < (1LL << 30),
-                    "attn_bwd: too many rows for one launch");
-    TCVOM_CHECK_ARG(work_floats == tcvom_attn_bwd_work(d) && aligned16(work), "attn_bwd: %lld floats of workspace", (long long)work_floats);
+    TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 128) <= ATTN_MAX_WGS && (long long)d->B * d->H * cdiv(d->Nk, 128) <= ATTN_MAX_WGS,
+                    "attn_bwd: %d sequences x %d heads x %d queries, %d keys", d->B, d->H, d->Nq, d->Nk);
+    TCVOM_CHECK_ARG(work_floats >= tcvom_attn_bwd_work(d) && aligned16(work), "attn_bwd: %lld floats of workspace", (long long)work_floats);
     for (int n = 0; n < 3; ++n) {
         TCVOM_CHECK_ARG(dout_stride[n] % 8 == 0 && dout_stride[n] >= 0 && dout_stride[1] < (1 << 24), "attn_bwd: stride %lld of dout",
                         (long long)dout_stride[n]);
@@ -527,7 +527,7 @@ extern "C" int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const voi
     a.delta = work;
     a.part = work + (int64_t)d->B * d->H * d->Nq;
     a.apart = attn_apart(d);
-    if (a.apart) a.partial = work + work_floats - 2 * (int64_t)d->B * d->Nk * d->H * d->D;
+    if (a.apart) a.partial = work + tcvom_attn_bwd_work(d) - 2 * (int64_t)d->B * d->Nk * d->H * d->D;
     const hipStream_t st = (hipStream_t)stream;
     const int DP = attn_width(d->D);
     if (d->type == TCVOM_TYPE_BF16) {

@@ -24,12 +24,10 @@ from . import _lib as L
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _check_cuda(name, *tensors):
-    """Tensors (or None) of one GPU."""
+def _check_cuda(name, needed, *others):
+    """`needed`: a tuple of tensors, `others`: tensors or None; all of one GPU."""
     index = None
-    for t in tensors:
-        if t is None:
-            continue
+    for t in needed + tuple(t for t in others if t is not None):
         if not isinstance(t, torch.Tensor):
             raise TypeError('%s: expected a tensor, got %s' % (name, type(t).__name__))
         if not t.is_cuda:
@@ -146,7 +144,7 @@ def relative_position_bias(table, q_len, k_len, max_distance=128, bidirectional=
     |j - i - q_start|); one-sided: every key after the query counts as distance 0.  The first half of a side's buckets hold one
     distance each, the others grow geometrically up to max_distance (at most 1024), the last holds everything beyond.  q_start:
     position of the first query."""
-    _check_cuda('relative_position_bias', table)
+    _check_cuda('relative_position_bias', (table,))
     _check_table('relative_position_bias', table)
     if dtype not in _TYPES:
         raise TypeError('relative_position_bias: dtype %s' % dtype)
@@ -228,12 +226,12 @@ def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causa
     """softmax(scale q k^T + bias) v with bias = relative_position_bias(table, ...), never formed as a matrix: [B, Nq, H, D].
 
     q [B, Nq, H, D], k / v [B, Nk, Hkv, D], bf16 or fp16, D a multiple of 8 up to 128; H a multiple of Hkv (consecutive heads share
-    keys; at most 64 of them for 32 queries and fewer).  Any strides with contiguous rows of D; others are copied.
+    keys).  Any strides with contiguous rows of D; others are copied.
     table fp32 [buckets, H] and max_distance as in relative_position_bias; bidirectional: default not causal.
     scale: default D ** -0.5, positive.  Key j sits at position j, query i of sequence b at i + q_start[b] (an int, or int32 [B]).
     Query i sees key j if j < k_lens[b] (int32 [B]; clamped to 0..Nk), key_mask[b, j] (bool or uint8 [B, Nk]) and, causal,
     j <= i + q_start[b].  A query that sees nothing gives zeros and no gradient.  What lies behind the lengths or under the mask
-    may hold anything, NaN included.  For one new token against caches of Nk slots: k_lens = lengths with the new token,
+    may hold anything, NaN included (a NaN or inf that a later query sees can reach earlier ones of a causal call: 0 x inf).  For one new token against caches of Nk slots: k_lens = lengths with the new token,
     q_start = k_lens - 1, causal.
 
     Gradients of q, k, v and table.  Probabilities and their gradients are rounded to the 16-bit type as operands of the matrix
@@ -242,7 +240,7 @@ def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causa
     q_starts = None
     if isinstance(q_start, torch.Tensor):
         q_starts, q_start = q_start, 0
-    _check_cuda(name, q, k, v, table, k_lens, key_mask, q_starts)
+    _check_cuda(name, (q, k, v, table), k_lens, key_mask, q_starts)
     _check_table(name, table)
     if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError('%s: q, k, v are all bf16 or all fp16, got %s, %s, %s' % (name, q.dtype, k.dtype, v.dtype))
@@ -362,7 +360,7 @@ def block_norm(x, y, post_weight=None, post_bias=None, gate=None, branch_scale=1
 
     Gradients of every tensor argument."""
     name = 'block_norm'
-    _check_cuda(name, x, y, post_weight, post_bias, gate, pre_weight, pre_bias)
+    _check_cuda(name, (x,), y, post_weight, post_bias, gate, pre_weight, pre_bias)
     if kind not in ('rms', 'layer'):
         raise ValueError('%s: kind %r' % (name, kind))
     if x.dtype not in _TYPES or (y is not None and (y.dtype not in _TYPES or (y.dtype != x.dtype and x.dtype != torch.float32))):

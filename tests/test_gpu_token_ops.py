@@ -342,3 +342,308 @@ def test_attention_and_its_gradients(case, dt):
     again = torch.autograd.grad(ops.biased_attention(leaf['q'], leaf['k'], leaf['v'], leaf['table'], **kw), [leaf[n] for n in names], dout.to(DEV))
     for n, a in zip(names, again):
         assert torch.equal(got[n], a), n
+
+
+def test_attention_with_the_longest_line_and_the_most_buckets():
+    """The largest LDS footprints: width 128, reach 1024, 256 buckets, with the table's gradient; 64 and 128 heads on one key head."""
+    for c in (dict(B=1, Nq=130, Nk=2300, H=2, Hkv=2, D=128, buckets=256, far=1024), dict(B=1, Nq=33, Nk=1500, H=2, Hkv=1, D=64, buckets=256, far=1024),
+              dict(B=1, Nq=2, Nk=600, H=64, Hkv=1, D=128, buckets=256, far=1024), dict(B=1, Nq=1, Nk=300, H=128, Hkv=1, D=32)):
+        test_attention_and_its_gradients(c, torch.bfloat16)
+
+
+@pytest.mark.parametrize('nq', [1, 70])
+def test_attention_reads_any_strides(nq):
+    """Heads in front of tokens, slices of a fused projection, a cache shared by the batch (stride 0), rows that have to be copied."""
+    B, Nk, H, D = 2, 150, 4, 64
+    base = dict(B=B, Nq=nq, Nk=Nk, H=H, Hkv=H, D=D)
+    host, at, see, kw = attn_case(base, torch.bfloat16)
+    q, k, v, t = (host[n].to(DEV) for n in ('q', 'k', 'v', 'table'))
+    want = ops.biased_attention(q, k, v, t)
+    heads_first = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]
+    assert not heads_first[1].is_contiguous()
+    assert torch.equal(want, ops.biased_attention(*heads_first, t))
+    fused = torch.cat([k, v], -1)
+    assert torch.equal(want, ops.biased_attention(q, fused[..., :D], fused[..., D:], t))
+    odd = torch.empty(B, Nk, H, D + 3, dtype=k.dtype, device=DEV)
+    odd[..., 1:D + 1] = k
+    assert torch.equal(want, ops.biased_attention(q, odd[..., 1:D + 1], v, t))
+    last = k.permute(0, 1, 3, 2).contiguous().permute(0, 1, 3, 2)           # innermost stride not 1
+    assert torch.equal(want, ops.biased_attention(q, last, v, t))
+    one_k, one_v = k[:1].expand(B, -1, -1, -1), v[:1].expand(B, -1, -1, -1)
+    assert torch.equal(ops.biased_attention(q, one_k.contiguous(), one_v.contiguous(), t), ops.biased_attention(q, one_k, one_v, t))
+    # gradients of broadcast keys and of a transposed dout
+    leaf = k[:1].clone().requires_grad_(True)
+    full = k[:1].expand(B, -1, -1, -1).contiguous().requires_grad_(True)
+    dout = rnd(B, H, nq, D, seed=6).to(q.dtype).to(DEV).transpose(1, 2)
+    ga, = torch.autograd.grad(ops.biased_attention(q, leaf.expand(B, -1, -1, -1), v, t), leaf, dout)
+    gb, = torch.autograd.grad(ops.biased_attention(q, full, v, t), full, dout.contiguous())
+    close(ga, gb.double().cpu().sum(0, keepdim=True), step(q.dtype) * gb.double().cpu().sum(0, keepdim=True).abs() * 1.01 + 1e-7, 'broadcast keys')
+
+
+@pytest.mark.parametrize('nq', [1, 40])
+def test_attention_offsets_past_32_bits(nq):
+    """Tokens 2^17 elements apart: the last key is 2.6e9 elements (5 GB) behind the first."""
+    Nk, D, step_ = 20000, 64, 1 << 17
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip('needs 12 GB of device memory')
+    store = torch.empty(Nk * step_, dtype=torch.bfloat16, device=DEV)
+    k = store.as_strided((1, Nk, 1, D), (0, step_, D, 1))
+    v = store.as_strided((1, Nk, 1, D), (0, step_, D, 1), D)
+    k.copy_(rnd(1, Nk, 1, D, seed=1))
+    v.copy_(rnd(1, Nk, 1, D, seed=2))
+    q, t = rnd(1, nq, 2, D, seed=3).bfloat16().to(DEV), rnd(32, 2, seed=4).float().to(DEV)
+    kc, vc = k.contiguous(), v.contiguous()
+    assert torch.equal(ops.biased_attention(q, k, v, t, q_start=Nk - nq, causal=True), ops.biased_attention(q, kc, vc, t, q_start=Nk - nq, causal=True))
+    dout = rnd(1, nq, 2, D, seed=5).bfloat16().to(DEV)
+    grads = []
+    for kk, vv in ((k, v), (kc, vc)):
+        leaves = [x.detach().requires_grad_(True) for x in (q, kk, vv, t)]
+        grads.append(torch.autograd.grad(ops.biased_attention(*leaves, q_start=Nk - nq, causal=True), leaves, dout))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_empty_rows_ignore_their_gradient():
+    c = dict(B=3, Nq=65, Nk=130, H=2, Hkv=2, D=64, lens=[0, 1, 130], causal=True, start=[0, -30, -40])
+    host, at, see, kw = attn_case(c, torch.bfloat16)
+    dout = rnd(*host['q'].shape, seed=5).bfloat16()
+    empty = ~see.any(2)
+    assert empty.any() and not empty.all()
+    grads = []
+    for fill in (0.0, float('nan'), float('inf')):
+        leaves = [host[n].to(DEV).requires_grad_(True) for n in ('q', 'k', 'v', 'table')]
+        d = dout.clone()
+        d[empty] = fill
+        out = ops.biased_attention(*leaves, **kw)
+        assert not out[empty.to(DEV)].any()
+        grads.append(torch.autograd.grad(out, leaves, d.to(DEV)))
+    for g in grads[1:]:
+        assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(g, grads[0]))
+    assert not grads[0][0][empty.to(DEV)].any()
+
+
+@pytest.mark.parametrize('dt', HALF, ids=ids)
+def test_one_token_at_a_time_equals_the_whole_sequence(dt):
+    """A cache that grows by a token a call, against the causal call over all tokens: the same sums in other orders, each rounded as its
+    own call rounds (probabilities and results: 2 u each side)."""
+    N, H, Hkv, D = 300, 4, 2, 64
+    q, k, v, t = rnd(2, N, H, D, seed=1).to(dt), rnd(2, N, Hkv, D, seed=2).to(dt), rnd(2, N, Hkv, D, seed=3).to(dt), rnd(32, H, seed=4).float()
+    q, k, v, t = (x.to(DEV) for x in (q, k, v, t))
+    whole = ops.biased_attention(q, k, v, t, causal=True).double().cpu()
+    cache_k, cache_v = torch.full_like(k, float('nan')), torch.full_like(v, float('nan'))
+    at, see = bucket_matrix(32, 128, False, N, N, 0)[None], (torch.arange(N)[None] <= torch.arange(N)[:, None])[None]
+    p = attention64(q.double().cpu(), k.double().cpu(), v.double().cpu(), t.double().cpu(), at.expand(2, -1, -1), see.expand(2, -1, -1), D ** -0.5)[1]
+    spread = torch.einsum('bhij,bjhd->bihd', p, v.double().cpu().abs().repeat_interleave(H // Hkv, 2))
+    for i in range(N):
+        cache_k[:, i], cache_v[:, i] = k[:, i], v[:, i]
+        lens = torch.full((2,), i + 1, dtype=torch.int32, device=DEV)
+        one = ops.biased_attention(q[:, i:i + 1], cache_k, cache_v, t, causal=True, k_lens=lens, q_start=lens - 1)
+        u = step(dt)
+        close(one[:, 0], whole[:, i], 2 * (u * whole[:, i].abs() * 1.01 + (u + 2e-5) * spread[:, i] + 1e-7), str(i))
+
+
+# --------------------------------------------------------------------------------------------- together
+def _block(p, x, h, table, **kw):
+    """Attention block over tokens, as the operators are used together: h -> q, k, v -> attention -> projection -> norms."""
+    B, N, Cc = h.shape
+    H, D = table.shape[1], p['wq'].shape[1] // table.shape[1]
+    q, k, v = ((h @ p[n]).view(B, N, -1, D) for n in ('wq', 'wk', 'wv'))
+    y = ops.biased_attention(q, k, v, table, **kw).reshape(B, N, H * D) @ p['wo']
+    return ops.block_norm(x, y, post_weight=p['post'], gate=p['gate'], pre_weight=p['pre'], residual_scale=0.9)
+
+
+def test_two_blocks_together_against_64_bits():
+    """bias -> attention -> norms, twice, on a 32-bit residual stream: outputs and every gradient against the same program in 64 bits.
+    bf16 steps in the chain (h, q, k, v, attention, projection, twice; and their gradients): about 12 roundings of u = 2^-8 that add up as
+    independent errors, sqrt(12) u = 1.4 % of a result's size, four times that asked of the relative 2-norm."""
+    B, N, Cc, H, Hkv, D = 2, 150, 128, 4, 2, 32
+    dt = torch.bfloat16
+    names = dict(wq=(Cc, H * D), wk=(Cc, Hkv * D), wv=(Cc, Hkv * D), wo=(H * D, Cc))
+    host = [dict({n: (rnd(*s, seed=10 * l + i) * s[0] ** -0.5).to(dt) for i, (n, s) in enumerate(names.items())},
+                 post=1 + rnd(Cc, seed=10 * l + 5, std=0.1).float(), pre=1 + rnd(Cc, seed=10 * l + 6, std=0.1).float(),
+                 gate=0.5 + rnd(B, Cc, seed=10 * l + 7, std=0.2).float()) for l in range(2)]
+    tables = [rnd(32, H, seed=30 + l).float() for l in range(2)]
+    x0, w0 = rnd(B, N, Cc, seed=40).float(), 1 + rnd(Cc, seed=41, std=0.1).float()
+    lens = [N, 101]
+    target = rnd(B, N, Cc, seed=42)
+    dev = [{n: t.to(DEV).requires_grad_(True) for n, t in p.items()} for p in host]
+    dtab = [t.to(DEV).requires_grad_(True) for t in tables]
+    x, w = x0.to(DEV).requires_grad_(True), w0.to(DEV).requires_grad_(True)
+    h = ops.block_norm(x, None, pre_weight=w)[1].to(dt)
+    cur = x
+    for p, t in zip(dev, dtab):
+        cur, h = _block(p, cur, h, t, causal=True, k_lens=torch.tensor(lens, dtype=torch.int32, device=DEV))
+    ((cur * target.float().to(DEV)).sum() + (h.float() * target.float().to(DEV)).sum()).backward()
+
+    ref = [{n: t.double().requires_grad_(True) for n, t in p.items()} for p in host]
+    rtab = [t.double().requires_grad_(True) for t in tables]
+    rx, rw = x0.double().requires_grad_(True), w0.double().requires_grad_(True)
+    at = bucket_matrix(32, 128, False, N, N, 0)[None].expand(B, -1, -1)
+    i, j = torch.arange(N)[:, None], torch.arange(N)[None]
+    see = torch.stack([(j <= i) & (j < n) for n in lens])
+    rh = norm64(rx, None, None, None, None, 1, 1.0, 1.0, rw, None, False, 1e-6)[1]
+    rcur = rx
+    for p, t in zip(ref, rtab):
+        q, k, v = ((rh @ p[n]).view(B, N, -1, D) for n in ('wq', 'wk', 'wv'))
+        y = attention64(q, k, v, t, at, see, D ** -0.5)[0].reshape(B, N, H * D) @ p['wo']
+        rcur, rh = norm64(rcur, y, p['post'], None, p['gate'], N, 1.0, 0.9, p['pre'], None, False, 1e-6)
+    ((rcur * target).sum() + (rh * target).sum()).backward()
+
+    bound = 4 * math.sqrt(12) * 2.0 ** -8
+    pairs = [('x', cur, rcur), ('h', h, rh), ('dx', x.grad, rx.grad), ('dw0', w.grad, rw.grad)]
+    pairs += [('dtable%d' % l, dtab[l].grad, rtab[l].grad) for l in range(2)]
+    pairs += [('d%s%d' % (n, l), dev[l][n].grad, ref[l][n].grad) for l in range(2) for n in host[l]]
+    for name, g, r in pairs:
+        r = r.detach()
+        err = float((g.detach().double().cpu() - r).norm() / r.norm())
+        assert err < bound, '%s: %.4f' % (name, err)
+
+
+def test_norm_gradient_against_differences():
+    """fp32, along random directions, on the GPU itself: central differences of step 1e-2 (error of third order, about 1e-4 of the value,
+    and rounding 2^-24 x |loss| / 1e-2, about 1e-4)."""
+    shape, Cc = (3, 7, 96), 96
+    t = [rnd(*shape, seed=1), rnd(*shape, seed=2), 1 + rnd(Cc, seed=3, std=0.1), rnd(Cc, seed=4), 0.5 + rnd(3, Cc, seed=5, std=0.2), 1 + rnd(Cc, seed=6, std=0.1), rnd(Cc, seed=7)]
+    t = [x.float().to(DEV).requires_grad_(True) for x in t]
+    wa, wb = rnd(*shape, seed=8).to(DEV), rnd(*shape, seed=9).to(DEV)
+
+    def loss(t):
+        xo, h = ops.block_norm(t[0], t[1], t[2], t[3], t[4], 0.8, 1.1, t[5], t[6], 'layer')
+        return (xo.double() * wa).sum() + (h.double() * wb).sum()
+
+    grads = torch.autograd.grad(loss(t), t)
+    for n, g in enumerate(grads):
+        d = rnd(*t[n].shape, seed=20 + n).float().to(DEV)
+        with torch.no_grad():
+            e = 1e-2
+            up, down = (loss([x + s * e * d if i == n else x for i, x in enumerate(t)]) for s in (1, -1))
+        want, got = float((up - down) / (2 * e)), float((g.double() * d.double()).sum())
+        size = float((g.double() * d.double()).abs().sum())
+        assert abs(want - got) < 2e-3 * size + 1e-3, (n, want, got)
+
+
+def test_bias_and_attention_agree_on_the_buckets():
+    """The matrix of relative_position_bias added to plain logits gives what biased_attention gives."""
+    B, N, H, D = 1, 200, 2, 64
+    q, k, v, t = rnd(B, N, H, D, seed=1).half().to(DEV), rnd(B, N, H, D, seed=2).half().to(DEV), rnd(B, N, H, D, seed=3).half().to(DEV), rnd(32, H, seed=4).float().to(DEV)
+    bias = ops.relative_position_bias(t, N, N).double().cpu()
+    x = D ** -0.5 * torch.einsum('bihd,bjhd->bhij', q.double().cpu(), k.double().cpu()) + bias
+    p = torch.softmax(x, -1)
+    want = torch.einsum('bhij,bjhd->bihd', p, v.double().cpu())
+    spread = torch.einsum('bhij,bjhd->bihd', p, v.double().cpu().abs())
+    u = step(torch.float16)
+    close(ops.biased_attention(q, k, v, t), want, u * want.abs() * 1.01 + (u + 2e-5) * spread + 1e-7)
+
+
+# --------------------------------------------------------------------------------------------- streams, graphs, refusals
+def test_on_another_stream():
+    host, at, see, kw = attn_case(dict(B=2, Nq=1, Nk=3000, H=8, Hkv=2, D=64), torch.bfloat16)
+    dev = [host[n].to(DEV) for n in ('q', 'k', 'v', 'table')]
+    x, w = rnd(64, 512, seed=1).bfloat16().to(DEV), torch.ones(512, device=DEV)
+    want = (ops.biased_attention(*dev, **kw), ops.block_norm(x, x, post_weight=w, pre_weight=w)[1], ops.relative_position_bias(dev[3], 100, 100))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = (ops.biased_attention(*dev, **kw), ops.block_norm(x, x, post_weight=w, pre_weight=w)[1], ops.relative_position_bias(dev[3], 100, 100))
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_captured_calls_replay_on_new_inputs():
+    """Forward and gradients of all three in a graph, and a split single-token call in another one, replayed with eager work between."""
+    shape = dict(B=2, Nq=96, Nk=96, H=4, Hkv=2, D=64)
+    few = dict(B=2, Nq=1, Nk=4000, H=4, Hkv=2, D=64)
+
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        r = lambda *s: torch.randn(s, generator=g)  # noqa: E731
+        return dict(q=r(2, 96, 4, 64).bfloat16(), k=r(2, 96, 2, 64).bfloat16(), v=r(2, 96, 2, 64).bfloat16(), t=r(32, 4), x=r(2, 96, 256).float(),
+                    w1=1 + 0.1 * r(256), w2=1 + 0.1 * r(256), gate=r(2, 256), do=r(2, 96, 256).float(), dh=r(2, 96, 256).bfloat16(), db=r(4, 50, 60).float(),
+                    fq=r(2, 1, 4, 64).bfloat16(), fk=r(2, 4000, 2, 64).bfloat16(), fv=r(2, 4000, 2, 64).bfloat16())
+
+    def train(s):
+        leaves = [s[n].detach().requires_grad_(True) for n in ('q', 'k', 'v', 't', 'x', 'w1', 'w2', 'gate')]
+        q, k, v, t, x, w1, w2, gate = leaves
+        y = ops.biased_attention(q, k, v, t, causal=True).reshape(2, 96, 256)
+        xo, h = ops.block_norm(x, y, post_weight=w1, gate=gate, pre_weight=w2)
+        b = ops.relative_position_bias(t, 50, 60)
+        return (xo.detach(), h.detach(), b.detach()) + torch.autograd.grad([xo, h, b], leaves, [s['do'], s['dh'], s['db']])
+
+    def token(s):
+        with torch.no_grad():
+            return (ops.biased_attention(s['fq'], s['fk'], s['fv'], s['t'], causal=True, q_start=3999),)
+
+    static = {n: t.to(DEV) for n, t in inputs(0).items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            train(static)
+            token(static)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for f in (train, token):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = f(static)
+        graphs.append((g, out, f))
+    for seed in (1, 2, 3):
+        for n, t in inputs(seed).items():
+            static[n].copy_(t)
+        for g, out, _ in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for _, out, f in graphs:
+            want = f(static)                                   # eager, between the replays
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+        torch.cuda.synchronize()
+
+
+def test_refusals():
+    z = lambda *s, **k: torch.zeros(s, device=DEV, **k)  # noqa: E731
+    b16 = dict(dtype=torch.bfloat16)
+    q, k, t = z(2, 4, 4, 64, **b16), z(2, 6, 2, 64, **b16), z(32, 4)
+    bad = [(TypeError, dict(q=q.float())), (TypeError, dict(k=k.half())), (ValueError, dict(k=z(2, 6, 3, 64, **b16))), (ValueError, dict(k=z(3, 6, 2, 64, **b16))),
+           (ValueError, dict(k=z(2, 6, 2, 32, **b16))), (ValueError, dict(k=k[0])), (ValueError, dict(t=z(32, 2))), (ValueError, dict(t=z(32, 4, **b16))),
+           (ValueError, dict(t=z(31, 4))), (ValueError, dict(scale=0.0)), (ValueError, dict(scale=float('nan'))), (ValueError, dict(max_distance=2000)),
+           (ValueError, dict(k_lens=z(2, dtype=torch.int64))), (ValueError, dict(k_lens=z(3, dtype=torch.int32))), (ValueError, dict(q_start=z(1, dtype=torch.int32))),
+           (ValueError, dict(key_mask=z(2, 6))), (ValueError, dict(key_mask=z(2, 5, dtype=torch.bool))), (ValueError, dict(q_start=1 << 30)),
+           (RuntimeError, dict(k=k.cpu())), (RuntimeError, dict(k_lens=torch.zeros(2, dtype=torch.int32))), (TypeError, dict(q=None))]
+    for err, kw in bad:
+        a = dict(q=q, k=k, t=t)
+        a.update({n: kw.pop(n) for n in list(kw) if n in a})
+        with pytest.raises(err):
+            ops.biased_attention(a['q'], a['k'], a['k'], a['t'], **kw)
+    for D in (4, 60, 136):
+        with pytest.raises(ValueError):
+            ops.biased_attention(z(1, 2, 2, D, **b16), z(1, 2, 2, D, **b16), z(1, 2, 2, D, **b16), z(32, 2))
+    with pytest.raises(ValueError):
+        ops.relative_position_bias(t, -1, 4)
+    with pytest.raises(TypeError):
+        ops.relative_position_bias(t, 4, 4, dtype=torch.float64)
+    x, w = z(2, 3, 64), torch.ones(64, device=DEV)
+    for err, a, kw in [(ValueError, (x, x), dict(kind='batch')), (TypeError, (x.double(), x), {}), (TypeError, (x.bfloat16(), x), {}), (TypeError, (x.bfloat16(), x.half()), {}),
+                       (ValueError, (x, x[:1]), {}), (ValueError, (x, x), dict(post_weight=w[:32])), (TypeError, (x, x), dict(gate=w.half())),
+                       (ValueError, (x, x), dict(post_weight=w.half())), (ValueError, (x, x), dict(post_bias=w)), (ValueError, (x, x), dict(pre_weight=w, pre_bias=w)),
+                       (ValueError, (x, x), dict(gate=z(3, 64))), (ValueError, (x, x), dict(gate=z(2, 3, 1))), (ValueError, (x, None), {}),
+                       (ValueError, (x, None), dict(pre_weight=w, gate=w)), (ValueError, (x, None), dict(pre_weight=w, residual_scale=0.5)),
+                       (ValueError, (z(2, 8200), z(2, 8200)), {}), (ValueError, (z(2, 0), z(2, 0)), {}), (TypeError, (None, x), {})]:
+        with pytest.raises(err):
+            ops.block_norm(*a, **kw)
+
+
+def test_second_derivatives_are_refused():
+    x, w = rnd(4, 64, seed=1).float().to(DEV).requires_grad_(True), torch.ones(64, device=DEV)
+    xo, h = ops.block_norm(x, x, pre_weight=w)
+    g, = torch.autograd.grad(h.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), x)
+
+
+def test_norm_of_no_tokens():
+    x = torch.zeros(0, 64, device=DEV, requires_grad=True)
+    w = torch.ones(64, device=DEV, requires_grad=True)
+    xo, h = ops.block_norm(x, torch.zeros(0, 64, device=DEV), post_weight=w, pre_weight=w.detach())
+    assert xo.shape == h.shape == (0, 64)
+    gx, gw = torch.autograd.grad([xo, h], [x, w], [torch.zeros_like(xo), torch.zeros_like(h)])
+    assert gx.shape == (0, 64) and not gw.any()
