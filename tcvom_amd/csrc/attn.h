@@ -49,7 +49,7 @@ struct AttnArgs {
     float* lse;                              // [B][H][Nq], base 2, -inf for a row without a key
     const void* dout;
     void *dq, *dk, *dv;
-    float *delta, *part;                     // backward: <dout, out> of every row; bucket sums of every workgroup
+    float *delta, *part, *dtable;            // backward: <dout, out> of every row; bucket sums of every workgroup; their result or null
     float* partial;                          // forward: the splits' outputs; backward: each head's dk and dv where a group is taken apart
     const int *k_lens, *q_starts;            // [B] or null
     const unsigned char* key_mask;           // [B][Nk] or null
@@ -74,8 +74,8 @@ __device__ __forceinline__ int seq_start(const AttnArgs& a, int b) {
 // workgroup -> (sequence and head, tile).  The hardware deals workgroups round-robin over the 8 XCDs, each with its own L2: the tiles of a
 // head, which share keys and values (or queries), stay on one.  Tiles of causal heads differ in work: all heads' longest ones go
 // first, so that none starts late (2 x 4080 tokens, 16 heads of 128: see attn_dkv_kernel); otherwise head by head, the fewest heads in an L2.
-__device__ __forceinline__ void work_item(const AttnArgs& a, int heads, int& bh, int& tile) {
-    const int id = blockIdx.x, total = gridDim.x;
+__device__ __forceinline__ void work_item(const AttnArgs& a, int id, int heads, int& bh, int& tile) {
+    const int total = heads * a.tiles;
     if (a.causal && heads % 8 == 0) {
         tile = id / heads;
         bh = id % heads;

@@ -17,7 +17,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
     float* line = line_ + MARGIN;
 
     int bh, tile;
-    work_item(a, a.B * a.H, bh, tile);
+    work_item(a, blockIdx.x, a.B * a.H, bh, tile);
     if (a.causal) tile = a.tiles - 1 - tile;
     const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
     const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5, col = lane & 31;

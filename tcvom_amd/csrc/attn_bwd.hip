@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     float* line = line_ + MARGIN;
 
     int bh, tile;
-    work_item(a, a.B * a.H, bh, tile);
+    work_item(a, blockIdx.x, a.B * a.H, bh, tile);
     if (a.causal) tile = a.tiles - 1 - tile;
     const int b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
     const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5, col = lane & 31;
@@ -214,19 +214,21 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     }
 }
 
-// dtable[n][h] = sum over the workgroups of head h, in 64 bits: a workgroup a head, 1024 threads = buckets x slices of the workgroups
-__global__ __launch_bounds__(1024) void attn_table_kernel(const float* part, float* dtable, int buckets, int H, long long parts) {
-    __shared__ double red[1024];
-    const int h = blockIdx.x, slices = 1024 / buckets, n = threadIdx.x % buckets, s = threadIdx.x / buckets;
+// dtable[n][h] = sum over the workgroups of head h of attn_dq_kernel, in 64 bits, by a workgroup a head: 256 threads = buckets x slices of
+// those workgroups.  The first workgroups of the dk / dv launch, which runs after that kernel.
+__device__ __forceinline__ void sum_table(const AttnArgs& a, int h, double* red) {
+    const int buckets = a.bk.num_buckets, slices = 256 / buckets, n = threadIdx.x % buckets, s = threadIdx.x / buckets;
+    const long long parts = (long long)a.B * ((a.Nq + 127) / 128);
     double t = 0.;
     if (s < slices)
-        for (long long i = s; i < parts; i += slices) t += (double)part[(h * parts + i) * buckets + n];
+#pragma unroll 4
+        for (long long i = s; i < parts; i += slices) t += (double)a.part[(h * parts + i) * buckets + n];
     red[threadIdx.x] = t;
     __syncthreads();
-    if (threadIdx.x >= buckets) return;
+    if ((int)threadIdx.x >= buckets) return;
     t = 0.;
     for (int i = 0; i < slices; ++i) t += red[i * buckets + threadIdx.x];
-    dtable[threadIdx.x * H + h] = (float)t;
+    a.dtable[threadIdx.x * a.H + h] = (float)t;
 }
 
 // ---- dk, dv: a wave owns 32 keys of one key head, the workgroup (128 keys) walks the queries of every head that shares them, 32 at a
@@ -247,10 +249,15 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     __shared__ __align__(16) float ls[4][QT], ld[4][QT];    // log-sums and deltas of the tiles: written two tiles ahead
     extern __shared__ float line_[];
     float* line = line_ + MARGIN;
+    const int extra = a.dtable ? a.H : 0;
+    if ((int)blockIdx.x < extra) {
+        sum_table(a, blockIdx.x, reinterpret_cast<double*>(lq));
+        return;
+    }
 
     const int heads = a.apart ? a.H : a.Hkv, G = a.apart ? 1 : a.H / a.Hkv;      // of the grid, and of a workgroup
     int bh, tile;
-    work_item(a, a.B * heads, bh, tile);
+    work_item(a, blockIdx.x - extra, a.B * heads, bh, tile);
     const int b = bh / heads, h0 = bh % heads * G, hk = h0 / (a.H / a.Hkv);
     const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5, col = lane & 31;
     const int start = seq_start(a, b), len = seq_keys(a, b);
@@ -476,27 +483,17 @@ static bool attn_apart(const tcvom_attn_desc* d) {
 }
 
 template <class T, int DP>
-static int launch_bwd(AttnArgs a, float* dtable, hipStream_t st) {
-    if (a.Nq > 0) {
-        a.tiles = cdiv(a.Nq, 128);
-        const dim3 grid((unsigned)((long long)a.B * a.H * a.tiles));
-        if (dtable) {
-            hipLaunchKernelGGL((attn_dq_kernel<T, DP, true>), grid, dim3(256), 5 * line_bytes(a), st, a);
-            hipLaunchKernelGGL(attn_table_kernel, dim3(a.H), dim3(1024), 0, st, a.part, dtable, a.bk.num_buckets, a.H, (long long)a.B * a.tiles);
-        } else {
-            hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), line_bytes(a), st, a);
-        }
-    }
-    if (a.Nk > 0) {
-        a.tiles = cdiv(a.Nk, 128);
-        const unsigned wgs = (unsigned)((long long)a.B * (a.apart ? a.H : a.Hkv) * a.tiles);
-        hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3(wgs), dim3(256), line_bytes(a), st, a);
-        if (a.apart) {
-            const dim3 grid(cdiv((long long)a.B * a.Nk * a.Hkv * (a.D / 4), 256), 2);
-            hipLaunchKernelGGL(attn_heads_kernel<T>, grid, dim3(256), 0, st, a);
-        }
-    }
-    return 0;
+static void launch_bwd(AttnArgs a, float* dtable, hipStream_t st) {
+    a.tiles = cdiv(a.Nq, 128);
+    const dim3 grid((unsigned)((long long)a.B * a.H * a.tiles));
+    if (dtable) hipLaunchKernelGGL((attn_dq_kernel<T, DP, true>), grid, dim3(256), 5 * line_bytes(a), st, a);
+    else hipLaunchKernelGGL((attn_dq_kernel<T, DP, false>), grid, dim3(256), line_bytes(a), st, a);
+    a.tiles = cdiv(a.Nk, 128);
+    a.dtable = dtable;
+    const long long wgs = (long long)a.B * (a.apart ? a.H : a.Hkv) * a.tiles + (dtable ? a.H : 0);
+    hipLaunchKernelGGL((attn_dkv_kernel<T, DP>), dim3((unsigned)wgs), dim3(256), line_bytes(a), st, a);
+    if (a.apart)
+        hipLaunchKernelGGL(attn_heads_kernel<T>, dim3(cdiv((long long)a.B * a.Nk * a.Hkv * (a.D / 4), 256), 2), dim3(256), 0, st, a);
 }
 
 extern "C" int64_t tcvom_attn_bwd_work(const tcvom_attn_desc* d) {

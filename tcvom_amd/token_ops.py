@@ -27,16 +27,19 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 def _check_cuda(name, needed, *others):
     """`needed`: a tuple of tensors, `others`: tensors or None; all of one GPU."""
     index = None
-    for t in needed + tuple(t for t in others if t is not None):
+    for n, t in enumerate(needed + others):
+        if t is None and n >= len(needed):
+            continue
         if not isinstance(t, torch.Tensor):
             raise TypeError('%s: expected a tensor, got %s' % (name, type(t).__name__))
-        if not t.is_cuda:
-            raise RuntimeError('tcvom_amd ops run on the GPU through libtcvom_hip.so only (no CPU fallback); %s got a %s tensor'
-                               % (name, t.device))
         i = t.get_device()
-        if index is not None and i != index:
-            raise RuntimeError('%s: tensors on cuda:%d and cuda:%d' % (name, index, i))
-        index = i
+        if i != index:
+            if i < 0:
+                raise RuntimeError('tcvom_amd ops run on the GPU through libtcvom_hip.so only (no CPU fallback); %s got a %s tensor'
+                                   % (name, t.device))
+            if index is not None:
+                raise RuntimeError('%s: tensors on cuda:%d and cuda:%d' % (name, index, i))
+            index = i
 
 
 def _c(t):
@@ -70,7 +73,11 @@ def _first_order(backward):
 
 def _tracked(*tensors):
     """Whether autograd has to see the call."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # =============================================================================================
@@ -332,20 +339,19 @@ class _BlockNorm(torch.autograd.Function):
         return dx, dy, dw1, db1, dg, dw2, db2, None, None, None, None, None
 
 
-def _gate_rows(x, gate):
-    """Tokens that share a row of the gate."""
-    lead = x.shape[:-1]
-    g = tuple(gate.shape[:-1])
-    if gate.shape[-1:] != x.shape[-1:]:
-        raise ValueError('block_norm: a gate of %s for %s' % (tuple(gate.shape), tuple(x.shape)))
-    g = g + (1,) * (len(lead) - len(g))
+def _gate_rows(shape, gate):
+    """Tokens that share a row of the gate, from the shapes."""
+    lead, g = shape[:-1], gate[:-1]
     n = len(g)
-    while n and g[n - 1] == 1:
+    while n and g[n - 1] == 1 and lead[n - 1:n] != (1,):
         n -= 1
-    if len(g) != len(lead) or g[:n] != tuple(lead[:n]):
+    if len(gate) == 0 or gate[-1] != shape[-1] or len(g) > len(lead) or g[:n] != lead[:n]:
         raise ValueError('block_norm: a gate of %s for %s: one of each channel, of each leading index, or of each token'
-                         % (tuple(gate.shape), tuple(x.shape)))
-    return max(math.prod(lead[n:]), 1)
+                         % (tuple(gate), tuple(shape)))
+    rows = max(math.prod(lead[n:]), 1)
+    if rows > 1 and math.prod(lead[:n]) > 32768:
+        raise ValueError('block_norm: %d gate rows of several tokens (at most 32768)' % math.prod(lead[:n]))
+    return rows
 
 
 def block_norm(x, y, post_weight=None, post_bias=None, gate=None, branch_scale=1.0, residual_scale=1.0, pre_weight=None, pre_bias=None,
@@ -363,29 +369,32 @@ def block_norm(x, y, post_weight=None, post_bias=None, gate=None, branch_scale=1
     _check_cuda(name, (x,), y, post_weight, post_bias, gate, pre_weight, pre_bias)
     if kind not in ('rms', 'layer'):
         raise ValueError('%s: kind %r' % (name, kind))
-    if x.dtype not in _TYPES or (y is not None and (y.dtype not in _TYPES or (y.dtype != x.dtype and x.dtype != torch.float32))):
-        raise TypeError('%s: x %s, y %s' % (name, x.dtype, None if y is None else y.dtype))
-    if x.dim() < 1 or not 0 < x.shape[-1] <= L.MAX_NORM_CHANNELS:
-        raise ValueError('%s: %s (1..%d channels)' % (name, tuple(x.shape), L.MAX_NORM_CHANNELS))
+    x_type, shape = x.dtype, x.shape
+    y_type = x_type if y is None else y.dtype
+    if x_type not in _TYPES or y_type not in _TYPES or (y_type != x_type and x_type != torch.float32):
+        raise TypeError('%s: x %s, y %s' % (name, x_type, y_type))
+    channels = shape[-1] if shape else 0
+    if not 0 < channels <= L.MAX_NORM_CHANNELS:
+        raise ValueError('%s: %s (1..%d channels)' % (name, tuple(shape), L.MAX_NORM_CHANNELS))
     if y is None:
         if pre_weight is None or post_weight is not None or post_bias is not None or gate is not None or residual_scale != 1.0:
             raise ValueError('%s: without y there is the pre norm only' % name)
-    elif y.shape != x.shape:
-        raise ValueError('%s: x %s, y %s' % (name, tuple(x.shape), tuple(y.shape)))
-    for w, b, what in ((post_weight, post_bias, 'post'), (pre_weight, pre_bias, 'pre')):
-        for t in (w, b):
-            if t is not None and (t.dtype != torch.float32 or t.shape != x.shape[-1:]):
-                raise ValueError('%s: the %s weight and bias are fp32 [%d], got %s %s' % (name, what, x.shape[-1], t.dtype, tuple(t.shape)))
-        if b is not None and (w is None or kind != 'layer'):
-            raise ValueError('%s: a %s bias goes with LayerNorm and a weight' % (name, what))
+    elif y.shape != shape:
+        raise ValueError('%s: x %s, y %s' % (name, tuple(shape), tuple(y.shape)))
+    for t in (post_weight, post_bias, pre_weight, pre_bias):
+        if t is not None and (t.dtype != torch.float32 or t.dim() != 1 or t.size(0) != channels):
+            raise ValueError('%s: weights and biases are fp32 [%d], got %s %s' % (name, channels, t.dtype, tuple(t.shape)))
+    if (post_bias is not None and (post_weight is None or kind != 'layer')) or (pre_bias is not None and (pre_weight is None or kind != 'layer')):
+        raise ValueError('%s: a bias goes with LayerNorm and a weight' % name)
     rows = 1
     if gate is not None:
-        if gate.dtype not in (torch.float32, y.dtype):
-            raise TypeError('%s: gate %s with y %s' % (name, gate.dtype, y.dtype))
-        rows = _gate_rows(x, gate)
-        if rows > 1 and x.numel() // x.shape[-1] // rows > 32768:
-            raise ValueError('%s: %d gate rows of several tokens (at most 32768)' % (name, x.numel() // x.shape[-1] // rows))
+        if gate.dtype != torch.float32 and gate.dtype != y_type:
+            raise TypeError('%s: gate %s with y %s' % (name, gate.dtype, y_type))
+        rows = _gate_rows(shape, gate.shape)
     args = (rows, float(branch_scale), float(residual_scale), float(eps), int(kind == 'layer'))
     tensors = (x, y, post_weight, post_bias, gate, pre_weight, pre_bias)
-    xo, h = _BlockNorm.apply(*tensors, *args) if _tracked(*tensors) else _block_norm(*(_c(t) for t in tensors), False, *args)[:2]
+    if _tracked(*tensors):
+        xo, h = _BlockNorm.apply(*tensors, *args)
+    else:
+        xo, h, _ = _block_norm(*[_c(t) for t in tensors], False, *args)
     return (x if y is None else xo), h
