@@ -432,8 +432,8 @@ static bool attn_few(const tcvom_attn_desc* d) { return d->Nq <= 32 && d->H / d-
 static void few_shape(const tcvom_attn_desc* d, int* tiles, int* splits) {
     *tiles = cdiv((long long)d->H / d->Hkv * d->Nq, 32);
     const long long wgs = (long long)d->B * d->Hkv * *tiles;
-    // two workgroups a CU, and at least 256 keys a workgroup
-    long long s = wgs ? 512 / wgs : 1;
+    // a workgroup a CU (two: 1 to 10 % slower), and at least 256 keys a workgroup
+    long long s = wgs ? 256 / wgs : 1;
     const long long most = d->Nk / 256;
     if (s > most) s = most;
     *splits = (int)(s < 1 ? 1 : s > 256 ? 256 : s);

@@ -80,7 +80,7 @@ extern "C" int tcvom_relbias_fwd(const float* table, void* out, const tcvom_rel_
 // past the two ends of the line, which is most of a long matrix, with 16-byte loads.  Each sum is made by one thread, or by a tree of
 // fixed shape, and written once: no atomics, equal calls give equal bits.
 constexpr int BIAS_ROWS = 16;
-template <class T>
+template <class T, int LANES>
 __global__ __launch_bounds__(256) void relbias_bwd_kernel(const T* dout, float* part, tcvom_rel_buckets bk, long long Nq, long long Nk,
                                                           long long q_start) {
     __shared__ float red[2][4];
@@ -105,39 +105,41 @@ __global__ __launch_bounds__(256) void relbias_bwd_kernel(const T* dout, float* 
         out[t] = s[0];
         return;
     }
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    // a row to LANES lanes: 16 rows at once while they are short
+    const int lane = threadIdx.x % LANES;
     float side[2] = {0.f, 0.f};
-    for (long long i = i0 + wave; i < i1; i += 4) {
+    for (long long i = i0 + threadIdx.x / LANES; i < i1; i += 256 / LANES) {
         const T* row = plane + i * Nk;
         // keys with line index <= 0 are j < jl, with index >= last j >= jr (last > 0)
-        long long jl = i + q_start - reach + 1, jr = i + q_start - reach + last;
-        jl = jl < 0 ? 0 : jl > Nk ? Nk : jl;
-        jr = jr < 0 ? 0 : jr > Nk ? Nk : jr;
-        // both sides together, four vectors of each in flight
+        const long long jl = min(max(i + q_start - reach + 1, 0LL), Nk), jr = min(max(i + q_start - reach + last, 0LL), Nk);
+        // of each side: up to V - 1 elements to a 16-byte boundary, vectors, up to V - 1 more; both sides and four vectors each at once
         const T* vec[2];
         int nv[2];
+        T edge[2][2];
+        bool in[2][2];
         float s[2][V];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             const long long ja = w ? jr : 0, jb = w ? Nk : jl;
-            long long head = ((16 - ((uintptr_t)(row + ja) & 15)) & 15) / sizeof(T);
-            if (head > jb - ja) head = jb - ja;
+            const long long head = min((long long)(((16 - ((uintptr_t)(row + ja) & 15)) & 15) / sizeof(T)), jb - ja);
             nv[w] = (int)((jb - ja - head) / V);
             vec[w] = row + ja + head;
+            const long long j = ja + head + (long long)nv[w] * V + lane;
+            in[w][0] = lane < head;
+            in[w][1] = j < jb;
+            edge[w][0] = row[in[w][0] ? ja + lane : 0];
+            edge[w][1] = row[in[w][1] ? j : 0];
 #pragma unroll
             for (int u = 0; u < V; ++u) s[w][u] = 0.f;
-            if (lane < head) s[w][0] = (float)row[ja + lane];
-            const long long j = ja + head + (long long)nv[w] * V + lane;
-            if (j < jb) s[w][V - 1] += (float)row[j];
         }
-        for (int n = lane; n < max(nv[0], nv[1]); n += 256) {
+        for (int n = lane; n < max(nv[0], nv[1]); n += 4 * LANES) {
             typename RawVec<T, V>::type f[2][4];
 #pragma unroll
             for (int w = 0; w < 2; ++w)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     f[w][k] = (typename RawVec<T, V>::type)(T)0.f;
-                    if (n + 64 * k < nv[w]) f[w][k] = load_raw<T, V>(vec[w] + (long long)(n + 64 * k) * V);
+                    if (n + LANES * k < nv[w]) f[w][k] = load_raw<T, V>(vec[w] + (long long)(n + LANES * k) * V);
                 }
 #pragma unroll
             for (int w = 0; w < 2; ++w)
@@ -148,6 +150,8 @@ __global__ __launch_bounds__(256) void relbias_bwd_kernel(const T* dout, float* 
         }
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
+            s[w][0] += in[w][0] ? (float)edge[w][0] : 0.f;
+            s[w][1] += in[w][1] ? (float)edge[w][1] : 0.f;
 #pragma unroll
             for (int o = V / 2; o > 0; o >>= 1)
 #pragma unroll
@@ -158,7 +162,7 @@ __global__ __launch_bounds__(256) void relbias_bwd_kernel(const T* dout, float* 
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
         const float t = wave_sum(side[w]);
-        if (lane == 0) red[w][wave] = t;
+        if ((threadIdx.x & 63) == 0) red[w][threadIdx.x >> 6] = t;
     }
     __syncthreads();
     if (threadIdx.x < 2) out[threadIdx.x ? last : 0] = (red[threadIdx.x][0] + red[threadIdx.x][1]) + (red[threadIdx.x][2] + red[threadIdx.x][3]);
@@ -201,12 +205,19 @@ extern "C" int tcvom_relbias_bwd(const void* dout, float* dtable, float* work, i
     const int last = line_reach(*buckets) + line_right(*buckets), chunks = cdiv(q_len, BIAS_ROWS);
     const dim3 grid(cdiv(last - 1, 256) + 1, chunks, heads);
     const hipStream_t st = (hipStream_t)stream;
-    if (type == TCVOM_TYPE_F32)
-        hipLaunchKernelGGL(relbias_bwd_kernel<float>, grid, dim3(256), 0, st, (const float*)dout, work, bk, q_len, k_len, q_start);
-    else if (type == TCVOM_TYPE_BF16)
-        hipLaunchKernelGGL(relbias_bwd_kernel<__bf16>, grid, dim3(256), 0, st, (const __bf16*)dout, work, bk, q_len, k_len, q_start);
-    else
-        hipLaunchKernelGGL(relbias_bwd_kernel<_Float16>, grid, dim3(256), 0, st, (const _Float16*)dout, work, bk, q_len, k_len, q_start);
+#define RELBIAS_BWD(T, LANES) \
+    hipLaunchKernelGGL((relbias_bwd_kernel<T, LANES>), grid, dim3(256), 0, st, (const T*)dout, work, bk, q_len, k_len, q_start)
+    // 8 x 1024 x 1024 bf16: 7.0 us with 16 lanes a row, 11.5 us with a wave; 16 x 4000 x 64: 20 and 58; rows of 6 KB and more: the same
+    if (k_len * (type == TCVOM_TYPE_F32 ? 4 : 2) <= 4096) {
+        if (type == TCVOM_TYPE_F32) RELBIAS_BWD(float, 16);
+        else if (type == TCVOM_TYPE_BF16) RELBIAS_BWD(__bf16, 16);
+        else RELBIAS_BWD(_Float16, 16);
+    } else {
+        if (type == TCVOM_TYPE_F32) RELBIAS_BWD(float, 64);
+        else if (type == TCVOM_TYPE_BF16) RELBIAS_BWD(__bf16, 64);
+        else RELBIAS_BWD(_Float16, 64);
+    }
+#undef RELBIAS_BWD
     TCVOM_LAUNCH_CHECK("relbias_bwd");
     hipLaunchKernelGGL(relbias_table_kernel, dim3(buckets->num_buckets, heads), dim3(256), 0, st, work, dtable, bk, heads, chunks);
     TCVOM_LAUNCH_CHECK("relbias_table");
