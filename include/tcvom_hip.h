@@ -720,17 +720,17 @@ typedef struct {
     const uint8_t* key_mask;
     tcvom_rel_buckets buckets;
 } tcvom_attn_desc;
-/* lse (or NULL): fp32 [B][H][Nq], log2 of the row's sum of exponentials, -inf for an empty row.  out_lo (or NULL): what rounding out to
- * 16 bits dropped, in 16 bits; asking for it also carries the probabilities in twice the bits (the backward's <dout, out> then is
- * good to 2^-16, which the table's gradient, a sum of differences, needs).  work: tcvom_attn_fwd_work floats. */
+/* lse (or NULL): fp32 [B][H][Nq], log2 of the row's sum of exponentials, -inf for an empty row.  out32 (or NULL): out before it is
+ * rounded to 16 bits; asking for it also carries the probabilities in twice the bits (the backward's <dout, out> then is good to 2^-17,
+ * which the table's gradient, a sum of differences, needs).  work: tcvom_attn_fwd_work floats. */
 int64_t tcvom_attn_fwd_work(const tcvom_attn_desc* d);
-int tcvom_attn_fwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, void* out, void* out_lo,
+int tcvom_attn_fwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, void* out, float* out32,
                    float* lse, float* work, int64_t work_floats, void* stream);
 /* Gradients from what the forward read and wrote (lse required); dout with strides like q's; dq / dk / dv contiguous, dtable (or NULL:
  * not asked for) fp32 like table.  Keys and rows without a pair get zeros.  Fixed order of additions. */
 int64_t tcvom_attn_bwd_work(const tcvom_attn_desc* d);
 int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, const void* out,
-                   const void* out_lo, const float* lse, const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv,
+                   const float* out32, const float* lse, const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv,
                    float* dtable, float* work, int64_t work_floats, void* stream);
 
 /* Norms around a block, T tokens of C <= 8192 channels, contiguous:

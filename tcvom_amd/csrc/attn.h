@@ -45,7 +45,8 @@ constexpr int KT = 64;                       // keys a tile
 struct AttnArgs {
     const void *q, *k, *v;
     const float* table;                      // [buckets][H]
-    void *out, *out_lo;                      // [B][Nq][H][D]; out_lo: out's rounding error in 16 bits (training), or null
+    void* out;                               // [B][Nq][H][D]
+    float* out32;                            // ... before it is rounded, for the backward, or null
     float* lse;                              // [B][H][Nq], base 2, -inf for a row without a key
     const void* dout;
     void *dq, *dk, *dv;

@@ -149,15 +149,15 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
         for (int g = 0; g < 4; ++g) {
             const int at = d * 32 + g * 8 + half * 4;
             if (at >= a.D) continue;
-            typename Mma<T>::v4 w, lo;
+            typename Mma<T>::v4 w;
+            f32x4_t f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float f = empty_or(sum, o[d][4 * g + j] * inv);
-                w[j] = (T)f;
-                lo[j] = (T)(f - (float)w[j]);
+                f[j] = empty_or(sum, o[d][4 * g + j] * inv);
+                w[j] = (T)f[j];
             }
             *reinterpret_cast<typename Mma<T>::v4*>((T*)a.out + row * a.D + at) = w;
-            if (LO) *reinterpret_cast<typename Mma<T>::v4*>((T*)a.out_lo + row * a.D + at) = lo;
+            if (LO) *reinterpret_cast<f32x4_t*>(a.out32 + row * a.D + at) = f;
         }
     if (a.lse && half == 0) a.lse[((long long)b * a.H + h) * a.Nq + qi] = sum == 0.f ? -INFINITY : m + log2f(sum) - Mma<T>::shift;
 }
@@ -448,7 +448,7 @@ extern "C" int64_t tcvom_attn_fwd_work(const tcvom_attn_desc* d) {
 
 template <class T, int DP>
 static void launch_fwd(AttnArgs a, const tcvom_attn_desc* d, hipStream_t st) {
-    if (attn_few(d) && !a.out_lo) {
+    if (attn_few(d) && !a.out32) {
         const int last = line_reach(a.bk) + line_right(a.bk);
         few_shape(d, &a.tiles, &a.splits);
         const size_t lds = sizeof(float) * a.bk.num_buckets * (a.H / a.Hkv) + last + 1;
@@ -461,21 +461,21 @@ static void launch_fwd(AttnArgs a, const tcvom_attn_desc* d, hipStream_t st) {
     a.tiles = cdiv(a.Nq, 128);
     const dim3 grid((unsigned)((long long)a.B * a.H * a.tiles));
     const size_t lds = line_bytes(a);
-    if (a.out_lo) hipLaunchKernelGGL((attn_fwd_kernel<T, DP, true>), grid, dim3(256), lds, st, a);
+    if (a.out32) hipLaunchKernelGGL((attn_fwd_kernel<T, DP, true>), grid, dim3(256), lds, st, a);
     else hipLaunchKernelGGL((attn_fwd_kernel<T, DP, false>), grid, dim3(256), lds, st, a);
 }
 
 extern "C" int tcvom_attn_fwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, void* out,
-                              void* out_lo, float* lse, float* work, int64_t work_floats, void* stream) {
+                              float* out32, float* lse, float* work, int64_t work_floats, void* stream) {
     AttnArgs a;
     if (const int rc = attn_check("attn_fwd", d, &a)) return rc;
     if (d->B == 0 || d->Nq == 0) return 0;
     TCVOM_CHECK_ARG(q && table && out && (d->Nk == 0 || (k && v)), "attn_fwd: null tensor");
-    TCVOM_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_lo), "attn_fwd: tensors start at multiples of 16 bytes");
+    TCVOM_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out32), "attn_fwd: tensors start at multiples of 16 bytes");
     TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 128) <= ATTN_MAX_WGS, "attn_fwd: %d sequences x %d heads x %d queries", d->B, d->H, d->Nq);
     TCVOM_CHECK_ARG(work_floats >= tcvom_attn_fwd_work(d) && (work || tcvom_attn_fwd_work(d) == 0), "attn_fwd: %lld floats of workspace",
                     (long long)work_floats);
-    a.q = q; a.k = k; a.v = v; a.table = table; a.out = out; a.out_lo = out_lo; a.lse = lse; a.partial = work;
+    a.q = q; a.k = k; a.v = v; a.table = table; a.out = out; a.out32 = out32; a.lse = lse; a.partial = work;
     const hipStream_t st = (hipStream_t)stream;
     const int DP = attn_width(d->D);
     if (d->type == TCVOM_TYPE_BF16) {

@@ -64,10 +64,13 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
         const bool ok = qi < a.Nq && d < a.D;
         qf[s] = load_or_zero<v8>(ok, Q + (long long)qi * a.qs[1] + d);
         gf[s] = load_or_zero<v8>(ok, dO + (long long)qi * a.dos[1] + d);
-        const v8 hi = load_or_zero<v8>(ok, (const T*)a.out + orow + d);
-        const v8 lo = load_or_zero<v8>(ok && a.out_lo, (const T*)a.out_lo + orow + d);
+        float o[8] = {};
+        if (ok) {
+            if (a.out32) load_vec<float, 8>(a.out32 + orow + d, o);
+            else load_vec<T, 8>((const T*)a.out + orow + d, o);
+        }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[s][j], (float)hi[j] + (float)lo[j], delta);
+        for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[s][j], o[j], delta);
     }
     // a row without a key has no gradient, whatever its dout holds
     const bool live = raw != -INFINITY;
@@ -503,13 +506,13 @@ extern "C" int64_t tcvom_attn_bwd_work(const tcvom_attn_desc* d) {
 }
 
 extern "C" int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, const void* out,
-                              const void* out_lo, const float* lse, const void* dout, const int64_t* dout_stride, void* dq, void* dk,
+                              const float* out32, const float* lse, const void* dout, const int64_t* dout_stride, void* dq, void* dk,
                               void* dv, float* dtable, float* work, int64_t work_floats, void* stream) {
     AttnArgs a;
     if (const int rc = attn_check("attn_bwd", d, &a)) return rc;
     TCVOM_CHECK_ARG(d->B > 0 && d->Nq > 0 && d->Nk > 0, "attn_bwd: B=%d Nq=%d Nk=%d", d->B, d->Nq, d->Nk);
     TCVOM_CHECK_ARG(q && k && v && table && out && lse && dout && dout_stride && dq && dk && dv && work, "attn_bwd: null tensor");
-    TCVOM_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_lo) && aligned16(dout) &&
+    TCVOM_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out32) && aligned16(dout) &&
                         aligned16(dq) && aligned16(dk) && aligned16(dv), "attn_bwd: tensors start at multiples of 16 bytes");
     TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 128) <= ATTN_MAX_WGS && (long long)d->B * d->H * cdiv(d->Nk, 128) <= ATTN_MAX_WGS,
                     "attn_bwd: %d sequences x %d heads x %d queries, %d keys", d->B, d->H, d->Nq, d->Nk);
@@ -519,7 +522,7 @@ extern "C" int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const voi
                         (long long)dout_stride[n]);
         a.dos[n] = dout_stride[n];
     }
-    a.q = q; a.k = k; a.v = v; a.table = table; a.out = (void*)out; a.out_lo = (void*)out_lo; a.lse = (float*)lse; a.dout = dout;
+    a.q = q; a.k = k; a.v = v; a.table = table; a.out = (void*)out; a.out32 = (float*)out32; a.lse = (float*)lse; a.dout = dout;
     a.dq = dq; a.dk = dk; a.dv = dv;
     a.delta = work;
     a.part = work + (int64_t)d->B * d->H * d->Nq;

@@ -186,33 +186,33 @@ def _attn_desc(q, k, v, buckets, causal, scale, k_lens, key_mask, q_start, q_sta
                       _p(k_lens), _p(q_starts), _p(key_mask), buckets)
 
 
-def _attention(q, k, v, table, train, out_lo, *args):
-    """(out, lse or None) of tensors in the kernels' layout."""
+def _attention(q, k, v, table, train, keep32, *args):
+    """(out, out in 32 bits or None, lse or None) of tensors in the kernels' layout."""
     d = C.byref(_attn_desc(q, k, v, *args))
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device) if train else None
-    lo = torch.empty_like(out) if out_lo else None
+    out32 = torch.empty(q.shape, dtype=torch.float32, device=q.device) if keep32 else None
     n = L.call('tcvom_attn_fwd_work', d)
     work = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
-    _launch(q.get_device(), 'tcvom_attn_fwd', d, q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), out.data_ptr(), _p(lo), _p(lse),
+    _launch(q.get_device(), 'tcvom_attn_fwd', d, q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), out.data_ptr(), _p(out32), _p(lse),
             _p(work), n)
-    return out, lo, lse
+    return out, out32, lse
 
 
 class _BiasedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, *args):
         q, k, v, table = _rows16(q), _rows16(k), _rows16(v), _c(table)
-        out, out_lo, lse = _attention(q, k, v, table, True, ctx.needs_input_grad[3], *args)
+        out, out32, lse = _attention(q, k, v, table, True, ctx.needs_input_grad[3], *args)
         buckets, causal, scale, k_lens, key_mask, q_start, q_starts = args
-        ctx.save_for_backward(q, k, v, table, out, out_lo, lse, k_lens, key_mask, q_starts)
+        ctx.save_for_backward(q, k, v, table, out, out32, lse, k_lens, key_mask, q_starts)
         ctx.args = (buckets, causal, scale, q_start)
         return out
 
     @staticmethod
     @_first_order
     def backward(ctx, dout):
-        q, k, v, table, out, out_lo, lse, k_lens, key_mask, q_starts = ctx.saved_tensors
+        q, k, v, table, out, out32, lse, k_lens, key_mask, q_starts = ctx.saved_tensors
         buckets, causal, scale, q_start = ctx.args
         dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
         dtable = torch.empty_like(table) if ctx.needs_input_grad[3] else None
@@ -222,7 +222,7 @@ class _BiasedAttention(torch.autograd.Function):
         d = C.byref(_attn_desc(q, k, v, buckets, causal, scale, k_lens, key_mask, q_start, q_starts))
         n = L.call('tcvom_attn_bwd_work', d)
         work = torch.empty(n, dtype=torch.float32, device=q.device)
-        _launch(q.get_device(), 'tcvom_attn_bwd', d, q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), out.data_ptr(), _p(out_lo),
+        _launch(q.get_device(), 'tcvom_attn_bwd', d, q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), out.data_ptr(), _p(out32),
                 lse.data_ptr(), dout.data_ptr(), (C.c_int64 * 3)(*_strides(dout)), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(dtable),
                 work.data_ptr(), n)
         return dq, dk, dv, dtable, None, None, None, None, None, None, None
