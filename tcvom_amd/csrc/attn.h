@@ -214,13 +214,19 @@ __device__ __forceinline__ f32x16_t zero16() {
     for (int r = 0; r < 16; ++r) z[r] = 0.f;
     return z;
 }
-// the line of head h, times log2(e), in line[0 .. last]; its two ends are repeated MARGIN entries outwards, so that a tile of 64 x 64 that
+// A bias in base 2.  Finite ones end at +-2^17: a larger one would swallow the score it is added to, and the rounding of maximum + bias
+// (half of 2^-6 there, 64 at 1e9) becomes a factor on the row's probabilities.  Infinite ones stay: -inf takes a distance out.
+__device__ __forceinline__ float base2_bias(float v) {
+    const float x = v * LOG2E;
+    return fabsf(x) > 131072.f && fabsf(v) != INFINITY ? copysignf(131072.f, x) : x;
+}
+// the line of head h, in base 2, in line[0 .. last]; its two ends are repeated MARGIN entries outwards, so that a tile of 64 x 64 that
 // crosses the line reads it without clamping
 constexpr int MARGIN = 128;
 __device__ __forceinline__ void fill_line(float* line, const AttnArgs& a, int h, int threads) {
     const int reach = line_reach(a.bk), last = reach + line_right(a.bk);
     for (int t = (int)threadIdx.x - MARGIN; t <= last + MARGIN; t += threads)
-        line[t] = a.table[rel_bucket(a.bk, min(max(t, 0), last) - reach) * a.H + h] * LOG2E;
+        line[t] = base2_bias(a.table[rel_bucket(a.bk, min(max(t, 0), last) - reach) * a.H + h]);
 }
 static inline size_t line_bytes(const AttnArgs& a) { return sizeof(float) * (line_reach(a.bk) + line_right(a.bk) + 1 + 2 * MARGIN); }
 

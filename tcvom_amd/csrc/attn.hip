@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     constexpr int KS = DP / 16, DB = DP / 32, CH = DP / 8, PER = 32 * CH / 64;
     __shared__ __align__(16) T lv[4][32 * DP];                         // after the loop: 32 x DP floats of two waves at a time
     __shared__ float lm[4][32], ll[4][32];
-    extern __shared__ float tab[];                                     // [buckets][G]: times log2(e), then the bucket of each line entry
+    extern __shared__ float tab[];                                     // [buckets][G] in base 2, then the bucket of each line entry
     const int G = a.H / a.Hkv, rows = G * a.Nq;
     const int reach = line_reach(a.bk), right = line_right(a.bk), last = reach + right;
     unsigned char* bucket = (unsigned char*)(tab + a.bk.num_buckets * G);
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     if (k0 < kz) fetch(k0);
     // (the first keys' loads are in flight)
     for (int t = threadIdx.x; t < a.bk.num_buckets * G; t += 256)
-        tab[t] = a.table[(long long)(t / G) * a.H + hk * G + t % G] * LOG2E;
+        tab[t] = base2_bias(a.table[(long long)(t / G) * a.H + hk * G + t % G]);
     for (int t = threadIdx.x; t <= last; t += 256) bucket[t] = (unsigned char)rel_bucket(a.bk, t - reach);
     __syncthreads();
     const float bias_lo = tab[bucket[0] * G + g], bias_hi = tab[bucket[last] * G + g];

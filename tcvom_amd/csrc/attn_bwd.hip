@@ -327,12 +327,12 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
         mg.load((const T*)a.dout + b * a.dos[0] + at_q.h * a.dos[2] + at_q.i * a.dos[1], a.dos[1], a.Nq - at_q.i, a.D, true, all);
         advance(at_q);
     };
-    auto store_g = [&](int t) {
-        // a row without a key has no gradient, whatever its dout holds: 0 x inf would not vanish in the products
+    // a row without a key has no gradient, whatever its q and dout hold: 0 x inf would not vanish in the products
+    auto store = [&](Mover<T, DP, QT>& m, T* tiles, int t) {
 #pragma unroll
         for (int n = 0; n < PER; ++n)
-            if (ls[t & 3][(threadIdx.x / CH + n * STEP) % QT] == INFINITY) mg.reg[n] = (u32x4_t){0, 0, 0, 0};
-        mg.store(lg + (t & 1) * TILE);
+            if (ls[t & 3][(threadIdx.x / CH + n * STEP) % QT] == INFINITY) m.reg[n] = (u32x4_t){0, 0, 0, 0};
+        m.store(tiles + (t & 1) * TILE);
     };
     const int total = nt * G;
     if (total > 0) {
@@ -344,9 +344,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
             fetch_stats();
             store_stats(1);
         }
-        mq.store(lq);
         __syncthreads();
-        store_g(0);
+        store(mq, lq, 0);
+        store(mg, lg, 0);
     }
     int i0 = i_first, h = h0 - 1;
     for (int t = 0; t < total; ++t) {
@@ -401,7 +401,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
         if constexpr (DP == 128) {
             __builtin_amdgcn_sched_barrier(0);               // (the next product's operands would not fit beside this one's)
             if (t + 1 < total) {
-                mq.store(lq + (buf ^ 1) * TILE);
+                store(mq, lq, t + 1);
                 fetch_g();
             }
         }
@@ -423,8 +423,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
             for (int d = 0; d < DB; ++d) dk[d] = Mma<T>::mma(Tile<T, DP>::cols(lq, ca, s * 16, d), p, dk[d]);
         }
         if (t + 1 < total) {
-            if (DP < 128) mq.store(lq + (buf ^ 1) * TILE);
-            store_g(t + 1);
+            if (DP < 128) store(mq, lq, t + 1);
+            store(mg, lg, t + 1);
         }
         if (t + 2 < total) store_stats(t + 2);
         __syncthreads();

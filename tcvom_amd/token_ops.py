@@ -157,6 +157,8 @@ def relative_position_bias(table, q_len, k_len, max_distance=128, bidirectional=
         raise TypeError('relative_position_bias: dtype %s' % dtype)
     if q_len < 0 or k_len < 0:
         raise ValueError('relative_position_bias: lengths %d, %d' % (q_len, k_len))
+    if not -(1 << 40) < q_start < 1 << 40:
+        raise ValueError('relative_position_bias: q_start %d' % q_start)
     buckets = rel_buckets(table.shape[0], int(max_distance), bool(bidirectional))
     run = _RelBias.apply if _tracked(table) else _rel_bias
     return run(table, buckets, int(q_len), int(k_len), int(q_start), dtype)
@@ -234,12 +236,13 @@ def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causa
 
     q [B, Nq, H, D], k / v [B, Nk, Hkv, D], bf16 or fp16, D a multiple of 8 up to 128; H a multiple of Hkv (consecutive heads share
     keys).  Any strides with contiguous rows of D; others are copied.
-    table fp32 [buckets, H] and max_distance as in relative_position_bias; bidirectional: default not causal.
+    table fp32 [buckets, H] and max_distance as in relative_position_bias; bidirectional: default not causal.  -inf takes a distance
+    out; finite entries count as at most 90852 (2^17 in base 2) in size.
     scale: default D ** -0.5, positive.  Key j sits at position j, query i of sequence b at i + q_start[b] (an int, or int32 [B]).
     Query i sees key j if j < k_lens[b] (int32 [B]; clamped to 0..Nk), key_mask[b, j] (bool or uint8 [B, Nk]) and, causal,
     j <= i + q_start[b].  A query that sees nothing gives zeros and no gradient.  What lies behind the lengths or under the mask
-    may hold anything, NaN included (a NaN or inf that a later query sees can reach earlier ones of a causal call: 0 x inf).  For one new token against caches of Nk slots: k_lens = lengths with the new token,
-    q_start = k_lens - 1, causal.
+    may hold anything, NaN included (a NaN or inf that a later query sees can reach earlier ones of a causal call: 0 x inf).  For one
+    new token against caches of Nk slots: k_lens = lengths with the new token, q_start = k_lens - 1, causal.
 
     Gradients of q, k, v and table.  Probabilities and their gradients are rounded to the 16-bit type as operands of the matrix
     products, everything else is held in 32 bits."""

@@ -422,6 +422,75 @@ def test_empty_rows_ignore_their_gradient():
 
 
 @pytest.mark.parametrize('dt', HALF, ids=ids)
+@pytest.mark.parametrize('D', [32, 64, 128])
+def test_empty_rows_ignore_their_query(D, dt):
+    """Rows in front of the first key of a causal call see nothing, whatever their q and dout hold, also beside rows that do."""
+    B, Nq, Nk, H, dead = 1, 200, 150, 2, 41
+    host = [rnd(B, n, H, D, seed=i).to(dt) for i, n in enumerate((Nq, Nk, Nk, Nq))]
+    table = rnd(32, H, seed=4).float().to(DEV)
+    results = []
+    for fill in (0.0, float('nan'), float('inf')):
+        q, k, v, dout = (t.clone() for t in host)
+        q[:, :dead] = fill
+        dout[:, :dead] = fill
+        leaves = [t.to(DEV).requires_grad_(True) for t in (q, k, v)] + [table.clone().requires_grad_(True)]
+        out = ops.biased_attention(*leaves, causal=True, q_start=-dead)
+        assert not out[:, :dead].any()
+        results.append([out] + list(torch.autograd.grad(out, leaves, dout.to(DEV))))
+    for r in results[1:]:
+        assert not r[1][:, :dead].any()
+        assert all(torch.isfinite(t).all() and torch.equal(t, w) for t, w in zip(r, results[0]))
+
+
+@pytest.mark.parametrize('dt', HALF, ids=ids)
+@pytest.mark.parametrize('nq', [5, 600])
+@pytest.mark.parametrize('low', [-1e4, -1e9, -1e30, torch.finfo(torch.float32).min, -float('inf')])
+def test_distances_masked_by_the_table(low, nq, dt):
+    """A very low bias of the last bucket keeps rows to their neighbourhood; padded rows, beyond it, see keys with that bias only: the
+    softmax of their scores (zeros for -inf).  Logits are rounded to half of 2^-6 around 2^17: three such roundings, of a logit, of the
+    maximum and of a split's or tile's, are 1.7 % of a probability, and as much again of their sum."""
+    B, Nk, H, D, far = 2, 700, 2, 64, 64
+    starts, lens = [40, 690 - nq], [700, 100]
+    q, k, v, dout = (rnd(B, n, H, D, seed=i).to(dt) for i, n in enumerate((nq, Nk, Nk, nq)))
+    table = rnd(32, H, seed=4).float()
+    table[15] = table[31] = low
+    at = torch.stack([bucket_matrix(32, far, True, nq, Nk, s) for s in starts])
+    see = torch.stack([(torch.arange(Nk) < n)[None].expand(nq, Nk) for n in lens])
+    lonely = (see & ~((at == 15) | (at == 31))).sum(-1) == 0
+    assert lonely.any() and not lonely.all()
+    kw = dict(max_distance=far, k_lens=torch.tensor(lens, dtype=torch.int32, device=DEV), q_start=torch.tensor(starts, dtype=torch.int32, device=DEV))
+    limit = 2.0 ** 17 / math.log2(math.e)
+    if low == -float('inf'):
+        see, clamped = see & ~lonely[:, :, None], table.double()
+    else:
+        clamped = table.double().clamp(min=-limit)
+    want, p = attention64(q.double(), k.double(), v.double(), clamped, at, see, D ** -0.5)
+    want = torch.where(see.any(-1)[:, :, None, None], want, torch.zeros_like(want))
+    spread = torch.einsum('bhij,bjhd->bihd', torch.nan_to_num(p), v.double().abs())
+    u = step(dt)
+    bound = u * want.abs() * 1.01 + (u + 2e-5) * spread + 1e-7 + torch.where(lonely[:, :, None, None], 0.034 * spread, torch.zeros_like(spread))
+    with torch.no_grad():
+        out = ops.biased_attention(q.to(DEV), k.to(DEV), v.to(DEV), table.to(DEV), **kw)
+    close(out, want, bound, 'out')
+    leaves = [t.to(DEV).requires_grad_(True) for t in (q, k, v, table)]
+    out = ops.biased_attention(*leaves, **kw)
+    close(out, want, bound, 'training out')
+    # gradients: those of the limit itself, and rows beyond the length with a dout of zeros add nothing
+    quiet = torch.where(lonely[:, :, None, None], torch.zeros_like(dout), dout)
+    if low != -float('inf'):
+        other = [t.to(DEV).requires_grad_(True) for t in (q, k, v, table.clamp(min=-90852.5))]
+        out_ = ops.biased_attention(*other, **kw)
+        assert torch.equal(out, out_) or low > -90852
+    for g in (quiet, dout):
+        grads = torch.autograd.grad(out, leaves, g.to(DEV), retain_graph=True)
+        assert all(torch.isfinite(t).all() for t in grads)
+        if low < -90852 and low != -float('inf'):
+            assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(out_, other, g.to(DEV), retain_graph=True)))
+        if g is quiet:
+            assert not grads[0].cpu()[lonely].any()
+
+
+@pytest.mark.parametrize('dt', HALF, ids=ids)
 def test_one_token_at_a_time_equals_the_whole_sequence(dt):
     """A cache that grows by a token a call, against the causal call over all tokens: the same sums in other orders, each rounded as its
     own call rounds (probabilities and results: 2 u each side)."""
