@@ -6,7 +6,14 @@ __device__ __forceinline__ float empty_or(float sum, float v) { return sum == 0.
 
 // ---- many queries: a workgroup of 4 waves takes 128 queries of one head, a wave 32 of them, all through the same tiles of 64 keys.
 // K and V tiles go to LDS through registers (the next tile's loads are in flight during this tile's products), two buffers, one
-// barrier a tile.
+// barrier a tile.  LO (training with a gradient of the table): a second product with what rounding dropped from the probabilities.
+//
+// Bound: the matrix and the vector unit of a SIMD, which do not run side by side here (a wave's 8 products of a 32 x 32 x 16 block 129 ns,
+// 64 fma 119 ns, 32 exponentials 131 ns, all together 267 ns): at width 64 a score costs about as long on the vector unit as its two products
+// take.  8160 x 8160 tokens, 8 heads of 64, bf16: 220 us = 620 TFLOP/s (a large library product reaches 1340).  4 x 1024, 8 heads of 64, fp16,
+// LO: 34 us; 2 x 4080 causal, 16 heads of 128 on 4, bf16, LO: 260-290 us
+// = 660-740 TFLOP/s.  Slower or no faster: 64 queries a wave (5 % faster at width 64 only, no registers
+// at 128), scores formed a tile ahead, row sums by a product with ones.
 template <class T, int DP, bool LO>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;
@@ -166,7 +173,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
 // columns of one score tile, so that shared keys are read once; the keys are cut into `splits` ranges for workgroups to fill the
 // chip, and a range is dealt 32 keys at a time to 4 waves that keep their own maximum, sum and output and join at the end.
 // K fragments go from memory to registers (a lane reads the 16 bytes it needs), V through a wave's own LDS rows to be transposed:
-// no barrier inside the loop, the next 32 keys in flight.
+// no barrier inside the loop, the next 32 keys in flight.  8 caches of 32768 slots, 2 x 128 wide, bf16 (201 MB): 48 us = 4.2 TB/s, the
+// join 4.8 us.
 template <class T, int DP>
 __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;
@@ -361,7 +369,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
 }
 
 // joins the splits of a row: a workgroup a row, a wave every fourth split, a lane 2 channels (D <= 128); all of a wave's loads are in
-// flight at once, the waves meet in LDS
+// flight at once, the waves meet in LDS.  128 rows of 16 splits, width 128: 4.8 us, a launch
 template <class T>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     __shared__ float red[4][64 * 2 + 1];
@@ -432,7 +440,7 @@ static bool attn_few(const tcvom_attn_desc* d) { return d->Nq <= 32 && d->H / d-
 static void few_shape(const tcvom_attn_desc* d, int* tiles, int* splits) {
     *tiles = cdiv((long long)d->H / d->Hkv * d->Nq, 32);
     const long long wgs = (long long)d->B * d->Hkv * *tiles;
-    // a workgroup a CU (two: 1 to 10 % slower), and at least 256 keys a workgroup
+    // a workgroup a CU (two: 1 to 10 % slower), and at least 256 keys a workgroup (the join is a launch of 4 us)
     long long s = wgs ? 256 / wgs : 1;
     const long long most = d->Nk / 256;
     if (s > most) s = most;
