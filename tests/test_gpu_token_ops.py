@@ -344,6 +344,75 @@ def test_attention_and_its_gradients(case, dt):
         assert torch.equal(got[n], a), n
 
 
+FROZEN = [
+    dict(B=2, Nq=1, Nk=197, H=4, Hkv=2, D=64),
+    dict(B=2, Nq=5, Nk=3000, H=8, Hkv=2, D=64, causal=True, start=[2995, 1200], lens=[3000, 1205]),
+    dict(B=1, Nq=32, Nk=1100, H=4, Hkv=2, D=32, mask=True),
+    dict(B=2, Nq=130, Nk=150, H=4, Hkv=4, D=128, causal=True, lens=[150, 0]),
+    dict(B=3, Nq=77, Nk=93, H=2, Hkv=1, D=40),
+]
+
+
+@pytest.mark.parametrize('dt', HALF, ids=ids)
+@pytest.mark.parametrize('case', FROZEN, ids=attn_id)
+def test_gradients_with_a_frozen_table(case, dt):
+    """Without the table's gradient the forward keeps its 16-bit output only: <dout, out> is off by the roundings of p and of out, u (|out| + sum
+    p |v|) |dout| together, and ds by p times that."""
+    host, at, see, kw = attn_case(case, dt)
+    D, u, G = case['D'], step(dt), case['H'] // case['Hkv']
+    ref = {n: t.double().requires_grad_(n != 'table') for n, t in host.items()}
+    want, p = attention64(ref['q'], ref['k'], ref['v'], ref['table'], at, see, D ** -0.5)
+    dout = rnd(*host['q'].shape, seed=5).to(dt)
+    names = ['q', 'k', 'v']
+    want_g = dict(zip(names, torch.autograd.grad(want, [ref[n] for n in names], dout.double())))
+    leaf = {n: t.to(DEV).requires_grad_(n != 'table') for n, t in host.items()}
+    out = ops.biased_attention(leaf['q'], leaf['k'], leaf['v'], leaf['table'], **kw)
+    got = dict(zip(names, torch.autograd.grad(out, [leaf[n] for n in names], dout.to(DEV))))
+    with torch.no_grad():
+        do = dout.double()
+        vv, kk = (host[n].double().repeat_interleave(G, 2) for n in ('v', 'k'))
+        vv = torch.where(see.any(1)[:, :, None, None], vv, torch.zeros_like(vv))
+        dp = torch.einsum('bihd,bjhd->bhij', do, vv)
+        ds = (p * (dp - (p * dp).sum(-1, keepdim=True))).abs()
+        size = p * (dp.abs() + (p * dp.abs()).sum(-1, keepdim=True))
+        spread = torch.einsum('bhij,bjhd->bihd', p, vv.abs())
+        off = 1.01 * u * (do.abs() * (want.abs() + spread)).sum(-1).permute(0, 2, 1)[..., None] * p
+        group = lambda t: t.reshape(t.shape[0], t.shape[1], case['Hkv'], G, D).sum(3)  # noqa: E731
+        e = u * (ds + off) + off + 2e-5 * size
+        slack = dict(q=D ** -0.5 * torch.einsum('bhij,bjhd->bihd', e, kk.abs()),
+                     k=group(D ** -0.5 * torch.einsum('bhij,bihd->bjhd', e, host['q'].double().abs())),
+                     v=group(torch.einsum('bhij,bihd->bjhd', (u + 2e-5) * p, do.abs())))
+    close(out, want.detach(), u * want.detach().abs() * 1.01 + (u + 2e-5) * spread + 1e-7, 'out')
+    for n in names:
+        tiny = 1e-6 if dt == torch.bfloat16 else 2.0 ** -25 * (2 + case['Nk'] + case['Nq'] * G)
+        close(got[n], want_g[n], u * 1.01 * want_g[n].abs() + slack[n] + tiny, 'd' + n)
+    # asked for one at a time, and together with the table's: v's gradient does not change (its p and dout are the same)
+    for n in names:
+        one = {m: t.to(DEV).requires_grad_(m == n) for m, t in host.items()}
+        g, = torch.autograd.grad(ops.biased_attention(one['q'], one['k'], one['v'], one['table'], **kw), [one[n]], dout.to(DEV))
+        assert torch.equal(g, got[n]), n
+
+
+@pytest.mark.parametrize('C', [40, 203, 1024])
+def test_norm_gradients_asked_for_one_at_a_time(C):
+    """Each gradient alone equals, bit for bit, the one asked for with all others; gates of channels, samples and tokens."""
+    B, N = 3, 37
+    host = dict(x=rnd(B, N, C, seed=1), y=rnd(B, N, C, seed=2), post_weight=rnd(C, seed=3), post_bias=rnd(C, seed=4), pre_weight=rnd(C, seed=5),
+                pre_bias=rnd(C, seed=6))
+    dx, dh = rnd(B, N, C, seed=7).float().to(DEV), rnd(B, N, C, seed=8).float().to(DEV)
+    for gate in ((C,), (B, C), (B, N, C)):
+        host['gate'] = rnd(*gate, seed=9)
+
+        def grads(wanted):
+            leaf = {n: t.float().to(DEV).requires_grad_(n in wanted) for n, t in host.items()}
+            out = ops.block_norm(**leaf, branch_scale=0.7, residual_scale=1.1, kind='layer')
+            return dict(zip(wanted, torch.autograd.grad(out, [leaf[n] for n in wanted], (dx, dh))))
+
+        every = grads(list(host))
+        for n in host:
+            assert torch.equal(grads([n])[n], every[n]), (gate, n)
+
+
 def test_attention_with_the_longest_line_and_the_most_buckets():
     """The largest LDS footprints: width 128, reach 1024, 256 buckets, with the table's gradient; 64 and 128 heads on one key head."""
     for c in (dict(B=1, Nq=130, Nk=2300, H=2, Hkv=2, D=128, buckets=256, far=1024), dict(B=1, Nq=33, Nk=1500, H=2, Hkv=1, D=64, buckets=256, far=1024),
