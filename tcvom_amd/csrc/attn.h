@@ -131,6 +131,12 @@ __device__ __forceinline__ unsigned keep(unsigned v) {
     asm volatile("" : "+v"(v));
     return v;
 }
+// v has arrived from memory from here on.  Without it the compiler, which cannot tell a loop's first turn from the others, waits for such a
+// load inside the loop -- and with it for the next tile's, issued just before.
+template <class V8, int N> __device__ __forceinline__ void arrived(V8 (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
+}
 // Operands from an LDS tile of rows of DP elements (layout: chunk_at).  A lane's byte offset differs between steps by an XOR of a few low
 // bits and a constant, so that one register and one instruction a step address them all.
 template <class T, int DP> struct Tile {
@@ -174,6 +180,7 @@ template <class T, int DP, int ROWS> struct Mover {
 #pragma unroll
             for (int n = 0; n < PER; ++n)
                 reg[n] = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const char*>(base + n * STEP * stride) + off);
+            asm volatile("; whole tile");           // (else the last load is shared with the other form, behind its zeroes and their wait)
             return;
         }
 #pragma unroll

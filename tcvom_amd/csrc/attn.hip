@@ -68,6 +68,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
         mk.store(lk);
         mv.store(lv);
     }
+    arrived(qf);
     __syncthreads();
     for (int t = 0; t < ntiles; ++t) {
         const int k0 = t * KT, buf = (t & 1) * TILE;

@@ -105,6 +105,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
         mk.store(lk);
         mv.store(lv);
     }
+    arrived(qf);
+    arrived(gf);
     __syncthreads();
     for (int t = 0; t < ntiles; ++t) {
         const int k0 = t * KT, buf = (t & 1) * TILE;
@@ -354,6 +356,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
         store(mq, lq, 0);
         store(mg, lg, 0);
     }
+    arrived(kf);
+    if constexpr (VREG) arrived(vf);
     int i0 = i_first, h = h0 - 1;
     for (int t = 0; t < total; ++t) {
         const int buf = t & 1;
