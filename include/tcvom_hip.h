@@ -727,8 +727,9 @@ typedef struct {
 int64_t tcvom_attn_fwd_work(const tcvom_attn_desc* d);
 int tcvom_attn_fwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, void* out, float* out32,
                    float* lse, float* work, int64_t work_floats, void* stream);
-/* Gradients from what the forward read and wrote (lse required); dout with strides like q's; dq / dk / dv contiguous, dtable (or NULL:
- * not asked for) fp32 like table.  Keys and rows without a pair get zeros.  Fixed order of additions. */
+/* Gradients from what the forward read and wrote (lse; out32 where dtable is asked for, else it is not read); dout with strides like
+ * q's; dq / dk / dv contiguous, dtable (or NULL: not asked for) fp32 like table.  Keys and rows without a pair get zeros.  Fixed order
+ * of additions. */
 int64_t tcvom_attn_bwd_work(const tcvom_attn_desc* d);
 int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, const void* out,
                    const float* out32, const float* lse, const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv,

@@ -18,6 +18,8 @@ template <class T, int DP, bool LO>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;
     constexpr int KS = DP / 16, DB = DP / 32, BM = 128, TILE = KT * DP;
+    // the running maximum may lag by 2^SLACK: probabilities then reach 2^(SLACK + SHIFT), the largest power of two of fp16
+    constexpr float SLACK = 4.f, SHIFT = Mma<T>::shift > 0.f ? Mma<T>::shift - SLACK : 0.f;
     __shared__ __align__(16) T lk[2 * TILE];
     __shared__ __align__(16) T lv[2 * TILE];
     extern __shared__ float line_[];
@@ -108,7 +110,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
             }
         }
         const float mn = max2(m, fmaf(half_max(max2(max16(x[0]), max16(x[1]))), mul, add));
-        if (__any(mn > m)) {
+        if (__any(mn > m + SLACK)) {                         // (any new maximum: half of the tiles of 8160 keys instead of a few)
             const float alpha = exp2_hw(m - (mn == -INFINITY ? 0.f : mn));
             l *= alpha;
 #pragma unroll
@@ -117,7 +119,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
                 for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
             m = mn;
         }
-        const float sub = Mma<T>::shift - (m == -INFINITY ? 0.f : m) + add;
+        const float sub = SHIFT - (m == -INFINITY ? 0.f : m) + add;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -167,7 +169,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
             *reinterpret_cast<typename Mma<T>::v4*>((T*)a.out + row * a.D + at) = w;
             if (LO) *reinterpret_cast<f32x4_t*>(a.out32 + row * a.D + at) = f;
         }
-    if (a.lse && half == 0) a.lse[((long long)b * a.H + h) * a.Nq + qi] = sum == 0.f ? -INFINITY : m + log2f(sum) - Mma<T>::shift;
+    if (a.lse && half == 0) a.lse[((long long)b * a.H + h) * a.Nq + qi] = sum == 0.f ? -INFINITY : m + log2f(sum) - SHIFT;
 }
 
 // ---- few queries (single tokens): bound by reading K and V once.  The G = H / Hkv heads that share keys times the queries are the 32

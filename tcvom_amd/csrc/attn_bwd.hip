@@ -60,20 +60,27 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     const long long stat = ((long long)b * a.H + h) * a.Nq + qi, orow = (((long long)b * a.Nq + qi) * a.H + h) * a.D;
     const float raw = qi < a.Nq ? a.lse[stat] : -INFINITY;
     v8 qf[KS], gf[KS];
+    f32x4_t of[2 * KS];
     float delta = 0.f;
+    // (every load is issued before one is waited for)
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
         const int d = s * 16 + half * 8;
         const bool ok = qi < a.Nq && d < a.D;
         qf[s] = load_or_zero<v8>(ok, Q + (long long)qi * a.qs[1] + d);
         gf[s] = load_or_zero<v8>(ok, dO + (long long)qi * a.dos[1] + d);
-        float o[8] = {};
-        if (ok) {
-            if (a.out32) load_vec<float, 8>(a.out32 + orow + d, o);
-            else load_vec<T, 8>((const T*)a.out + orow + d, o);
+        if (TABLE) {
+            of[2 * s] = load_or_zero<f32x4_t>(ok, a.out32 + orow + d);
+            of[2 * s + 1] = load_or_zero<f32x4_t>(ok, a.out32 + orow + d + 4);
+        } else {
+            of[s] = __builtin_bit_cast(f32x4_t, load_or_zero<v8>(ok, (const T*)a.out + orow + d));
         }
+    }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[s][j], o[j], delta);
+    for (int s = 0; s < KS; ++s) {
+        const v8 o = __builtin_bit_cast(v8, of[s]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) delta = fmaf((float)gf[s][j], TABLE ? of[2 * s + j / 4][j % 4] : (float)o[j], delta);
     }
     // a row without a key has no gradient, whatever its dout holds
     const bool live = raw != -INFINITY;
@@ -522,6 +529,7 @@ extern "C" int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const voi
     if (const int rc = attn_check("attn_bwd", d, &a)) return rc;
     TCVOM_CHECK_ARG(d->B > 0 && d->Nq > 0 && d->Nk > 0, "attn_bwd: B=%d Nq=%d Nk=%d", d->B, d->Nq, d->Nk);
     TCVOM_CHECK_ARG(q && k && v && table && out && lse && dout && dout_stride && dq && dk && dv && work, "attn_bwd: null tensor");
+    TCVOM_CHECK_ARG(!dtable || out32, "attn_bwd: the table's gradient needs the output in 32 bits");
     TCVOM_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out32) && aligned16(dout) &&
                         aligned16(dq) && aligned16(dk) && aligned16(dv), "attn_bwd: tensors start at multiples of 16 bytes");
     TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 128) <= ATTN_MAX_WGS && (long long)d->B * d->H * cdiv(d->Nk, 128) <= ATTN_MAX_WGS,
