@@ -16,8 +16,8 @@
 // give equal bits.  (Adding the elements with LDS atomics took 53 cycles an instruction, one lane after the other: 16 of them a block
 // were as long as its matrix products.)
 //
-// Bound as the forward by matrix plus vector time: 3 products and 5 vector instructions a score.  4 x 1024 tokens, 8 heads of 64, fp16: 46 us; 2 x
-// 4080 causal, 16 heads of 128 on 4, bf16: 300-340 us = 560-640 TFLOP/s.
+// Bound as the forward by matrix plus vector time: 3 products and 5 vector instructions a score.  4 x 1024 tokens, 8 heads of 64, fp16: 45 us; 2 x
+// 4080 causal, 16 heads of 128 on 4, bf16: 290-330 us = 580-660 TFLOP/s.
 template <class T, int DP, bool TABLE>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;
@@ -254,8 +254,8 @@ __device__ __forceinline__ void sum_table(const AttnArgs& a, int h, double* red)
 // few workgroups (attn_apart) each head of a group gets workgroups of its own, which write fp32 partial sums [2][B][Nk][H][D] that
 // attn_heads_kernel adds in order.  The tiles with most queries come first.
 //
-// Bound as above, 4 products a score.  4 x 1024 tokens, 8 heads of 64, fp16: 45 us; 2 x 4080 causal, 16 heads of 128 on 4, bf16: 400-440 us =
-// 580-640 TFLOP/s, attn_heads_kernel 23 us (150 MB, part of them still in the last cache).
+// Bound as above, 4 products a score.  4 x 1024 tokens, 8 heads of 64, fp16: 43 us; 2 x 4080 causal, 16 heads of 128 on 4, bf16: 380-440 us =
+// 580-670 TFLOP/s, attn_heads_kernel 23 us (150 MB, part of them still in the last cache).
 template <class T, int DP>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;

@@ -2,8 +2,8 @@
 //     x' = residual_scale x + branch_scale g N1(y),    h = N2(x')
 // N = RMSNorm (t r w, r = 1 / sqrt(mean t^2 + eps)) or LayerNorm ((t - m) r w + b).  Bound: HBM bytes -- x, y in and x', h out once
 // forward (x, y, dx', dh in and dx, dy out backward), everything between in registers.  8192 rows of 4096, bf16: forward 49.5 us = 5.4 TB/s,
-// backward 90 us = 4.5 TB/s + 4.8 us for the column sums (a copy reaches 5.1); 8160 rows of 512, fp32 x and bf16 y: 12.6 us = 4.0 TB/s and
-// 18.6 us = 4.0 TB/s + 5.4 us; 4 rows of 4096: 4.1 us, a launch.
+// backward 82 us = 4.9 TB/s + 4.4 us for the column sums (a copy reaches 5.1); 8160 rows of 512, fp32 x and bf16 y: 12.6 us = 4.0 TB/s and
+// 18 us = 4.2 TB/s + 5.4 us; 4 rows of 4096: 4.1 us, a launch.
 //
 // One row belongs to TPR threads, each with NV vectors of 8 channels: 16 lanes at <= 128 channels, up to 512 threads at 8192.  A
 // workgroup has R such row groups and walks its rows with the weights in registers.  TAIL: the channels are no multiple of 8; rows
