@@ -10,7 +10,8 @@ needs these.  The reference has no counterpart.
 
 Element types are arguments: bf16, fp16 and, for the bias matrix and the norms, fp32, in either build of the library.  16-bit results are
 rounded to nearest even without saturation.  Gradients are added in a fixed order: equal calls give equal bits.  First derivatives
-only.
+only.  A call may be captured into a graph, its backward too -- while no eager graph of the same leaves lives (torch would join the capture
+to that graph's stream and end the process).
 """
 import ctypes as C
 import functools
