@@ -95,6 +95,9 @@ template <int DP> __device__ __forceinline__ int chunk_at(int r, int c) {
     else return r * 4 + (c ^ ((r >> 2) & 3));
 }
 
+// NaN stays NaN; v_maximum3_f32
+__device__ __forceinline__ float max2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ __forceinline__ float max3(float a, float b, float c) { return max2(max2(a, b), c); }
 __device__ __forceinline__ float half_max(float v) {       // maximum over lanes l and l ^ 32
     const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __builtin_elementwise_maximum(__uint_as_float(s[0]), __uint_as_float(s[1]));
@@ -124,6 +127,45 @@ __device__ __forceinline__ typename Mma<T>::v8 pack_rest(const f32x16_t& p, type
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i] = (T)(p[8 * s + i] - (float)hi[i]);
     return r;
+}
+
+// Score gradients ds = p (dp - delta) as 16-bit operands.  They are as large as dout times p: in fp16 those of a long row, or of a small dout, lie
+// below 2^-14, its smallest normal number, and those of a large dout times large values beyond its largest.  fp16 therefore holds
+// 2^e ds, with an e (here up = 2^e) for each column of the product, a query of dq and a key of dk, that falls whenever a block of the column
+// would pass 2^15: the block's largest then becomes 2^11 .. 2^12, the sums so far follow (times a power of two: no rounding), and 2^-e
+// comes off in 32 bits at the store.  What is 2^26 times smaller than a column's largest still is a normal number.  bf16 has the exponents of
+// fp32 and needs none of it.  4 x 1024 tokens, 8 heads of 64, fp16: dq
+// 44 -> 47 us, dk / dv 42 -> 48 us; 2 x 4080 causal, 16 heads of 128 on 4: 278 -> 295 and 372 -> 378 us.
+template <class T> constexpr float DS_UP = Mma<T>::shift > 0.f ? 0x1p100f : 1.f;
+template <class T, int DB>
+__device__ __forceinline__ void ds_fit(const f32x16_t& x, float& up, f32x16_t (&sums)[DB]) {
+    if constexpr (Mma<T>::shift > 0.f) {
+        float t[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) t[n] = max3(fabsf(x[4 * n]), fabsf(x[4 * n + 1]), fabsf(x[4 * n + 2]));
+        const float top = half_max(max3(max3(t[0], fabsf(x[3]), t[1]), max3(fabsf(x[7]), t[2], fabsf(x[11])), max2(t[3], fabsf(x[15]))));
+        if (__any(top * up > 32768.f)) {
+            const int e = __builtin_amdgcn_frexp_expf(up) - 1, now = top * up > 32768.f ? min(e, 12 - __builtin_amdgcn_frexp_expf(top)) : e;
+            const float f = ldexpf(1.f, now - e);
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sums[d][r] *= f;
+            up = ldexpf(1.f, now);
+        }
+    }
+}
+template <class T>
+__device__ __forceinline__ typename Mma<T>::v8 pack_ds(const f32x16_t& x, float up, int s) {
+    if constexpr (!(Mma<T>::shift > 0.f)) return pack_step<T>(x, s);
+    typename Mma<T>::v8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (T)(x[8 * s + i] * up);
+    return r;
+}
+template <class T>
+__device__ __forceinline__ float ds_down(float sum, float up) {
+    return Mma<T>::shift > 0.f ? ldexpf(sum, 1 - __builtin_amdgcn_frexp_expf(up)) : sum;
 }
 
 // v, computed here: not hoisted out of a loop into a register of its own
@@ -202,9 +244,6 @@ template <class T, int DP, int ROWS> struct Mover {
         }
     }
 };
-// NaN stays NaN; v_maximum3_f32
-__device__ __forceinline__ float max2(float a, float b) { return __builtin_elementwise_maximum(a, b); }
-__device__ __forceinline__ float max3(float a, float b, float c) { return max2(max2(a, b), c); }
 __device__ __forceinline__ float max16(const f32x16_t& x) {
     return max3(max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[8])),
                 max3(max3(x[9], x[10], x[11]), x[12], x[13]), max2(x[14], x[15]));

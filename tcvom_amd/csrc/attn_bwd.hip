@@ -6,7 +6,8 @@
 // over all heads that share them) walks the queries.  Scores are formed in both: 7 products instead of the 5 of a single pass, which
 // would have to add dq (or dk, dv) into memory in an order that changes from run to run.
 //
-// Rounding to 16 bits: p and ds as operands of the matrix products, as the forward rounds p.  The bucket sums take ds in 32 bits.
+// Rounding to 16 bits: p and ds as operands of the matrix products, as the forward rounds p (fp16: p times 2^15, ds times a running power of
+// two, ds_fit).  The bucket sums take ds in 32 bits.
 #include "attn.h"
 
 // ---- dq, delta, bucket sums: a wave owns 32 queries of one head (S^T and dP^T as in the forward), the workgroup walks tiles of 64 keys.
@@ -16,7 +17,7 @@
 // give equal bits.  (Adding the elements with LDS atomics took 53 cycles an instruction, one lane after the other: 16 of them a block
 // were as long as its matrix products.)
 //
-// Bound as the forward by matrix plus vector time: 3 products and 5 vector instructions a score.  4 x 1024 tokens, 8 heads of 64, fp16: 45 us; 2 x
+// Bound as the forward by matrix plus vector time: 3 products and 5 vector instructions a score.  4 x 1024 tokens, 8 heads of 64, fp16: 47 us; 2 x
 // 4080 causal, 16 heads of 128 on 4, bf16: 290-330 us = 580-660 TFLOP/s.
 template <class T, int DP, bool TABLE>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
@@ -103,7 +104,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     f32x16_t acc[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) acc[d] = zero16();
-    float far_lo = 0.f, far_hi = 0.f;
+    float far_lo = 0.f, far_hi = 0.f, up = DS_UP<T>;
     const float c = a.scale * LOG2E;
     const unsigned rows_at = Tile<T, DP>::rows_at(lane), cols_at = Tile<T, DP>::cols_at(lane);
     if (ntiles > 0) fetch(0);
@@ -165,9 +166,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
                     total += (s[0] + s[1]) + (s[2] + s[3]);
                 }
             }
+            ds_fit<T>(x, up, acc);
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const v8 p = pack_step<T>(x, s);
+                const v8 p = pack_ds<T>(x, up, s);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) acc[d] = Mma<T>::mma(Tile<T, DP>::cols(lk, ca, kb * 32 + s * 16, d), p, acc[d]);
             }
@@ -189,7 +191,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
                 if (at >= a.D) continue;
                 typename Mma<T>::v4 w;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) w[j] = (T)(acc[d][4 * g + j] * a.scale);
+                for (int j = 0; j < 4; ++j) w[j] = (T)ds_down<T>(acc[d][4 * g + j] * a.scale, up);
                 *reinterpret_cast<typename Mma<T>::v4*>((T*)a.dq + orow + at) = w;
             }
     }
@@ -254,7 +256,7 @@ __device__ __forceinline__ void sum_table(const AttnArgs& a, int h, double* red)
 // few workgroups (attn_apart) each head of a group gets workgroups of its own, which write fp32 partial sums [2][B][Nk][H][D] that
 // attn_heads_kernel adds in order.  The tiles with most queries come first.
 //
-// Bound as above, 4 products a score.  4 x 1024 tokens, 8 heads of 64, fp16: 43 us; 2 x 4080 causal, 16 heads of 128 on 4, bf16: 380-440 us =
+// Bound as above, 4 products a score.  4 x 1024 tokens, 8 heads of 64, fp16: 48 us; 2 x 4080 causal, 16 heads of 128 on 4, bf16: 380-440 us =
 // 580-670 TFLOP/s, attn_heads_kernel 23 us (150 MB, part of them still in the last cache).
 template <class T, int DP>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
@@ -299,6 +301,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
         dk[d] = zero16();
         dv[d] = zero16();
     }
+    float up = DS_UP<T>;
     const float c = a.scale * LOG2E;
     const unsigned rows_at = Tile<T, DP>::rows_at(lane), cols_at = Tile<T, DP>::cols_at(lane);
     constexpr float small = Mma<T>::shift > 0.f ? 1.f / 32768.f : 1.f;       // 2^-shift
@@ -329,9 +332,10 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
         advance(at_s);
     };
     auto store_stats = [&](int t) {
-        if (threadIdx.x < QT) {
-            ls[t & 3][threadIdx.x] = rs == -INFINITY ? INFINITY : rs - Mma<T>::shift;       // p = 0 in rows that are empty or past the end
-            ld[t & 3][threadIdx.x] = rd * small;
+        const unsigned n = DP == 128 ? keep(threadIdx.x) : threadIdx.x;
+        if (n < QT) {
+            ls[t & 3][n] = rs == -INFINITY ? INFINITY : rs - Mma<T>::shift;       // p = 0 in rows that are empty or past the end
+            ld[t & 3][n] = rd * small;
         }
     };
     auto all = [](int) { return true; };
@@ -433,9 +437,10 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
             x[4 * q + 2] *= fmaf(g[4 * q + 2], small, -d4.z);
             x[4 * q + 3] *= fmaf(g[4 * q + 3], small, -d4.w);
         }
+        ds_fit<T>(x, up, dk);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const v8 p = pack_step<T>(x, s);
+            const v8 p = pack_ds<T>(x, up, s);
 #pragma unroll
             for (int d = 0; d < DB; ++d) dk[d] = Mma<T>::mma(Tile<T, DP>::cols(lq, ca, s * 16, d), p, dk[d]);
         }
@@ -456,7 +461,8 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
             for (int q = 0; q < 4; ++q) {
                 const int at = d * 32 + q * 8 + half * 4;
                 if (at >= a.D) continue;
-                *reinterpret_cast<float4*>(dst + at) = make_float4(dk[d][4 * q], dk[d][4 * q + 1], dk[d][4 * q + 2], dk[d][4 * q + 3]);
+                *reinterpret_cast<float4*>(dst + at) = make_float4(ds_down<T>(dk[d][4 * q], up), ds_down<T>(dk[d][4 * q + 1], up),
+                                                                   ds_down<T>(dk[d][4 * q + 2], up), ds_down<T>(dk[d][4 * q + 3], up));
                 *reinterpret_cast<float4*>(dst + next + at) = make_float4(dv[d][4 * q], dv[d][4 * q + 1], dv[d][4 * q + 2], dv[d][4 * q + 3]);
             }
         return;
@@ -471,7 +477,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
             typename Mma<T>::v4 w, u;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                w[j] = (T)(dk[d][4 * q + j] * a.scale);
+                w[j] = (T)ds_down<T>(dk[d][4 * q + j] * a.scale, up);
                 u[j] = (T)(dv[d][4 * q + j] * small);
             }
             *reinterpret_cast<typename Mma<T>::v4*>((T*)a.dk + row + at) = w;

@@ -246,7 +246,8 @@ def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causa
     new token against caches of Nk slots: k_lens = lengths with the new token, q_start = k_lens - 1, causal.
 
     Gradients of q, k, v and table.  Probabilities and their gradients are rounded to the 16-bit type as operands of the matrix
-    products, everything else is held in 32 bits."""
+    products (in fp16 times powers of two, so that a small dout loses no bits of them and a large one does not overflow), everything
+    else is held in 32 bits."""
     name = 'biased_attention'
     q_starts = None
     if isinstance(q_start, torch.Tensor):

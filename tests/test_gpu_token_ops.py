@@ -393,6 +393,57 @@ def test_gradients_with_a_frozen_table(case, dt):
         assert torch.equal(g, got[n]), n
 
 
+DOUTS = [
+    dict(B=1, Nq=300, Nk=4000, H=2, Hkv=1, D=64),
+    dict(B=2, Nq=300, Nk=300, H=4, Hkv=1, D=128, causal=True, lens=[300, 177]),
+    dict(B=1, Nq=130, Nk=517, H=2, Hkv=2, D=32),
+    dict(B=1, Nq=700, Nk=200, H=2, Hkv=2, D=40, mask=True),
+]
+
+
+@pytest.mark.parametrize('dt', HALF, ids=ids)
+@pytest.mark.parametrize('std', [1e-4, 1.0, 4e3, 'rows'])
+@pytest.mark.parametrize('which', ['q', 'k'])
+@pytest.mark.parametrize('case', DOUTS, ids=attn_id)
+def test_gradients_of_small_and_large_douts(case, which, std, dt):
+    """dout of deviation 1e-4, 1, 4000 (with values of 16: score gradients up to 1e6) and 1e-3 .. 1e3 from row to row.  The other operand of the
+    product is lifted or lowered by 2^6, so that the gradient itself is within fp16's range: what the score gradients lose would show.  Bound of an
+    element: its own rounding (u |w|, or half of fp16's last step, 2^-24) and, as independent errors, those of the ds it sums, u |ds| each
+    plus the 32-bit part.  Twice their deviation bounds the root mean square of error / bound by 1 (equally distributed roundings have half a step
+    / sqrt 3)."""
+    host, at, see, kw = attn_case(case, dt)
+    other = 'k' if which == 'q' else 'q'
+    lift = {1e-4: 64.0, 4e3: 1 / 64}.get(std, 1.0)
+    host[other], host[which] = host[other] * lift, host[which] / lift
+    if std == 4e3:
+        host['v'] = host['v'] * 16
+    D, u, G = case['D'], step(dt), case['H'] // case['Hkv']
+    size = 10.0 ** torch.linspace(-3, 3, case['Nq'], dtype=torch.float64)[None, :, None, None] if std == 'rows' else std
+    dout = (rnd(*host['q'].shape, seed=5) * size).to(dt)
+    ref = {n: t.double().requires_grad_(n == which) for n, t in host.items()}
+    want, p = attention64(ref['q'], ref['k'], ref['v'], ref['table'], at, see, D ** -0.5)
+    w, = torch.autograd.grad(want, ref[which], dout.double())
+    leaf = {n: t.to(DEV).requires_grad_(True) for n, t in host.items()}
+    out = ops.biased_attention(leaf['q'], leaf['k'], leaf['v'], leaf['table'], **kw)
+    g, = torch.autograd.grad(out, leaf[which], dout.to(DEV))
+    assert torch.isfinite(g).all()
+    with torch.no_grad():
+        vv, kk = (host[n].double().repeat_interleave(G, 2) for n in ('v', 'k'))
+        vv = torch.where(see.any(1)[:, :, None, None], vv, torch.zeros_like(vv))
+        dp = torch.einsum('bihd,bjhd->bhij', dout.double(), vv)
+        ds = (p * (dp - (p * dp).sum(-1, keepdim=True))).abs()
+        terms = p * (dp.abs() + (p * dp.abs()).sum(-1, keepdim=True))
+        e = (u * ds + 2e-5 * terms) ** 2 / D
+        if which == 'q':
+            var = torch.einsum('bhij,bjhd->bihd', e, kk ** 2)
+        else:
+            var = torch.einsum('bhij,bihd->bjhd', e, host['q'].double() ** 2)
+            var = var.reshape(var.shape[0], var.shape[1], case['Hkv'], G, D).sum(3)
+        bound = 2 * var.sqrt() + (u * w.abs()).clamp(min=2.0 ** -25 if dt == torch.float16 else 2.0 ** -134)
+        rms = float((((g.double().cpu() - w) / bound) ** 2).mean().sqrt())
+    assert rms < 1, rms
+
+
 @pytest.mark.parametrize('C', [40, 203, 1024])
 def test_norm_gradients_asked_for_one_at_a_time(C):
     """Each gradient alone equals, bit for bit, the one asked for with all others; gates of channels, samples and tokens."""
