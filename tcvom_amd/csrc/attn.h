@@ -269,10 +269,16 @@ __device__ __forceinline__ float base2_bias(float v) {
 // the line of head h, in base 2, in line[0 .. last]; its two ends are repeated MARGIN entries outwards, so that a tile of 64 x 64 that
 // crosses the line reads it without clamping
 constexpr int MARGIN = 128;
-__device__ __forceinline__ void fill_line(float* line, const AttnArgs& a, int h, int threads) {
+// ... returns whether this thread wrote a NaN or +inf
+__device__ __forceinline__ bool fill_line(float* line, const AttnArgs& a, int h, int threads) {
     const int reach = line_reach(a.bk), last = reach + line_right(a.bk);
-    for (int t = (int)threadIdx.x - MARGIN; t <= last + MARGIN; t += threads)
-        line[t] = base2_bias(a.table[rel_bucket(a.bk, min(max(t, 0), last) - reach) * a.H + h]);
+    bool odd = false;
+    for (int t = (int)threadIdx.x - MARGIN; t <= last + MARGIN; t += threads) {
+        const float v = base2_bias(a.table[rel_bucket(a.bk, min(max(t, 0), last) - reach) * a.H + h]);
+        line[t] = v;
+        odd |= !(v < INFINITY);
+    }
+    return odd;
 }
 static inline size_t line_bytes(const AttnArgs& a) { return sizeof(float) * (line_reach(a.bk) + line_right(a.bk) + 1 + 2 * MARGIN); }
 

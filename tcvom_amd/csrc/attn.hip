@@ -103,6 +103,14 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
             const int lim = my_limit - k0;
             const unsigned long long see = lim >= 64 ? bits : lim <= 0 ? 0 : bits & ((1ull << lim) - 1);
             const unsigned s0 = (unsigned)see >> (4 * half), s1 = (unsigned)(see >> 32) >> (4 * half);
+            if (!(add < INFINITY)) {                         // (a bias of NaN or +inf, added to -inf below, would reach rows that see none of these keys)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x[kb][r] = fmaf(x[kb][r], c, add);
+                mul = 1.f;
+                add = 0.f;
+            }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 x[0][r] = pick(s0, r, x[0][r], -INFINITY);

@@ -267,6 +267,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     constexpr bool VREG = DP < 128;                         // values, operand B of dP = dO V^T, in registers; width 128 has none left
     __shared__ __align__(16) T lv[VREG ? 8 : BN * DP];
     __shared__ __align__(16) float ls[4][QT], ld[4][QT];    // log-sums and deltas of the tiles: written two tiles ahead
+    __shared__ int odds[4];                                 // a wave each: `odd` of its share of the line
     extern __shared__ float line_[];
     float* line = line_ + MARGIN;
     const int extra = a.dtable ? a.H : 0;
@@ -370,6 +371,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     arrived(kf);
     if constexpr (VREG) arrived(vf);
     int i0 = i_first, h = h0 - 1;
+    int odd = 0;                                             // whether the head's bias has a NaN or +inf somewhere
     for (int t = 0; t < total; ++t) {
         const int buf = t & 1;
         i0 -= QT;
@@ -377,8 +379,10 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
         if (i0 < i_first) {                                  // another head's bias
             i0 = i_last;
             __syncthreads();
-            fill_line(line, a, ++h, 256);
+            const int any = __any(fill_line(line, a, ++h, 256));
+            if (lane == 0) odds[wave] = any;
             __syncthreads();
+            odd = __builtin_amdgcn_readfirstlane(odds[0] | odds[1] | odds[2] | odds[3]);
         }
         // the next tile: at width 128 its dO is fetched once its Q has left the registers
         if (t + 2 < total) fetch_stats();
@@ -407,6 +411,16 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
             for (int r = 0; r < 16; ++r) x[r] = exp2_hw(fmaf(x[r], c, at[-8 * (r / 4) - r % 4] - sub[r]));
         }
         const int first = a.causal ? key - start - i0 - 4 * half : -1 << 30;     // the first row of the tile that sees the key, less 4 half
+        if (odd) {                                           // rows that are empty or past the end: exp2(bias - inf) is not always 0 then
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float4 s4 = *reinterpret_cast<const float4*>(&ls[t & 3][8 * q + 4 * half]);
+                x[4 * q] = s4.x == INFINITY ? 0.f : x[4 * q];
+                x[4 * q + 1] = s4.y == INFINITY ? 0.f : x[4 * q + 1];
+                x[4 * q + 2] = s4.z == INFINITY ? 0.f : x[4 * q + 2];
+                x[4 * q + 3] = s4.w == INFINITY ? 0.f : x[4 * q + 3];
+            }
+        }
         if (!seen || first > -4) {
             const int from = seen ? first : 1 << 30;
 #pragma unroll

@@ -238,7 +238,7 @@ def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causa
     q [B, Nq, H, D], k / v [B, Nk, Hkv, D], bf16 or fp16, D a multiple of 8 up to 128; H a multiple of Hkv (consecutive heads share
     keys).  Any strides with contiguous rows of D; others are copied.
     table fp32 [buckets, H] and max_distance as in relative_position_bias; bidirectional: default not causal.  -inf takes a distance
-    out; finite entries count as at most 90852 (2^17 in base 2) in size.
+    out; finite entries count as at most 90852 (2^17 in base 2) in size; those of distances that no query sees may hold anything.
     scale: default D ** -0.5, positive.  Key j sits at position j, query i of sequence b at i + q_start[b] (an int, or int32 [B]).
     Query i sees key j if j < k_lens[b] (int32 [B]; clamped to 0..Nk), key_mask[b, j] (bool or uint8 [B, Nk]) and, causal,
     j <= i + q_start[b].  A query that sees nothing gives zeros and no gradient.  What lies behind the lengths or under the mask

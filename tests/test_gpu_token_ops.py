@@ -444,6 +444,40 @@ def test_gradients_of_small_and_large_douts(case, which, std, dt):
     assert rms < 1, rms
 
 
+UNUSED = [
+    dict(B=1, Nq=200, Nk=200, H=2, Hkv=1, D=64, causal=True, bidirectional=True, buckets=16, far=20),
+    dict(B=2, Nq=33, Nk=64, H=2, Hkv=2, D=32, far=200),
+    dict(B=2, Nq=33, Nk=64, H=2, Hkv=2, D=128, far=200),
+    dict(B=2, Nq=5, Nk=64, H=2, Hkv=2, D=64, causal=True, bidirectional=True, start=30),
+    dict(B=1, Nq=130, Nk=300, H=2, Hkv=2, D=64, causal=True, start=-20, far=200),
+    dict(B=2, Nq=150, Nk=400, H=2, Hkv=2, D=64, lens=[90, 0], buckets=64, far=300),
+]
+
+
+@pytest.mark.parametrize('dt', HALF, ids=ids)
+@pytest.mark.parametrize('fill', [float('nan'), float('inf'), -float('inf')])
+@pytest.mark.parametrize('case', UNUSED, ids=attn_id)
+def test_table_entries_that_no_pair_uses(case, fill, dt):
+    """Distances that no query sees (keys after it of a causal call, beyond the lengths, of rows that do not exist) may hold anything."""
+    host, at, see, kw = attn_case(case, dt)
+    used = torch.zeros(host['table'].shape[0], dtype=torch.bool)
+    used[at[see.expand_as(at)].unique()] = True
+    assert not used.all()
+    dout = rnd(*host['q'].shape, seed=5).to(dt).to(DEV)
+    results = []
+    for f in (0.0, fill):
+        table = host['table'].clone()
+        table[~used] = f
+        leaves = [t.to(DEV).requires_grad_(True) for t in (host['q'], host['k'], host['v'], table)]
+        with torch.no_grad():
+            plain = ops.biased_attention(*leaves, **kw)
+        out = ops.biased_attention(*leaves, **kw)
+        results.append([plain, out] + list(torch.autograd.grad(out, leaves, dout)))
+    for name, a, b in zip(('inference', 'out', 'dq', 'dk', 'dv', 'dtable'), *results):
+        assert torch.equal(a, b), name
+    assert not results[1][-1][~used].any()
+
+
 @pytest.mark.parametrize('C', [40, 203, 1024])
 def test_norm_gradients_asked_for_one_at_a_time(C):
     """Each gradient alone equals, bit for bit, the one asked for with all others; gates of channels, samples and tokens."""
