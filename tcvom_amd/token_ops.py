@@ -10,7 +10,7 @@ needs these.  The reference has no counterpart.
 
 Element types are arguments: bf16, fp16 and, for the bias matrix and the norms, fp32, in either build of the library.  16-bit results are
 rounded to nearest even without saturation.  Gradients are added in a fixed order: equal calls give equal bits.  First derivatives
-only.  A call may be captured into a graph, its backward too -- while no eager graph of the same leaves lives (torch would join the capture
+only, in reverse mode.  A call may be captured into a graph, its backward too -- while no eager graph of the same leaves lives (torch would join the capture
 to that graph's stream and end the process).
 """
 import ctypes as C
@@ -18,6 +18,7 @@ import functools
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -73,7 +74,10 @@ def _first_order(backward):
 
 
 def _tracked(*tensors):
-    """Whether autograd has to see the call."""
+    """Whether autograd has to see the call: for gradients, or to refuse forward-mode derivatives (dual tensors need no gradient and
+    have an address like others; torch raises NotImplementedError for a function without a rule for them, under no_grad too)."""
+    if forward_ad._current_level >= 0:
+        return True
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:

@@ -12,6 +12,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from tcvom_amd import _lib as L
 from tcvom_amd import ops
@@ -861,6 +862,24 @@ def test_second_derivatives_are_refused():
     g, = torch.autograd.grad(h.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), x)
+
+
+@pytest.mark.parametrize('grad', [True, False])
+def test_forward_mode_derivatives_are_refused(grad):
+    q, t = rnd(1, 4, 2, 64, seed=1).bfloat16().to(DEV), rnd(32, 2, seed=2).float().to(DEV)
+    x, w = rnd(4, 64, seed=3).float().to(DEV), torch.ones(64, device=DEV)
+    calls = [(ops.biased_attention, [q, q, q, t]), (ops.relative_position_bias, [t, 4, 4]), (ops.block_norm, [x, x, w, None, w, 1.0, 1.0, w])]
+    for f, args in calls:
+        with torch.set_grad_enabled(grad), fwd.dual_level():
+            for i, a in enumerate(args):
+                if isinstance(a, torch.Tensor):
+                    with pytest.raises(NotImplementedError):
+                        f(*args[:i], fwd.make_dual(a, torch.ones_like(a)), *args[i + 1:])
+            inside = f(*args)
+        with torch.no_grad():
+            outside = f(*args)
+        first = lambda r: r[0] if isinstance(r, tuple) else r  # noqa: E731
+        assert torch.equal(first(inside), first(outside))
 
 
 def test_norm_of_no_tokens():

@@ -5,6 +5,7 @@ from fractions import Fraction
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from tcvom_amd import _lib as L
 from tcvom_amd import ops, token_ops
@@ -176,3 +177,21 @@ def test_cpu_tensors_are_refused():
         ops.block_norm(q, q, pre_weight=torch.ones(8))
     with pytest.raises(TypeError):
         ops.block_norm(None, q)
+
+
+@pytest.mark.parametrize('grad', [True, False])
+def test_forward_mode_derivatives_are_refused(grad, monkeypatch):
+    """A dual tensor needs no gradient and has an address: the call must not pass autograd by, which would drop the tangent."""
+    monkeypatch.setattr(token_ops, '_check_cuda', lambda *a: None)
+    monkeypatch.setattr(token_ops, '_rel_bias', lambda table, *a: table.detach().clone())
+    monkeypatch.setattr(token_ops, '_attention', lambda q, *a: (q.detach().clone(), None, None))
+    monkeypatch.setattr(token_ops, '_block_norm', lambda x, *a: (x.detach().clone(), None, None))
+    t, q, x = torch.randn(32, 2), torch.randn(1, 4, 2, 8).bfloat16(), torch.randn(3, 8)
+    with torch.set_grad_enabled(grad), fwd.dual_level():
+        dual = lambda a: fwd.make_dual(a, torch.ones_like(a))  # noqa: E731
+        for call in (lambda: ops.relative_position_bias(dual(t), 4, 4), lambda: ops.biased_attention(q, dual(q), q, t),
+                     lambda: ops.biased_attention(q, q, q, dual(t)), lambda: ops.block_norm(x, dual(x)), lambda: ops.block_norm(x, x, gate=dual(x))):
+            with pytest.raises(NotImplementedError):
+                call()
+        assert torch.equal(ops.relative_position_bias(t, 4, 4), t)                 # no dual tensor among the arguments
+    assert torch.equal(ops.relative_position_bias(t, 4, 4), t)
