@@ -699,8 +699,9 @@ typedef struct {
 } tcvom_rel_buckets;
 
 /* out[h][i][j] = table[bucket(j - i - q_start)][h]: table fp32 [num_buckets][heads], out [heads][q_len][k_len] of `type`.
- * _bwd: dtable[b][h] = sum of dout over the elements with that bucket; work = tcvom_relbias_bwd_work(...) floats.  Fixed order of
- * additions: equal calls give equal bits. */
+ * _bwd: dtable[b][h] = sum of dout over the elements with that bucket, for up to TCVOM_MAX_RELBIAS_BWD_QUERIES rows;
+ * work = tcvom_relbias_bwd_work(...) floats.  Fixed order of additions: equal calls give equal bits. */
+#define TCVOM_MAX_RELBIAS_BWD_QUERIES (65535 * 16)
 int tcvom_relbias_fwd(const float* table, void* out, const tcvom_rel_buckets* buckets, int32_t heads, int64_t q_len, int64_t k_len,
                       int64_t q_start, int32_t type, void* stream);
 int64_t tcvom_relbias_bwd_work(const tcvom_rel_buckets* buckets, int32_t heads, int64_t q_len);
@@ -729,7 +730,8 @@ int tcvom_attn_fwd(const tcvom_attn_desc* d, const void* q, const void* k, const
                    float* lse, float* work, int64_t work_floats, void* stream);
 /* Gradients from what the forward read and wrote (lse; out32 where dtable is asked for, else it is not read); dout with strides like
  * q's; dq / dk / dv contiguous, dtable (or NULL: not asked for) fp32 like table.  Keys and rows without a pair get zeros.  Fixed order
- * of additions. */
+ * of additions.  Forward and backward: B H ceil(Nq / 128), backward B Hkv ceil(Nk / 128) + H too, are at most TCVOM_MAX_ATTN_WORKGROUPS. */
+#define TCVOM_MAX_ATTN_WORKGROUPS (1 << 23)
 int64_t tcvom_attn_bwd_work(const tcvom_attn_desc* d);
 int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const void* k, const void* v, const float* table, const void* out,
                    const float* out32, const float* lse, const void* dout, const int64_t* dout_stride, void* dq, void* dk, void* dv,

@@ -63,6 +63,7 @@ class SnDot(C.Structure):
 
 
 MAX_BUCKETS, MAX_BUCKET_STARTS, MAX_BUCKET_REACH, MAX_NORM_CHANNELS = 256, 128, 1024, 8192
+MAX_RELBIAS_BWD_QUERIES, MAX_ATTN_WORKGROUPS = 65535 * 16, 1 << 23
 
 
 class RelBuckets(C.Structure):

@@ -283,6 +283,6 @@ __device__ __forceinline__ bool fill_line(float* line, const AttnArgs& a, int h,
 static inline size_t line_bytes(const AttnArgs& a) { return sizeof(float) * (line_reach(a.bk) + line_right(a.bk) + 1 + 2 * MARGIN); }
 
 // host side
-constexpr long long ATTN_MAX_WGS = 1 << 23;            // a grid has fewer than 2^32 threads
+static_assert(TCVOM_MAX_ATTN_WORKGROUPS < (1LL << 32) / 256, "a grid has fewer than 2^32 threads");
 int attn_check(const char* who, const tcvom_attn_desc* d, AttnArgs* a);
 static inline int attn_width(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }

@@ -491,7 +491,7 @@ extern "C" int tcvom_attn_fwd(const tcvom_attn_desc* d, const void* q, const voi
     if (d->B == 0 || d->Nq == 0) return 0;
     TCVOM_CHECK_ARG(q && table && out && (d->Nk == 0 || (k && v)), "attn_fwd: null tensor");
     TCVOM_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out32), "attn_fwd: tensors start at multiples of 16 bytes");
-    TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 128) <= ATTN_MAX_WGS, "attn_fwd: %d sequences x %d heads x %d queries", d->B, d->H, d->Nq);
+    TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 128) <= TCVOM_MAX_ATTN_WORKGROUPS, "attn_fwd: %d sequences x %d heads x %d queries", d->B, d->H, d->Nq);
     TCVOM_CHECK_ARG(work_floats >= tcvom_attn_fwd_work(d) && (work || tcvom_attn_fwd_work(d) == 0), "attn_fwd: %lld floats of workspace",
                     (long long)work_floats);
     a.q = q; a.k = k; a.v = v; a.table = table; a.out = out; a.out32 = out32; a.lse = lse; a.partial = work;

@@ -519,7 +519,8 @@ __global__ __launch_bounds__(256) void attn_heads_kernel(AttnArgs a) {
 }
 
 static bool attn_apart(const tcvom_attn_desc* d) {
-    return d->H > d->Hkv && (long long)d->B * d->Hkv * cdiv(d->Nk, 128) < 2048;
+    const long long tiles = cdiv(d->Nk, 128);
+    return d->H > d->Hkv && tiles * d->B * d->Hkv < 2048 && tiles * d->B * d->H + d->H <= TCVOM_MAX_ATTN_WORKGROUPS;
 }
 
 template <class T, int DP>
@@ -552,7 +553,8 @@ extern "C" int tcvom_attn_bwd(const tcvom_attn_desc* d, const void* q, const voi
     TCVOM_CHECK_ARG(!dtable || out32, "attn_bwd: the table's gradient needs the output in 32 bits");
     TCVOM_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out32) && aligned16(dout) &&
                         aligned16(dq) && aligned16(dk) && aligned16(dv), "attn_bwd: tensors start at multiples of 16 bytes");
-    TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 128) <= ATTN_MAX_WGS && (long long)d->B * d->H * cdiv(d->Nk, 128) <= ATTN_MAX_WGS,
+    TCVOM_CHECK_ARG((long long)d->B * d->H * cdiv(d->Nq, 128) <= TCVOM_MAX_ATTN_WORKGROUPS &&
+                        (long long)d->B * d->Hkv * cdiv(d->Nk, 128) + d->H <= TCVOM_MAX_ATTN_WORKGROUPS,
                     "attn_bwd: %d sequences x %d heads x %d queries, %d keys", d->B, d->H, d->Nq, d->Nk);
     TCVOM_CHECK_ARG(work_floats >= tcvom_attn_bwd_work(d) && aligned16(work), "attn_bwd: %lld floats of workspace", (long long)work_floats);
     for (int n = 0; n < 3; ++n) {

@@ -82,6 +82,8 @@ extern "C" int tcvom_relbias_fwd(const float* table, void* out, const tcvom_rel_
 // fixed shape, and written once: no atomics, equal calls give equal bits.  12 x 2041 x 2041 fp32: 62 us = 3.2 TB/s (a sum that only reads
 // reaches 3.9); 8 x 1024 x 1024 bf16: 7.1 us.  Chunks of 8, 32 or 64 rows: no faster.
 constexpr int BIAS_ROWS = 16;
+// chunks of rows are blocks of the grid's second dimension, and a bucket's entries of all chunks are counted in 32 bits
+static_assert(TCVOM_MAX_RELBIAS_BWD_QUERIES <= 65535 * BIAS_ROWS && TCVOM_MAX_RELBIAS_BWD_QUERIES / BIAS_ROWS * (TCVOM_MAX_BUCKET_REACH + 1LL) < (1LL << 31), "");
 template <class T, int LANES>
 __global__ __launch_bounds__(256) void relbias_bwd_kernel(const T* dout, float* part, tcvom_rel_buckets bk, long long Nq, long long Nk,
                                                           long long q_start) {
@@ -199,7 +201,7 @@ extern "C" int tcvom_relbias_bwd(const void* dout, float* dtable, float* work, i
     TCVOM_CHECK_ARG(dout && dtable && work && heads > 0 && heads <= 65535 && q_len > 0 && k_len > 0,
                     "relbias_bwd: heads=%d q_len=%lld k_len=%lld", heads, (long long)q_len, (long long)k_len);
     TCVOM_CHECK_ARG(type >= TCVOM_TYPE_F32 && type <= TCVOM_TYPE_F16, "relbias_bwd: type %d", type);
-    TCVOM_CHECK_ARG(q_len <= 65535LL * BIAS_ROWS && (int64_t)cdiv(q_len, BIAS_ROWS) * TCVOM_MAX_BUCKET_REACH < (1LL << 31) && k_len < (1LL << 31) && q_start < (1LL << 40) && q_start > -(1LL << 40),
+    TCVOM_CHECK_ARG(q_len <= TCVOM_MAX_RELBIAS_BWD_QUERIES && k_len < (1LL << 31) && q_start < (1LL << 40) && q_start > -(1LL << 40),
                     "relbias_bwd: lengths");
     if (const int rc = check_buckets("relbias_bwd", buckets)) return rc;
     const tcvom_rel_buckets bk = pad_buckets(*buckets);

@@ -155,7 +155,7 @@ def relative_position_bias(table, q_len, k_len, max_distance=128, bidirectional=
     table: fp32 [buckets, heads].  Bidirectional: half the buckets for keys behind the query, half for keys after it (distance
     |j - i - q_start|); one-sided: every key after the query counts as distance 0.  The first half of a side's buckets hold one
     distance each, the others grow geometrically up to max_distance (at most 1024), the last holds everything beyond.  q_start:
-    position of the first query."""
+    position of the first query.  Where the table needs a gradient: at most 1048560 queries."""
     _check_cuda('relative_position_bias', (table,))
     _check_table('relative_position_bias', table)
     if dtype not in _TYPES:
@@ -165,7 +165,10 @@ def relative_position_bias(table, q_len, k_len, max_distance=128, bidirectional=
     if not -(1 << 40) < q_start < 1 << 40:
         raise ValueError('relative_position_bias: q_start %d' % q_start)
     buckets = rel_buckets(table.shape[0], int(max_distance), bool(bidirectional))
-    run = _RelBias.apply if _tracked(table) else _rel_bias
+    tracked = _tracked(table)
+    if tracked and q_len > L.MAX_RELBIAS_BWD_QUERIES:
+        raise ValueError('relative_position_bias: %d queries with a gradient (at most %d)' % (q_len, L.MAX_RELBIAS_BWD_QUERIES))
+    run = _RelBias.apply if tracked else _rel_bias
     return run(table, buckets, int(q_len), int(k_len), int(q_start), dtype)
 
 
@@ -285,6 +288,8 @@ def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causa
     buckets = rel_buckets(table.shape[0], int(max_distance), bool(not causal if bidirectional is None else bidirectional))
     args = (buckets, int(causal), scale, _c(k_lens), key_mask, int(q_start), _c(q_starts))
     if _tracked(q, k, v, table):
+        if B * Hkv * -(-Nk // 128) + H > L.MAX_ATTN_WORKGROUPS:
+            raise ValueError('%s: %d sequences x %d key heads x %d keys with gradients (at most 2^30 rows of keys)' % (name, B, Hkv, Nk))
         return _BiasedAttention.apply(q, k, v, table, *args)
     return _attention(_rows16(q), _rows16(k), _rows16(v), _c(table), False, False, *args)[0]
 

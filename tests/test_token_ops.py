@@ -195,3 +195,35 @@ def test_forward_mode_derivatives_are_refused(grad, monkeypatch):
                 call()
         assert torch.equal(ops.relative_position_bias(t, 4, 4), t)                 # no dual tensor among the arguments
     assert torch.equal(ops.relative_position_bias(t, 4, 4), t)
+
+
+def test_what_the_gradient_cannot_do_is_refused_by_the_call(monkeypatch):
+    """A call whose backward would be refused is refused itself, and only then."""
+    monkeypatch.setattr(token_ops, '_check_cuda', lambda *a: None)
+    monkeypatch.setattr(token_ops, '_rel_bias', lambda table, *a: table.detach())
+    monkeypatch.setattr(token_ops, '_attention', lambda q, *a: (q.detach(), None, None))
+    t = torch.zeros(32, 2)
+    leaf = torch.zeros(32, 2, requires_grad=True)
+    limit = L.MAX_RELBIAS_BWD_QUERIES
+    ops.relative_position_bias(t, limit + 1, 1)
+    ops.relative_position_bias(leaf, limit, 1)
+    with pytest.raises(ValueError, match='with a gradient'):
+        ops.relative_position_bias(leaf, limit + 1, 1)
+    b = token_ops.rel_buckets(32, 128, True)
+    for n, why in ((limit, 'workspace'), (limit + 1, 'lengths')):
+        with pytest.raises(L.TcvomError, match=why):
+            L.call('tcvom_relbias_bwd', ANY, ANY, ANY, 0, C.byref(b), 2, n, 4, 0, 0, None)
+    q, rows = torch.zeros(4, 1, 2, 8).bfloat16(), lambda n: torch.zeros(4, 1, 1, 8).bfloat16().expand(4, n, 1, 8)
+    many, most = rows(1 << 28), rows((1 << 28) - 128)
+    ops.biased_attention(q, many, many, t)
+    ops.biased_attention(q, most, most, leaf)
+    with pytest.raises(ValueError, match='with gradients'):
+        ops.biased_attention(q, many, many, leaf)
+
+
+@pytest.mark.parametrize('kw,why', [(dict(B=1, Nq=1, Nk=1 << 25, H=64, Hkv=1, D=8), 'workspace'), (dict(B=4, Nq=1, Nk=1 << 28, H=2, Hkv=1, D=8), 'keys'),
+                                    (dict(B=4, Nq=1, Nk=(1 << 28) - 128, H=2, Hkv=1, D=8), 'workspace'), (dict(B=1, Nq=1, Nk=128 * 2047, H=8192, Hkv=1, D=8), 'workspace')])
+def test_long_keys_and_the_gradient(kw, why):
+    """The limit counts the workgroups that there are: of key heads (64 heads on one of 2^25 keys are 2^18), apart only where they fit."""
+    with pytest.raises(L.TcvomError, match=why):
+        L.call('tcvom_attn_bwd', C.byref(desc(**kw)), ANY, ANY, ANY, ANY, ANY, ANY, ANY, ANY, (C.c_int64 * 3)(8, 8, 8), ANY, ANY, ANY, ANY, ANY, 0, None)
