@@ -10,8 +10,9 @@ needs these.  The reference has no counterpart.
 
 Element types are arguments: bf16, fp16 and, for the bias matrix and the norms, fp32, in either build of the library.  16-bit results are
 rounded to nearest even without saturation.  Gradients are added in a fixed order: equal calls give equal bits.  First derivatives
-only, in reverse mode.  A call may be captured into a graph, its backward too -- while no eager graph of the same leaves lives (torch would join the capture
-to that graph's stream and end the process).
+only, in reverse mode.  A call may be captured into a graph, its backward too -- while no graph that an eager call on the default
+stream made of the same leaves lives: torch would join the capture to that stream and end the process.  Such a backward is refused where the
+eager call was one of these operators (a leaf that only other operations hold is not known here).
 """
 import ctypes as C
 import functools
@@ -62,12 +63,35 @@ def _launch(device, name, *args):
         return L.call(name, *args, stream)
 
 
+_AccumulateGrad = type(torch.empty(0, requires_grad=True).view(0).grad_fn.next_functions[0][0])
+_ON_DEFAULT_STREAM = 'tcvom_amd: leaf of an eager graph on the default stream'
+
+
+def _mark_leaves(device, out):
+    """Marks the nodes that will add the gradients of the leaves of `out`, made by a call on the default stream.  Such a node belongs to the
+    stream of its first use and is shared by every graph of its leaf; it, and the mark, go with the last of them."""
+    if out.grad_fn is not None and torch._C._cuda_getCurrentRawStream(device) == 0:
+        for node, _ in out.grad_fn.next_functions:
+            if type(node) is _AccumulateGrad:
+                node.metadata[_ON_DEFAULT_STREAM] = True
+
+
+def _refuse_marked_leaves(ctx):
+    """In a backward pass that is being captured."""
+    for node, _ in ctx.next_functions:
+        if type(node) is _AccumulateGrad and _ON_DEFAULT_STREAM in node.metadata:
+            raise RuntimeError('%s: captured into a graph while an eager graph of the default stream holds the same leaf (shape %s).  Drop the '
+                               'results of eager calls first, or make them on another stream' % (ctx.name(), tuple(node.variable.shape)))
+
+
 def _first_order(backward):
     """once_differentiable, whose wrapping is left out of the usual backward (which builds no graph)."""
     guarded = once_differentiable(backward)
 
     @functools.wraps(backward)
     def run(ctx, *grads):
+        if torch.cuda.is_current_stream_capturing():
+            _refuse_marked_leaves(ctx)
         return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
     return run
@@ -168,8 +192,12 @@ def relative_position_bias(table, q_len, k_len, max_distance=128, bidirectional=
     tracked = _tracked(table)
     if tracked and q_len > L.MAX_RELBIAS_BWD_QUERIES:
         raise ValueError('relative_position_bias: %d queries with a gradient (at most %d)' % (q_len, L.MAX_RELBIAS_BWD_QUERIES))
-    run = _RelBias.apply if tracked else _rel_bias
-    return run(table, buckets, int(q_len), int(k_len), int(q_start), dtype)
+    args = (table, buckets, int(q_len), int(k_len), int(q_start), dtype)
+    if not tracked:
+        return _rel_bias(*args)
+    out = _RelBias.apply(*args)
+    _mark_leaves(table.get_device(), out)
+    return out
 
 
 # =============================================================================================
@@ -290,7 +318,9 @@ def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causa
     if _tracked(q, k, v, table):
         if B * Hkv * -(-Nk // 128) + H > L.MAX_ATTN_WORKGROUPS:
             raise ValueError('%s: %d sequences x %d key heads x %d keys with gradients (at most 2^30 rows of keys)' % (name, B, Hkv, Nk))
-        return _BiasedAttention.apply(q, k, v, table, *args)
+        out = _BiasedAttention.apply(q, k, v, table, *args)
+        _mark_leaves(q.get_device(), out)
+        return out
     return _attention(_rows16(q), _rows16(k), _rows16(v), _c(table), False, False, *args)[0]
 
 
@@ -409,6 +439,7 @@ def block_norm(x, y, post_weight=None, post_bias=None, gate=None, branch_scale=1
     tensors = (x, y, post_weight, post_bias, gate, pre_weight, pre_bias)
     if _tracked(*tensors):
         xo, h = _BlockNorm.apply(*tensors, *args)
+        _mark_leaves(x.get_device(), h if xo is None else xo)
     else:
         xo, h, _ = _block_norm(*[_c(t) for t in tensors], False, *args)
     return (x if y is None else xo), h

@@ -823,6 +823,32 @@ def test_captured_calls_replay_on_new_inputs():
         torch.cuda.synchronize()
 
 
+def test_captured_backward_beside_an_eager_graph_is_refused():
+    """... before torch joins the capture to the default stream; the capture itself stays whole, and one without the eager graph goes on."""
+    x, y, w = rnd(5, 64, seed=1).float().to(DEV), rnd(5, 64, seed=2).float().to(DEV), torch.ones(64, device=DEV, requires_grad=True)
+    d = torch.ones_like(x)
+    eager = ops.block_norm(x, y, post_weight=w)[0]
+    refused, ok = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(refused):
+        out = ops.block_norm(x, y, post_weight=w)[0]
+        with pytest.raises(RuntimeError, match='eager graph of the default stream'):
+            torch.autograd.grad(out, w, d)
+    refused.replay()
+    assert torch.equal(out, eager)
+    want, = torch.autograd.grad(eager, w, d)
+    del eager, out
+    with torch.cuda.graph(ok):
+        got, = torch.autograd.grad(ops.block_norm(x, y, post_weight=w)[0], w, d)
+    for n in (1, 2):
+        y.mul_(2 * n)
+        ok.replay()
+        torch.cuda.synchronize()
+        eager = ops.block_norm(x, y, post_weight=w)[0]
+        assert torch.equal(got, torch.autograd.grad(eager, w, d)[0])
+    assert not torch.equal(got, want)
+
+
 def test_refusals():
     z = lambda *s, **k: torch.zeros(s, device=DEV, **k)  # noqa: E731
     b16 = dict(dtype=torch.bfloat16)

@@ -199,6 +199,7 @@ def test_forward_mode_derivatives_are_refused(grad, monkeypatch):
 
 def test_what_the_gradient_cannot_do_is_refused_by_the_call(monkeypatch):
     """A call whose backward would be refused is refused itself, and only then."""
+    monkeypatch.setattr(torch._C, '_cuda_getCurrentRawStream', lambda device: 0)
     monkeypatch.setattr(token_ops, '_check_cuda', lambda *a: None)
     monkeypatch.setattr(token_ops, '_rel_bias', lambda table, *a: table.detach())
     monkeypatch.setattr(token_ops, '_attention', lambda q, *a: (q.detach(), None, None))
@@ -227,3 +228,47 @@ def test_long_keys_and_the_gradient(kw, why):
     """The limit counts the workgroups that there are: of key heads (64 heads on one of 2^25 keys are 2^18), apart only where they fit."""
     with pytest.raises(L.TcvomError, match=why):
         L.call('tcvom_attn_bwd', C.byref(desc(**kw)), ANY, ANY, ANY, ANY, ANY, ANY, ANY, ANY, (C.c_int64 * 3)(8, 8, 8), ANY, ANY, ANY, ANY, ANY, 0, None)
+
+
+def test_captured_backward_beside_an_eager_graph_is_refused(monkeypatch):
+    """Refused while a graph of the default stream holds the leaf, and no longer; by all three, for any of their leaves."""
+    where = dict(stream=0, capturing=False)
+    monkeypatch.setattr(token_ops, '_check_cuda', lambda *a: None)
+    monkeypatch.setattr(token_ops, '_launch', lambda *a: None)
+    monkeypatch.setattr(token_ops, '_rel_bias', lambda t, *a: t.new_zeros(2, 4, 4))
+    monkeypatch.setattr(token_ops, '_attention', lambda q, *a: (q.detach().clone(), q.detach().float(), q.new_zeros(1, 2, 4).float()))
+    monkeypatch.setattr(token_ops, '_block_norm', lambda x, *a: (x.detach().clone(), None, x.new_zeros(3, 4)))
+    monkeypatch.setattr(torch._C, '_cuda_getCurrentRawStream', lambda device: where['stream'])
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: where['capturing'])
+
+    def on(stream, capturing=False):
+        where.update(stream=stream, capturing=capturing)
+
+    t, q, x, y = torch.randn(32, 2), torch.randn(1, 4, 2, 8).bfloat16(), torch.randn(3, 8), torch.randn(3, 8)
+    calls = [(lambda t: ops.relative_position_bias(t, 4, 4), t), (lambda t: ops.biased_attention(q, q, q, t), t), (lambda k: ops.biased_attention(q, k, q, t), q),
+             (lambda y: ops.block_norm(x, y)[0], y), (lambda g: ops.block_norm(x, y, gate=g)[0], y)]
+    for call, value in calls:
+        leaf = value.clone().requires_grad_(True)
+
+        def captured(source=leaf):
+            on(7, True)
+            out = call(source)
+            return torch.autograd.grad(out, leaf, torch.zeros_like(out))
+
+        on(0)
+        eager = call(leaf)
+        with pytest.raises(RuntimeError, match='eager graph of the default stream'):
+            captured()
+        captured(leaf * 1)                                   # not through this operator's own leaf
+        on(0)
+        torch.autograd.grad(eager, leaf, torch.zeros_like(eager))                  # the eager pass itself
+        del eager
+        captured()
+        on(3)
+        eager = call(leaf)                                   # another stream: the capture joins it and leaves it again
+        captured()
+        on(0)
+        with torch.no_grad():
+            call(leaf)
+        del eager
+        captured()
