@@ -253,7 +253,7 @@ __device__ __forceinline__ void sum_table(const AttnArgs& a, int h, double* red)
 // dK^T = Q^T dS.
 //
 // Causal key tiles have very different numbers of queries, and a group of heads that share keys multiplies a workgroup's work: with
-// few workgroups (attn_apart) each head of a group gets workgroups of its own, which write fp32 partial sums [2][B][Nk][H][D] that
+// few workgroups (attn_apart says how few) each head of a group gets workgroups of its own, which write fp32 partial sums [2][B][Nk][H][D] that
 // attn_heads_kernel adds in order.  The tiles with most queries come first.
 //
 // Bound as above, 4 products a score.  4 x 1024 tokens, 8 heads of 64, fp16: 48 us; 2 x 4080 causal, 16 heads of 128 on 4, bf16: 380-440 us =
@@ -518,9 +518,16 @@ __global__ __launch_bounds__(256) void attn_heads_kernel(AttnArgs a) {
     *reinterpret_cast<typename Mma<T>::v4*>((T*)(blockIdx.y ? a.dv : a.dk) + row * a.D + c) = v;
 }
 
+// Heads apart: more workgroups, of equal lengths, for 8 bytes of workspace a channel of every head's keys and a pass over them.  The chip holds 512
+// workgroups.  dk / dv apart against together, 16 heads on 4, bf16, us:
+//     not causal, 2048 tokens, width 64: 384 workgroups (together) 333 / 363, 448: 363 / 350, 512: 438 / 408, 1024: 786 / 713; width 128, 448: 652 / 619
+//     causal, key heads a multiple of 8 (longest tiles first, work_item): 512: 249 / 290, 640: 303 / 287, 1024: 500 / 427; width 128, 512: 452 / 560,
+//     640: 569 / 538, 1024: 941 / 749
+//     causal, others (tiles of a head one after the other, the last ones alone): 576: 264 / 348, 832: 392 / 504, 1152: 1010 / 1253, 1920: 1615 / 1889
 static bool attn_apart(const tcvom_attn_desc* d) {
-    const long long tiles = cdiv(d->Nk, 128);
-    return d->H > d->Hkv && tiles * d->B * d->Hkv < 2048 && tiles * d->B * d->H + d->H <= TCVOM_MAX_ATTN_WORKGROUPS;
+    const long long tiles = cdiv(d->Nk, 128), heads = (long long)d->B * d->Hkv;
+    const int limit = !d->causal ? 447 : heads % 8 == 0 ? 512 : 2047;
+    return d->H > d->Hkv && tiles * heads <= limit && tiles * d->B * d->H + d->H <= TCVOM_MAX_ATTN_WORKGROUPS;
 }
 
 template <class T, int DP>

@@ -445,6 +445,14 @@ def test_gradients_of_small_and_large_douts(case, which, std, dt):
     assert rms < 1, rms
 
 
+@pytest.mark.parametrize('D', [32, 64, 128])
+@pytest.mark.parametrize('c', [dict(B=260, Nq=20, Nk=33, Hkv=2), dict(B=260, Nq=33, Nk=20, Hkv=2, causal=True), dict(B=1025, Nq=9, Nk=17, Hkv=2, causal=True, start=8)],
+                         ids=attn_id)
+def test_heads_that_share_keys_in_one_workgroup(c, D):
+    """So many sequences that dk and dv of a group of heads are summed by the workgroup that owns the keys; with fewer they meet in memory."""
+    test_attention_and_its_gradients(dict(c, H=4, D=D), torch.float16 if D == 64 else torch.bfloat16)
+
+
 UNUSED = [
     dict(B=1, Nq=200, Nk=200, H=2, Hkv=1, D=64, causal=True, bidirectional=True, buckets=16, far=20),
     dict(B=2, Nq=33, Nk=64, H=2, Hkv=2, D=32, far=200),

@@ -272,3 +272,18 @@ def test_captured_backward_beside_an_eager_graph_is_refused(monkeypatch):
             call(leaf)
         del eager
         captured()
+
+
+@pytest.mark.parametrize('causal,heads,most', [(0, 4, 447), (1, 8, 512), (1, 3, 2047)])
+def test_workspace_of_heads_apart(causal, heads, most):
+    """Partial sums of every head only where few workgroups would own the keys."""
+    def floats(wgs, H=64):
+        B, Hkv, Nk, Nq = heads, 1, 128 * wgs // heads, 128
+        rows = B * H * Nq + B * H * 32
+        return L.call('tcvom_attn_bwd_work', C.byref(desc(B=B, Hkv=Hkv, H=H, Nk=Nk, Nq=Nq, causal=causal))) - rows, 2 * B * Nk * H * 64
+
+    below, above = most // heads * heads, (most // heads + 1) * heads
+    got, partial = floats(below)
+    assert got == partial
+    assert floats(above)[0] == 0
+    assert floats(below, H=1)[0] == 0
