@@ -197,6 +197,22 @@ def test_block_norm_and_its_gradients(case, types):
     assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize('types', NORM_TYPES, ids=lambda t: '%s-%s' % (ids(t[0]), ids(t[1])))
+def test_block_norm_types(types):
+    """x' has x's type and h has y's, or x's without y; each within the rounding of that type."""
+    xt, yt = types
+    x, y, w = rnd(6, 72, seed=1).to(xt), rnd(6, 72, seed=2).to(yt), 1 + rnd(72, seed=3, std=0.2).float()
+    for grad in (False, True):
+        dev = [t.to(DEV).requires_grad_(grad) for t in (x, y, w)]
+        xo, h = ops.block_norm(dev[0], dev[1], post_weight=dev[2], pre_weight=dev[2])
+        h0 = ops.block_norm(dev[0], None, pre_weight=dev[2])[1]
+        wxo, wh = norm64(x.double(), y.double(), w.double(), None, None, 1, 1.0, 1.0, w.double(), None, False, 1e-6)
+        wh0 = norm64(x.double(), None, None, None, None, 1, 1.0, 1.0, w.double(), None, False, 1e-6)[1]
+        for got, want, t in ((xo, wxo, xt), (h, wh, yt), (h0, wh0, xt)):
+            assert got.dtype == t
+            close(got, want, step(t) * want.abs() * (1 + 1e-3) + 2e-6 * (1 + want.abs().max()))
+
+
 def test_block_norm_passes_only_one_gradient():
     x, y, w = rnd(4, 6, 256, seed=1).float(), rnd(4, 6, 256, seed=2).float(), 1 + rnd(256, seed=3, std=0.1).float()
     for which in (0, 1):
@@ -451,6 +467,28 @@ def test_gradients_of_small_and_large_douts(case, which, std, dt):
 def test_heads_that_share_keys_in_one_workgroup(c, D):
     """So many sequences that dk and dv of a group of heads are summed by the workgroup that owns the keys; with fewer they meet in memory."""
     test_attention_and_its_gradients(dict(c, H=4, D=D), torch.float16 if D == 64 else torch.bfloat16)
+
+
+@pytest.mark.parametrize('dt', HALF, ids=ids)
+@pytest.mark.parametrize('case', FROZEN, ids=attn_id)
+def test_gradient_of_v_with_and_without_the_tables(case, dt):
+    """Another forward kernel and log-sum, the same dv within the rounding of p and of the result; and equal bits alone and with the others."""
+    host, at, see, kw = attn_case(case, dt)
+    u, G = step(dt), case['H'] // case['Hkv']
+    ref = {n: t.double().requires_grad_(n == 'v') for n, t in host.items()}
+    want, p = attention64(ref['q'], ref['k'], ref['v'], ref['table'], at, see, case['D'] ** -0.5)
+    dout = rnd(*host['q'].shape, seed=5).to(dt)
+    w, = torch.autograd.grad(want, ref['v'], dout.double())
+    sums = torch.einsum('bhij,bihd->bjhd', p.detach(), dout.double().abs())
+    sums = sums.reshape(sums.shape[0], sums.shape[1], case['Hkv'], G, case['D']).sum(3)
+    tiny = 0.0 if dt == torch.bfloat16 else 2.0 ** -25
+    got = {}
+    for wanted in ('v', 'v table', 'q k v', 'q k v table'):
+        leaf = {n: t.to(DEV).requires_grad_(n in wanted.split()) for n, t in host.items()}
+        out = ops.biased_attention(leaf['q'], leaf['k'], leaf['v'], leaf['table'], **kw)
+        got[wanted], = torch.autograd.grad(out, leaf['v'], dout.to(DEV))
+        close(got[wanted], w, u * 1.01 * w.abs() + (u + 2e-5) * sums + tiny, wanted)
+    assert torch.equal(got['v'], got['q k v']) and torch.equal(got['v table'], got['q k v table'])
 
 
 UNUSED = [
