@@ -309,6 +309,24 @@ def other_configs(steps, warmup):
     return out
 
 
+def compact(result):
+    """The line for stdout, short enough for readers that keep a few KB of it only: of the side runs their figures and dominant kernel, of
+    the roofline the families with at least 2 % of the time.  The whole object goes to stderr."""
+    out = dict(result)
+    if 'roofline' in out:
+        r = out['roofline'] = {k: v for k, v in out['roofline'].items() if k != 'algorithmic_mib_per_launch'}
+        least = 0.02 * sum(e['ms'] for e in r['all_igemm'].values())
+        r['all_igemm'] = {k: e for k, e in r['all_igemm'].items() if e['ms'] >= least}
+    if 'other_configs' in out:
+        keep = ('value', 'unit', 'ms_per_step', 'steps', 'dtype', 'window_mfma_frac', 'final_loss', 'error')
+        out['other_configs'] = {}
+        for name, r in result['other_configs'].items():
+            out['other_configs'][name] = {k: r[k] for k in keep if k in r}
+            if 'roofline' in r:
+                out['other_configs'][name]['roofline'] = {k: r['roofline'][k] for k in ('kernel', 'achieved', 'frac') if k in r['roofline']}
+    return out
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument('--gpus', type=int, default=1)
@@ -606,7 +624,10 @@ def main():
                                     'dtssd_style_delta': float(torch.sqrt(((d_a - d_r)[um[:, 1]] ** 2).mean())),
                                     'max_abs_diff': float(dd.abs().max()), 'unknown_pixels': int(um.sum()), 'bound_alpha_mse': 1e-4}
                 del model_p, out_p
-        print(json.dumps(result))
+        line = compact(result)
+        if line != result:
+            print('bench.py, in full: ' + json.dumps(result), file=sys.stderr)
+        print(json.dumps(line))
     if world > 1:
         dist.destroy_process_group()
 

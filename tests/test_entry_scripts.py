@@ -497,3 +497,20 @@ def test_bench_fba_config_line():
     res = json.loads(lines[0])
     assert 'FBA+TAM' in res['metric'] and res['unit'] == 'windows/s' and res['value'] > 0 and res['n_gpus'] == 1
     assert res['roofline']['bound'] == 'mfma' and res['roofline']['achieved'] > 0 and 'all_igemm' in res['roofline']
+
+
+def test_bench_line_is_short():
+    """The line of a full default run, from one that was kept: a reader that holds the last 8 KB of stdout gets it whole, with the figures of
+    the headline and of every side run."""
+    import json
+    import bench
+    with open(os.path.join(REPO, 'profiles', 'r06_f_bench_1gpu.json')) as f:
+        full = json.loads(f.read())
+    line = bench.compact(full)
+    assert len(json.dumps(full)) > 16000 and len(json.dumps(line)) < 7500
+    for k in ('metric', 'value', 'unit', 'n_gpus', 'steps', 'warmup', 'ms_per_step', 'higher_is_better', 'scaling', 'vs_baseline', 'dtype', 'data', 'config',
+              'parity', 'hbm', 'cpu_baseline'):
+        assert line[k] == full[k], k
+    assert line['roofline']['frac'] == full['roofline']['frac'] and full['roofline']['kernel'] in line['roofline']['all_igemm']
+    assert all(full['roofline']['all_igemm'][k] == e for k, e in line['roofline']['all_igemm'].items())
+    assert {n: (r['value'], r['ms_per_step']) for n, r in line['other_configs'].items()} == {n: (r['value'], r['ms_per_step']) for n, r in full['other_configs'].items()}
