@@ -63,7 +63,7 @@ def _launch(device, name, *args):
         return L.call(name, *args, stream)
 
 
-_AccumulateGrad = type(torch.empty(0, requires_grad=True).view(0).grad_fn.next_functions[0][0])
+_AccumulateGrad = torch._C._functions.AccumulateGrad
 _ON_DEFAULT_STREAM = 'tcvom_amd: leaf of an eager graph on the default stream'
 
 

@@ -1,6 +1,9 @@
 """Token operators without a GPU: the buckets' definition, the plain implementations that the GPU tests compare with (their gradients
 against differences), and what the C entry points refuse before any launch."""
 import ctypes as C
+import os
+import subprocess
+import sys
 from fractions import Fraction
 
 import pytest
@@ -287,3 +290,10 @@ def test_workspace_of_heads_apart(causal, heads, most):
     assert got == partial
     assert floats(above)[0] == 0
     assert floats(below, H=1)[0] == 0
+
+
+@pytest.mark.parametrize('mode', ['no_grad', 'inference_mode'])
+def test_first_import_without_gradients(mode):
+    code = 'import torch\nwith torch.%s():\n    from tcvom_amd import ops, token_ops\n' % mode
+    code += 'x = torch.zeros(2, requires_grad=True)\nassert type((x * 2).grad_fn.next_functions[0][0]) is token_ops._AccumulateGrad'
+    subprocess.run([sys.executable, '-c', code], check=True, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), timeout=300)
