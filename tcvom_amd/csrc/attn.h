@@ -135,7 +135,7 @@ __device__ __forceinline__ typename Mma<T>::v8 pack_rest(const f32x16_t& p, type
 // would pass 2^15: the block's largest then becomes 2^11 .. 2^12, the sums so far follow (times a power of two: no rounding), and 2^-e
 // comes off in 32 bits at the store.  What is 2^26 times smaller than a column's largest still is a normal number.  bf16 has the exponents of
 // fp32 and needs none of it.  4 x 1024 tokens, 8 heads of 64, fp16: dq
-// 44 -> 47 us, dk / dv 42 -> 48 us; 2 x 4080 causal, 16 heads of 128 on 4: 278 -> 295 and 372 -> 378 us.
+// 41.6 -> 43.0 us, dk / dv 39.8 -> 45.3 us; 2 x 4080 causal, 16 heads of 128 on 4: 268 -> 284 and 351 -> 363 us.
 template <class T> constexpr float DS_UP = Mma<T>::shift > 0.f ? 0x1p100f : 1.f;
 template <class T, int DB>
 __device__ __forceinline__ void ds_fit(const f32x16_t& x, float& up, f32x16_t (&sums)[DB]) {

@@ -8,11 +8,12 @@ __device__ __forceinline__ float empty_or(float sum, float v) { return sum == 0.
 // K and V tiles go to LDS through registers (the next tile's loads are in flight during this tile's products), two buffers, one
 // barrier a tile.  LO (training with a gradient of the table): a second product with what rounding dropped from the probabilities.
 //
-// Bound: issuing matrix and vector instructions.  A wave alone takes 129 ns for 8 products of 32 x 32 x 16, 119 ns for 64 fma, 131 ns for 32
-// exponentials, 267 ns for all three; at width 64 a block of 32 x 32 scores costs 8 products and the vector unit as long again, and the two
-// waves a SIMD that one frame of 8 heads gives hide little of each other.  8160 x 8160 tokens, 8 heads of 64, bf16: 205 us = 665 TFLOP/s, four
-// such frames 730 us = 746 TFLOP/s (a large library product: 1340).  4 x 1024, 8 heads of 64, fp16, LO: 31 us; 2 x 4080 causal, 16 heads of
-// 128 on 4, bf16, LO: 245-270 us = 700-780 TFLOP/s.  Slower or no faster: 64 queries a wave (5 % faster at width 64 only, no registers at 128),
+// Bound: the vector unit and the matrix unit in turns.  At width 64 a block of 32 x 32 scores takes 96 vector instructions, 16 of them
+// exponentials of four times the length, and 8 products; with the two waves a SIMD that one frame of 8 heads gives, the counters see vector
+// instructions in 66 % and products in 33 % of the cycles: hardly any of the one beside the other, and a wave waits for data or a barrier
+// 22 % of its time.  Steady times (the clock of a fresh process takes some 150 calls to settle, 15 to 20 % slower until then): 8160 x 8160
+// tokens, 8 heads of 64, bf16: 182 us = 749 TFLOP/s, four such frames 647 us = 843 TFLOP/s (a large library product: 1340).  4 x 1024, 8 heads
+// of 64, fp16, LO: 28 us, one wave a SIMD; 2 x 4080 causal, 16 heads of 128 on 4, bf16, LO: 226 us = 905 TFLOP/s of its three products.  Slower or no faster: 64 queries a wave (5 % faster at width 64 only, no registers at 128),
 // scores formed a tile ahead, row sums by a product with ones, products of the two key blocks in turn, a higher wave priority for them.
 template <class T, int DP, bool LO>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
@@ -184,8 +185,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
 // columns of one score tile, so that shared keys are read once; the keys are cut into `splits` ranges for workgroups to fill the
 // chip, and a range is dealt 32 keys at a time to 4 waves that keep their own maximum, sum and output and join at the end.
 // K fragments go from memory to registers (a lane reads the 16 bytes it needs), V through a wave's own LDS rows to be transposed:
-// no barrier inside the loop, the next 32 keys in flight.  8 caches of 32768 slots, 2 x 128 wide, bf16 (201 MB): 44-48 us = 4.2-4.6
-// TB/s, the join 4.8 us.
+// no barrier inside the loop, the next 32 keys in flight.  8 caches of 32768 slots, 2 x 128 wide, bf16, lengths drawn between half
+// and all (233 MB by the counters): 42 us = 5.5 TB/s (a plain read: 6.4), the join 4.7 us.
 template <class T, int DP>
 __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;

@@ -17,8 +17,10 @@
 // give equal bits.  (Adding the elements with LDS atomics took 53 cycles an instruction, one lane after the other: 16 of them a block
 // were as long as its matrix products.)
 //
-// Bound as the forward by matrix plus vector time: 3 products and 5 vector instructions a score.  4 x 1024 tokens, 8 heads of 64, fp16: 47 us; 2 x
-// 4080 causal, 16 heads of 128 on 4, bf16: 290-330 us = 580-660 TFLOP/s.
+// Bound as the forward by matrix plus vector time: 3 products and 5 vector instructions a score.  4 x 1024 tokens, 8 heads of 64, fp16: 43 us (one
+// wave a SIMD, waiting 41 % of its time); 2 x 4080 causal, 16 heads of 128 on 4, bf16: 261 us = 785 TFLOP/s.  With the table's gradient five lines
+// and the skewed blocks share a CU's LDS: beyond a reach of 280 (bidirectional; 560 one-sided) a CU holds one workgroup instead of two, 8 x 2048, 16
+// heads of 64, bf16: 303 us at max_distance 256, 509 at 512, 585 at 1024.
 template <class T, int DP, bool TABLE>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;
@@ -256,8 +258,8 @@ __device__ __forceinline__ void sum_table(const AttnArgs& a, int h, double* red)
 // few workgroups (attn_apart says how few) each head of a group gets workgroups of its own, which write fp32 partial sums [2][B][Nk][H][D] that
 // attn_heads_kernel adds in order.  The tiles with most queries come first.
 //
-// Bound as above, 4 products a score.  4 x 1024 tokens, 8 heads of 64, fp16: 48 us; 2 x 4080 causal, 16 heads of 128 on 4, bf16: 380-440 us =
-// 580-670 TFLOP/s, attn_heads_kernel 23 us (150 MB, part of them still in the last cache).
+// Bound as above, 4 products a score.  4 x 1024 tokens, 8 heads of 64, fp16: 45 us (one wave a SIMD, waiting 40 % of its time); 2 x 4080
+// causal, 16 heads of 128 on 4, bf16: 336 us = 812 TFLOP/s, attn_heads_kernel 23 us (150 MB, part of them still in the last cache).
 template <class T, int DP>
 __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(AttnArgs a) {
     typedef typename Mma<T>::v8 v8;

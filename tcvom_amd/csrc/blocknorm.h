@@ -1,9 +1,11 @@
 // Norms around a block, shared by blocknorm.hip (forward) and blocknorm_bwd.hip:
 //     x' = residual_scale x + branch_scale g N1(y),    h = N2(x')
 // N = RMSNorm (t r w, r = 1 / sqrt(mean t^2 + eps)) or LayerNorm ((t - m) r w + b).  Bound: HBM bytes -- x, y in and x', h out once
-// forward (x, y, dx', dh in and dx, dy out backward), everything between in registers.  8192 rows of 4096, bf16: forward 49.5 us = 5.4 TB/s,
-// backward 82 us = 4.9 TB/s + 4.4 us for the column sums (a copy reaches 5.1); 8160 rows of 512, fp32 x and bf16 y: 12.6 us = 4.0 TB/s and
-// 18 us = 4.2 TB/s + 5.4 us; 4 rows of 4096: 4.1 us, a launch.
+// forward (x, y, dx', dh in and dx, dy out backward), everything between in registers.  8192 rows of 4096, bf16: forward 50 us = 5.3 TB/s,
+// backward 80 us = 5.0 TB/s + 4.0 us for the column sums (a copy reaches 5.1), all fp32: 100 and 166 us, the same rates; 8160 rows of 512, fp32 x
+// and bf16 y: 13 us = 3.8 TB/s and 17 us = 4.4 TB/s + 5.2 us; 4 rows of 4096: 3.9 us, a launch.  Channels just above a step of the launch tables
+// leave lanes idle: 131072 rows of 128 bf16 24 and 37 us (5.6 TB/s), of 136 52 and 74 us (2.8), of 256 75 and 82 us (3.6 and 4.9); 32768 rows of 512
+// 24 and 37 us, of 520 28 and 49 us (4.9 and 4.2).
 //
 // One row belongs to TPR threads, each with NV vectors of 8 channels: 16 lanes at <= 128 channels, up to 512 threads at 8192.  A
 // workgroup has R such row groups and walks its rows with the weights in registers.  TAIL: the channels are no multiple of 8; rows

@@ -12,7 +12,7 @@ enum { SUM_W1 = 0, SUM_B1, SUM_W2, SUM_B2, SUM_G, SUMS };
 
 // FULL: y, dx' and dh are all there and the channels a multiple of 8.  The loads of a row are then the same ones on every path (a row or
 // channel past the end reads the last one again), so that the compiler can count those in flight and wait for a row's own only; between
-// branches it waits for all (8192 rows of 4096, bf16: 90 us without, 82 us with).
+// branches it waits for all (8192 rows of 4096, bf16: 90 us without, 82 us with, at that step).
 template <class TX, class TY, int TPR, int R, int NV, bool TAIL, bool LAYER, bool FULL>
 __global__ __launch_bounds__(TPR * R, 2) void block_norm_bwd_kernel(NormArgs a) {
     constexpr int RED = TPR > 64 ? 4 * R * (TPR / 64) : 1;
@@ -61,7 +61,9 @@ __global__ __launch_bounds__(TPR * R, 2) void block_norm_bwd_kernel(NormArgs a) 
     // the next DEPTH rows' loads are in flight while this one's sums wait at their barriers
     constexpr int DEPTH = NV == 1 ? 2 : 1;
     constexpr bool AHEAD = NV == 1 || !LAYER;               // (16 channels a thread of LayerNorm leave no registers: 8192 x 6000
-                                                            // bf16 forward and backward 486 us reading ahead with spills, 286 us without)
+                                                            // bf16 forward and backward 486 us reading ahead, 280 us without.  Some of these widest
+                                                            // forms still spill: LayerNorm 7 registers, with an fp32 x 14, with odd channels or one
+                                                            // incoming gradient up to 66; RMS with an fp32 x 6 to 32)
     struct Raw {
         typename RawVec<TX, V>::type x[NV], dx[NV];
         typename RawVec<TY, V>::type y[NV], dh[NV];

@@ -5,7 +5,7 @@
 
 // ---- forward: a wave a row.  The head's line is formed once a workgroup in LDS; a 16-byte vector whose distances all lie past one end
 // of the line is a constant, the others look each element up.  8 x 2040 x 8160 bf16: 42 us = 6.3 TB/s (a fill reaches 6.9); 12 x 2041 x 2041
-// fp32: 33 us = 6.1 TB/s; 8 x 1024 x 1024 bf16: 8.4 us.
+// fp32: 33 us = 6.1 TB/s; 8 x 1024 x 1024 bf16: 8.1 us.
 template <class T>
 __global__ __launch_bounds__(256) void relbias_fwd_kernel(const float* table, T* out, tcvom_rel_buckets bk, int heads, long long Nq,
                                                           long long Nk, long long q_start, int rows_per_wg) {
@@ -79,8 +79,8 @@ extern "C" int tcvom_relbias_fwd(const float* table, void* out, const tcvom_rel_
 // Two kinds of workgroup in one launch (blockIdx.x): the BAND ones own 256 inner line entries each, a thread an entry: it walks the
 // rows of the chunk, its key moving one step a row, so that a wave reads consecutive elements; the FAR one (the last) sums what lies
 // past the two ends of the line, which is most of a long matrix, with 16-byte loads.  Each sum is made by one thread, or by a tree of
-// fixed shape, and written once: no atomics, equal calls give equal bits.  12 x 2041 x 2041 fp32: 62 us = 3.2 TB/s (a sum that only reads
-// reaches 3.9); 8 x 1024 x 1024 bf16: 7.1 us.  Chunks of 8, 32 or 64 rows: no faster.
+// fixed shape, and written once: no atomics, equal calls give equal bits.  12 x 2041 x 2041 fp32: 62 us = 3.2 TB/s, half of what a
+// plain read of as much reaches (30 us): the waves wait 61 % of their time, a row's far sums one after the other; 8 x 1024 x 1024 bf16: 6.9 us.  Chunks of 8, 32 or 64 rows: no faster.
 constexpr int BIAS_ROWS = 16;
 // chunks of rows are blocks of the grid's second dimension, and a bucket's entries of all chunks are counted in 32 bits
 static_assert(TCVOM_MAX_RELBIAS_BWD_QUERIES <= 65535 * BIAS_ROWS && TCVOM_MAX_RELBIAS_BWD_QUERIES / BIAS_ROWS * (TCVOM_MAX_BUCKET_REACH + 1LL) < (1LL << 31), "");
