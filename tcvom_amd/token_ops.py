@@ -97,16 +97,18 @@ def _first_order(backward):
     return run
 
 
-def _tracked(*tensors):
-    """Whether autograd has to see the call: for gradients, or to refuse forward-mode derivatives (dual tensors need no gradient and
-    have an address like others; torch raises NotImplementedError for a function without a rule for them, under no_grad too)."""
-    if forward_ad._current_level >= 0:
-        return True
+def _differentiated(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
     return False
+
+
+def _tracked(*tensors):
+    """Whether autograd has to see the call: for gradients, or to refuse forward-mode derivatives (dual tensors need no gradient and
+    have an address like others; torch raises NotImplementedError for a function without a rule for them, under no_grad too)."""
+    return forward_ad._current_level >= 0 or _differentiated(*tensors)
 
 
 # =============================================================================================
@@ -189,11 +191,10 @@ def relative_position_bias(table, q_len, k_len, max_distance=128, bidirectional=
     if not -(1 << 40) < q_start < 1 << 40:
         raise ValueError('relative_position_bias: q_start %d' % q_start)
     buckets = rel_buckets(table.shape[0], int(max_distance), bool(bidirectional))
-    tracked = _tracked(table)
-    if tracked and q_len > L.MAX_RELBIAS_BWD_QUERIES:
+    if q_len > L.MAX_RELBIAS_BWD_QUERIES and _differentiated(table):
         raise ValueError('relative_position_bias: %d queries with a gradient (at most %d)' % (q_len, L.MAX_RELBIAS_BWD_QUERIES))
     args = (table, buckets, int(q_len), int(k_len), int(q_start), dtype)
-    if not tracked:
+    if not _tracked(table):
         return _rel_bias(*args)
     out = _RelBias.apply(*args)
     _mark_leaves(table.get_device(), out)
@@ -281,8 +282,8 @@ def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causa
     new token against caches of Nk slots: k_lens = lengths with the new token, q_start = k_lens - 1, causal.
 
     Gradients of q, k, v and table.  Probabilities and their gradients are rounded to the 16-bit type as operands of the matrix
-    products (in fp16 times powers of two, so that a small dout loses no bits of them and a large one does not overflow), everything
-    else is held in 32 bits."""
+    products (in fp16 times powers of two, so that a small dout loses no bits of them and a large one does not overflow); where
+    the table needs no gradient, <dout, out> of dq and dk is formed from the rounded result.  Everything else is held in 32 bits."""
     name = 'biased_attention'
     q_starts = None
     if isinstance(q_start, torch.Tensor):
@@ -315,9 +316,9 @@ def biased_attention(q, k, v, table, max_distance=128, bidirectional=None, causa
         raise ValueError('%s: q_start %d' % (name, q_start))
     buckets = rel_buckets(table.shape[0], int(max_distance), bool(not causal if bidirectional is None else bidirectional))
     args = (buckets, int(causal), scale, _c(k_lens), key_mask, int(q_start), _c(q_starts))
+    if B * Hkv * -(-Nk // 128) + H > L.MAX_ATTN_WORKGROUPS and _differentiated(q, k, v, table):
+        raise ValueError('%s: %d sequences x %d key heads x %d keys with gradients (at most 2^30 rows of keys)' % (name, B, Hkv, Nk))
     if _tracked(q, k, v, table):
-        if B * Hkv * -(-Nk // 128) + H > L.MAX_ATTN_WORKGROUPS:
-            raise ValueError('%s: %d sequences x %d key heads x %d keys with gradients (at most 2^30 rows of keys)' % (name, B, Hkv, Nk))
         out = _BiasedAttention.apply(q, k, v, table, *args)
         _mark_leaves(q.get_device(), out)
         return out

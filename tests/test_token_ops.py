@@ -223,6 +223,11 @@ def test_what_the_gradient_cannot_do_is_refused_by_the_call(monkeypatch):
     ops.biased_attention(q, most, most, leaf)
     with pytest.raises(ValueError, match='with gradients'):
         ops.biased_attention(q, many, many, leaf)
+    with fwd.dual_level():                                   # (such calls pass through autograd, but nothing asks for a gradient)
+        ops.relative_position_bias(t, limit + 1, 1)
+        ops.biased_attention(q, many, many, t)
+        with torch.no_grad():
+            ops.relative_position_bias(leaf, limit + 1, 1)
 
 
 @pytest.mark.parametrize('kw,why', [(dict(B=1, Nq=1, Nk=1 << 25, H=64, Hkv=1, D=8), 'workspace'), (dict(B=4, Nq=1, Nk=1 << 28, H=2, Hkv=1, D=8), 'keys'),
