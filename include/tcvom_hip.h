@@ -713,7 +713,8 @@ int tcvom_relbias_bwd(const void* dout, float* dtable, float* work, int64_t work
  *     out[b,i,h] = sum_j softmax_j( scale <q[b,i,h], k[b,j,h Hkv / H]> + table[bucket(j - i - q_start_b)][h] ) v[b,j,h Hkv / H]
  * over the keys j < k_lens[b] (NULL: Nk) with key_mask[b][j] != 0 (NULL: all) and, causal, j <= i + q_start_b (q_starts[b], NULL: q_start).
  * A row without such a key is zero; what lies behind the lengths and under the mask is not looked at.  Finite
- * table entries count as at most 2^17 / log2(e) in size; -inf takes a distance out.  A HOST struct. */
+ * table entries count as at most 2^17 / log2(e) in size; -inf takes a distance out; those of distances that no row sees may hold
+ * anything.  A HOST struct. */
 typedef struct {
     int32_t B, Nq, Nk, H, Hkv, D, type, causal, q_start;
     float scale;                 /* > 0 */
